@@ -65,6 +65,10 @@ class RecordJob(C.Structure):
     _fields_ = [("src", ProjSrc * 3), ("rec", C.c_void_p)]
 
 
+class Fp8RecLayout(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("w1", "w3", "w2", "s1", "s3", "s2", "total")]
+
+
 class KernelStat(C.Structure):
     _fields_ = [("name", C.c_char * 40), ("launches", C.c_uint32), ("total_ms", C.c_float)]
 
@@ -109,6 +113,7 @@ def load() -> C.CDLL:
         "hb_a4_quant": (i, [vp, vp, i, i, i, vp, vp, vp, vp]),
         "hb_route_softmax_topk": (i, [vp, vp, i, i, i, i, i, i, vp, vp, vp]),
         "hb_route_sigmoid_topk": (i, [vp, vp, vp, i, i, i, f, vp, vp, vp]),
+        "hb_route_grouped_topk": (i, [vp, vp, i, i, i, i, i, i, i, i, vp, i, f, vp, vp, vp]),
         "hb_build_moe_pairs": (i, [vp, vp, vp, i, i, vp, i, i, vp, vp]),
         "hb_moe_combine": (i, [vp, vp, vp, vp, i, i, i, i, vp, vp]),
         "hb_moe_decode_supported": (i, [i, i]),
@@ -141,6 +146,13 @@ def load() -> C.CDLL:
         "hb_moe_prefill": (i, [vp, vp, i, i, vp, vp, i, i, vp, i, i, f, vp, vp, i, vp, C.POINTER(PfCombine)]),
         "hb_nvfp4_gemm_a4": (i, [vp, C.POINTER(QMat), vp, vp, vp, i, vp, i, vp]),
         "hb_fp4_peak_probe": (i, [vp, i, C.POINTER(f)]),
+        "hb_fp8_quant_rows": (i, [vp, vp, i, i, i, vp, i, vp, i, vp]),
+        "hb_fp8_quantize": (i, [vp, vp, i, i, i, vp, vp, vp]),
+        "hb_fp8_gemm_ws_bytes": (sz, [i, i, i]),
+        "hb_fp8_gemm": (i, [vp, C.POINTER(QMat), vp, i, vp, i, i, vp, vp, i, vp, vp]),
+        "hb_fp8_rec_layout_make": (i, [i, i, C.POINTER(Fp8RecLayout)]),
+        "hb_moe_fp8_ws_bytes": (sz, [i, i, i, i, i]),
+        "hb_moe_fp8": (i, [vp, vp, vp, i, i, vp, i, i, vp, i, i, f, vp, C.POINTER(PfCombine), vp, vp]),
         "hb_moe_layer_ws_bytes": (sz, [i, i, i, i, i]),
         "hb_moe_layer": (i, [vp, vp, i, i, i, i, i, i, vp, f, vp, i, vp, i, vp, i, i, f, vp, vp, vp, vp, vp]),
         "hb_dispatch_plan": (i, [vp, i, i, i, i, i, vp, C.POINTER(Plan)]),

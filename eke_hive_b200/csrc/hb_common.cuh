@@ -100,6 +100,9 @@ inline size_t hb_align256(size_t b) { return (b + 255) / 256 * 256; }
 inline bool hb_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ------------------------------------------------------------------------------------------------ device toolbox
+namespace hb {
+struct TileRef { int slot0, rows, expert; };   // consecutive slots of one expert's run of the sorted pairs, as many as a GEMM tile takes
+}  // namespace hb
 #ifdef __CUDACC__
 namespace hb {
 

@@ -24,6 +24,14 @@ bool hbk_moe_layer_a16_takes(const hb_ctx* ctx, int M, int K, int E, int H, int 
 int hbk_moe_layer_a16(hb_ctx* ctx, const uint8_t* const* lt, int E, const uint8_t* shared_rec, const int32_t* ids, const float* w, int M, int K, const void* x, int H,
                       int I, float limit, const float* lg, int ld, int col, void* out, void* ws, cudaStream_t st);
 int hbk_nvfp4_setup(hb_ctx* ctx);
+// the plan of a grouped GEMM (k_moe_prefill.cu): pairs sorted by expert, runs cut into tiles of equal size of at most bm pairs
+namespace hb { struct TileRef; }
+struct hbk_plan {
+  const int32_t* ids; int P, E; const uint8_t* const* tab; int bm;
+  int* hist; int* perm; int* pos_of; hb::TileRef* tiles; int* n_tiles; int* n_slots;
+};
+int hbk_pf_plan(hb_ctx* ctx, const hbk_plan& p, cudaStream_t st);
+size_t hbk_pf_plan_hist_bytes(int E);
 
 int hbk_route_softmax_topk(hb_ctx* ctx, const float* logits, int ld, int M, int E, int k, int renorm, int logits_bf16, int32_t* ids, float* w,
                            cudaStream_t st, bool pdl);

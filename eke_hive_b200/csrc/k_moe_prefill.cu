@@ -51,7 +51,6 @@ static_assert(PF_SF_COL0 + 48 * PF_ST <= PF_TMEM_COLS, "tensor memory");
 static_assert(PF_STAGE % 1024 == 0, "stage buffers must keep the 1024-byte alignment of the swizzle atom");
 static_assert(PF_SMEM <= 227 * 1024, "shared memory");
 
-struct TileRef { int slot0, rows, expert; };   // up to 128 consecutive slots of one expert's run of the sorted pairs (the bf16-activation GEMM: up to 64, 128 or 256)
 }  // namespace hb
 #include "pf_a16.cuh"
 namespace hb {
@@ -711,6 +710,15 @@ extern "C" __attribute__((visibility("default"))) int hb_a16_trace_read(long lon
   return (int)cudaMemcpyFromSymbol(out, g_a16_trace, (size_t)n * 8);
 }
 #endif
+
+int hbk_pf_plan(hb_ctx* ctx, const hbk_plan& p, cudaStream_t st) {
+  PlanArgs pl{p.ids, p.P, p.E, p.tab, p.bm, 1, p.hist, p.perm, p.pos_of, p.tiles, p.n_tiles, p.n_slots, reinterpret_cast<unsigned int*>(ctx->dev_err) + kErrPlanMeet, ctx->dev_err};
+  int ctas = (p.P + 2047) / 2048;
+  if (ctas > PLAN_MAX_CTAS) ctas = PLAN_MAX_CTAS;
+  if (ctas > ctx->sm_count) ctas = ctx->sm_count;                              // the CTAs meet inside the kernel: all must be resident
+  return hb_launch(ctx, "pf_plan", false, pf_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), 0, st, pl);
+}
+size_t hbk_pf_plan_hist_bytes(int E) { return (size_t)PLAN_MAX_CTAS * E * 4; }
 
 int hbk_moe_prefill_setup(hb_ctx* ctx) {
   HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(pf_gemm_kernel<PF_PLAIN>), cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM));

@@ -16,8 +16,8 @@ from . import _lib
 from ._lib import Config, HbError, MoePair, PfCombine, RecLayout
 
 __all__ = ["Context", "context", "ExpertRecLayout", "nvfp4_dequant", "nvfp4_gemv", "nvfp4_quantize", "requant_nvfp4", "a4_quant", "router_softmax_topk",
-           "router_topk", "build_moe_pairs", "moe_combine", "moe_decode_ws_bytes", "moe_decode", "fn_moe_decode_routed", "fn_moe_decode_routed_static", "static_max_pairs", "moe_decode_routed_f32", "moe_layer_decode",
-           "moe_decode_supported", "GMat", "dense_gemv", "dense_gemv_gu", "dense_gemv_ws_bytes", "lb_dequant", "dispatch_plan", "moe_layer", "moe_layer_ws_bytes", "PeerExchange", "moe_decode_ep_local", "moe_prefill_supported", "moe_prefill_ws_bytes", "fn_moe_prefill", "nvfp4_gemm_a4", "fp4_peak_probe", "FMT_NVFP4", "FMT_LB3_G64", "FMT_LB2_G64", "expert_dequant", "csf_decode", "record_pack", "record_pack_ws_bytes", "record_jobs", "record_pack_batch", "CSF_OK", "CSF_EXC_INDEX", "CSF_EXC_DELTA", "CSF_EXC_VALUE", "CSF_CODE", "gather_rows", "swiglu_rows", "scatter_add_rows", "add_f32", "make_pairs", "rec_table", "HbError"]
+           "router_topk", "router_grouped_topk", "build_moe_pairs", "moe_combine", "moe_decode_ws_bytes", "moe_decode", "fn_moe_decode_routed", "fn_moe_decode_routed_static", "static_max_pairs", "moe_decode_routed_f32", "moe_layer_decode",
+           "moe_decode_supported", "GMat", "dense_gemv", "dense_gemv_gu", "dense_gemv_ws_bytes", "lb_dequant", "dispatch_plan", "moe_layer", "moe_layer_ws_bytes", "PeerExchange", "moe_decode_ep_local", "moe_prefill_supported", "moe_prefill_ws_bytes", "fn_moe_prefill", "nvfp4_gemm_a4", "fp4_peak_probe", "fp8_quant_rows", "fp8_quantize", "fp8_gemm_ws_bytes", "fp8_gemm", "Fp8RecLayout", "fp8_record", "moe_fp8_ws_bytes", "moe_fp8", "FMT_NVFP4", "FMT_LB3_G64", "FMT_LB2_G64", "FMT_FP8_B128", "expert_dequant", "csf_decode", "record_pack", "record_pack_ws_bytes", "record_jobs", "record_pack_batch", "CSF_OK", "CSF_EXC_INDEX", "CSF_EXC_DELTA", "CSF_EXC_VALUE", "CSF_CODE", "gather_rows", "swiglu_rows", "scatter_add_rows", "add_f32", "make_pairs", "rec_table", "HbError"]
 
 
 def _L():
@@ -197,6 +197,20 @@ def router_topk(logits: torch.Tensor, bias: torch.Tensor | None, k: int, scale: 
     return ids, w
 
 
+def router_grouped_topk(logits: torch.Tensor, k: int, n_group: int = 1, topk_group: int = 1, group_top: int = 2, score: str = "sigmoid", bias=None,
+                        renorm: bool = True, scale: float = 1.0, E: int | None = None, ids=None, w=None, ctx: Context | None = None):
+    """hb_route_grouped_topk: top-k among the experts of the topk_group best of n_group groups; score "sigmoid" or "softmax", selection on
+    score + bias, weights from the score alone.  logits fp32 [M, ld]; returns ids int32 [M, k], w fp32 [M, k]."""
+    ctx = ctx or context()
+    M, ld = logits.shape[0], logits.stride(0)
+    E = logits.shape[1] if E is None else E
+    ids = torch.empty((M, k), dtype=torch.int32, device=logits.device) if ids is None else ids
+    w = torch.empty((M, k), dtype=torch.float32, device=logits.device) if w is None else w
+    ctx.check(_L().hb_route_grouped_topk(ctx.handle, _p(logits), ld, M, E, k, n_group, topk_group, group_top, {"softmax": 0, "sigmoid": 1}[score], _p(bias),
+                                         int(renorm), scale, _p(ids), _p(w), _stream()))
+    return ids, w
+
+
 def rec_table(recs: list[torch.Tensor | None]) -> torch.Tensor:
     """Device array of record pointers (int64), 0 for a missing record."""
     dev = next(r.device for r in recs if r is not None)
@@ -331,12 +345,13 @@ def moe_layer(logits, x, rec_tab, li: int, E: int, K: int, H: int, I: int, share
 
 
 # ---------------------------------------------------------------------------------------------------- dense GEMV (hb_qmat)
-FMT_NVFP4, FMT_LB3_G64, FMT_LB2_G64 = 0, 1, 2
+FMT_NVFP4, FMT_LB3_G64, FMT_LB2_G64, FMT_FP8_B128 = 0, 1, 2, 3
 
 
 class GMat:
     """hive::q27::GMat for the formats this library takes: device tensors of one [N, K] weight matrix.
-    NVFP4: w u8 [N, K/2], s u8 [N, K/16], g.  LB2/LB3: w u8 codes (LB3: low plane then high plane), s / zp fp16 [N, K/64]."""
+    NVFP4: w u8 [N, K/2], s u8 [N, K/16], g.  LB2/LB3: w u8 codes (LB3: low plane then high plane), s / zp fp16 [N, K/64].
+    FP8_B128 (fp8_gemm): w e4m3 codes [N, K], s fp32 [ceil(N/128), ceil(K/128)]."""
 
     def __init__(self, fmt: int, N: int, K: int, w, s, zp=None, g: float = 1.0):
         from ._lib import QMat
@@ -373,6 +388,93 @@ def lb_dequant(W: GMat, out=None, ctx: Context | None = None):
     ctx = ctx or context()
     out = torch.empty((W.N, W.K), dtype=torch.bfloat16, device=W.w.device) if out is None else out
     ctx.check(_L().hb_lb_dequant(ctx.handle, C.byref(W.c), _p(out), _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------- 8-bit floats, a scale per block of 128
+def _rows(t):
+    assert t.stride(-1) == 1, "rows must be contiguous"
+    return t.stride(0)
+
+
+def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
+    """hb_fp8_quant_rows: x bf16 [M, K] → (codes u8 [M, K], scales fp32 [ceil(K/128), M])."""
+    ctx = ctx or context()
+    assert x.dtype == torch.bfloat16
+    M, K = x.shape
+    q = torch.empty((M, K), dtype=torch.uint8, device=x.device) if q is None else q
+    s = torch.empty((-(-K // 128), M), dtype=torch.float32, device=x.device) if s is None else s
+    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, _p(x), _rows(x), M, K, _p(q), _rows(q), _p(s), _rows(s), _stream()))
+    return q, s
+
+
+def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
+    """hb_fp8_quantize: a weight fp32 or bf16 [N, K] → (codes u8 [N, K], scales fp32 [ceil(N/128), ceil(K/128)])."""
+    ctx = ctx or context()
+    assert w.dtype in (torch.float32, torch.bfloat16) and w.is_contiguous()
+    N, K = w.shape
+    q = torch.empty((N, K), dtype=torch.uint8, device=w.device) if q is None else q
+    s = torch.empty((-(-N // 128), -(-K // 128)), dtype=torch.float32, device=w.device) if s is None else s
+    ctx.check(_L().hb_fp8_quantize(ctx.handle, _p(w), int(w.dtype == torch.bfloat16), N, K, _p(q), _p(s), _stream()))
+    return q, s
+
+
+def fp8_gemm_ws_bytes(M: int, N: int, K: int) -> int:
+    return int(_L().hb_fp8_gemm_ws_bytes(M, N, K))
+
+
+def fp8_gemm(W: GMat, xq, xs, out_dtype=torch.bfloat16, y=None, ws=None, ctx: Context | None = None):
+    """hb_fp8_gemm: y [M, N] (bf16 or fp32) = rows quantised by fp8_quant_rows times the block-scaled matrix W (FMT_FP8_B128)."""
+    ctx = ctx or context()
+    M = xq.shape[0]
+    y = torch.empty((M, W.N), dtype=out_dtype, device=xq.device) if y is None else y
+    ws = torch.empty(fp8_gemm_ws_bytes(M, W.N, W.K), dtype=torch.uint8, device=xq.device) if ws is None else ws
+    yb, yf = (_p(y), None) if y.dtype == torch.bfloat16 else (None, _p(y))
+    ctx.check(_L().hb_fp8_gemm(ctx.handle, C.byref(W.c), _p(xq), _rows(xq), _p(xs), _rows(xs), M, yb, yf, _rows(y), _p(ws), _stream()))
+    return y
+
+
+class Fp8RecLayout:
+    """hb_fp8_rec_layout: byte offsets of an FP8 expert record."""
+
+    def __init__(self, H: int, I: int):
+        from ._lib import Fp8RecLayout as R
+        r = R()
+        st = _L().hb_fp8_rec_layout_make(H, I, C.byref(r))
+        if st != 0:
+            raise HbError(st, f"bad expert shape H={H} I={I} (multiples of 128)")
+        self.H, self.I = H, I
+        for n, _ in R._fields_:
+            setattr(self, n, int(getattr(r, n)))
+
+
+def fp8_record(H: int, I: int, gate, up, down, out=None):
+    """One expert's record (u8 tensor of Fp8RecLayout(H, I).total bytes) from its (codes, scales) pairs as fp8_quantize gives them."""
+    L = Fp8RecLayout(H, I)
+    out = torch.zeros(L.total, dtype=torch.uint8, device=gate[0].device) if out is None else out
+    for (q, s), w0, s0, n in ((gate, L.w1, L.s1, (I, H)), (up, L.w3, L.s3, (I, H)), (down, L.w2, L.s2, (H, I))):
+        assert tuple(q.shape) == n and tuple(s.shape) == (n[0] // 128, n[1] // 128) and s.dtype == torch.float32
+        out[w0:w0 + q.numel()] = q.contiguous().view(torch.uint8).view(-1)
+        out[s0:s0 + 4 * s.numel()] = s.contiguous().view(-1).view(torch.uint8)
+    return out
+
+
+def moe_fp8_ws_bytes(M: int, K: int, E: int, H: int, I: int) -> int:
+    return int(_L().hb_moe_fp8_ws_bytes(M, K, E, H, I))
+
+
+def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg=None, col: int = 0, limit: float = 0.0, out=None, out_dtype=torch.bfloat16,
+            ws=None, ctx: Context | None = None):
+    """hb_moe_fp8: routed experts of FP8 records for any number of rows; ids int32 / w fp32 [M, K], x bf16 [M, H].  bf16 out adds the gated shared
+    rows where given; out_dtype (or out.dtype) float32 gives the routed sum alone."""
+    ctx = ctx or context()
+    M, K = ids.shape
+    assert x.is_contiguous() and ids.is_contiguous() and w.is_contiguous()
+    out = torch.empty((M, H), dtype=out_dtype, device=x.device) if out is None else out
+    ws = torch.empty(moe_fp8_ws_bytes(M, K, E, H, I), dtype=torch.uint8, device=x.device) if ws is None else ws
+    assert out.dtype == torch.bfloat16 or (shared is None and lg is None), "shared rows are added to a bf16 output"
+    cmb = C.byref(PfCombine(_p(shared), _p(lg), 0 if lg is None else lg.stride(0), col, _p(out))) if out.dtype == torch.bfloat16 else None
+    ctx.check(_L().hb_moe_fp8(ctx.handle, _p(ids), _p(w), M, K, _p(rec_tab), li, E, _p(x), H, I, limit, None if cmb else _p(out), cmb, _p(ws), _stream()))
     return out
 
 

@@ -89,15 +89,16 @@ typedef struct hb_pf_combine {
 } hb_pf_combine;
 
 /* Dense weight matrix of the 27B-style decode GEMV — stands in for hive::q27::GMat (engine/include/hive/q27/q27_kernels.h:17-36). */
-typedef enum hb_wfmt { HB_FMT_NVFP4 = 0, HB_FMT_LB3_G64 = 1, HB_FMT_LB2_G64 = 2 } hb_wfmt;
+typedef enum hb_wfmt { HB_FMT_NVFP4 = 0, HB_FMT_LB3_G64 = 1, HB_FMT_LB2_G64 = 2, HB_FMT_FP8_B128 = 3 /* hb_fp8_gemm only */ } hb_wfmt;
 typedef struct hb_qmat {
   int fmt;            /* hb_wfmt */
   int N, K;           /* out × in */
   const uint8_t* w;   /* NVFP4: e2m1 [N,K/2].  LB2: codes [N,K/4] (4 per byte, low bits first).
-                         LB3: low-two-bit plane [N,K/4] followed by the high-bit plane [N,K/8] (8 per byte, low bit first). */
-  const void* s;      /* NVFP4: e4m3 [N,K/16].  LB*: fp16 [N,K/64] */
+                         LB3: low-two-bit plane [N,K/4] followed by the high-bit plane [N,K/8] (8 per byte, low bit first).
+                         FP8_B128: e4m3 [N,K] */
+  const void* s;      /* NVFP4: e4m3 [N,K/16].  LB*: fp16 [N,K/64].  FP8_B128: fp32 [ceil(N/128), ceil(K/128)], value = code · s of its 128 × 128 block */
   const void* zp;     /* LB*: fp16 zero-points [N,K/64]; value = (q - zp) * s.  NVFP4: NULL */
-  float g;            /* NVFP4 per-tensor scale (multiplies); LB*: ignored */
+  float g;            /* NVFP4 per-tensor scale (multiplies); other formats: ignored */
 } hb_qmat;
 
 /* ---- context (house style of the reference's C ABIs: engine/include/hive/qtts/qtts_capi.h:4-35) ---- */
@@ -152,6 +153,19 @@ HB_API int hb_route_softmax_topk(hb_ctx* ctx, const float* logits, int ld, int M
 /* hive::glm::router_topk — engine/include/hive/glm/glm_kernels.h:12-17, engine/src/glm/glm_kernels.cu:35-53 */
 HB_API int hb_route_sigmoid_topk(hb_ctx* ctx, const float* logits, const float* bias, int M, int E, int k, float scale, int32_t* ids,
                                  float* w, void* stream);
+/* (No counterpart in the reference.)  Routing limited to groups of experts, the general router of this library's two score functions.  Per
+ * row of logits l (fp32 [M,ld], columns 0..E-1):
+ *   s = sigmoid(l) or softmax(l) over the E experts;  c = s + bias (fp32 [E], NULL = none): the bias balances the load, it picks but does not weigh;
+ *   the E experts are n_group runs of E / n_group; a group's value is the sum of its group_top (1 or 2) largest c; the topk_group groups of
+ *   the largest values stay;  the k experts of the largest c among theirs are picked, best first;
+ *   w = s of the pick, divided by (the picks' sum + 1e-20) when renorm, times scale.
+ * Ties go to the smaller index, for groups and for experts.  The selection is that of 64-bit arithmetic: experts whose scores differ by less than
+ * fp32 resolves are still told apart.  A logit of -inf has score 0, NaN counts as -inf, a softmax row with nothing but those has all scores 0;
+ * ids are always k different experts of the groups kept.  +inf is not accepted by the softmax (its weights are then NaN).
+ * E ≤ 1024, k ≤ 16, n_group ≤ 32 a divisor of E (1: no groups), k ≤ topk_group · E / n_group.  M = 0 does nothing. */
+enum { HB_SCORE_SOFTMAX = 0, HB_SCORE_SIGMOID = 1 };
+HB_API int hb_route_grouped_topk(hb_ctx* ctx, const float* logits, int ld, int M, int E, int k, int n_group, int topk_group, int group_top, int score,
+                                 const float* bias, int renorm, float scale, int32_t* ids, float* w, void* stream);
 /* hive::qwen::build_moe_pairs — engine/include/hive/qwen/qwen_kernels.h:63-66 */
 HB_API int hb_build_moe_pairs(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, const uint8_t* const* rec_tab, int li, int E,
                               hb_moe_pair* pairs, void* stream);
@@ -292,6 +306,45 @@ HB_API int hb_nvfp4_gemm_a4(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, co
 /* Measures the FP4 tensor-pipe ceiling of the device: every SM issues `rounds`×4 block-scaled 128×256×64 MMAs on operands held in
  * shared memory (no loads, no epilogue); *tflops = dense FP4 TFLOP/s.  Synchronises the device.  (No reference counterpart.) */
 HB_API int hb_fp4_peak_probe(hb_ctx* ctx, int rounds, float* tflops);
+
+/* ---- 8-bit floats with a scale per block of 128 (e4m3 codes, fp32 scales) ----
+ * The format of the reference's FP8 expert and shared-expert matrices (engine/include/hive/glm/glm_moe_fp8.h:24-43): a weight [N,K] is e4m3 codes
+ * with one fp32 scale per 128 × 128 block.  Activations are quantised on the way into a product: e4m3 codes with one fp32 scale per
+ * row and 128 values of K.  K is a multiple of 16 throughout; the last block of a row may be short.
+ *
+ * Quantisation of a block (both kinds): amax = its largest magnitude, s = amax / 448, code = e4m3(v · 448 / amax) to the nearest code, ties to the
+ * even one; the product and the quotient are fp32 (for bf16 input the code is then the one nearest to the exact quotient).  A block of zeros has s = 0
+ * and codes 0.
+ * A block that holds an infinity or a NaN has s = NaN, codes 0: whatever is computed from it is NaN.
+ *
+ * hb_fp8_quant_rows: x bf16 [M,K] (row stride ldx elements) → q [M,K] (row stride ldq bytes, a multiple of 16) and s fp32 [ceil(K/128)][lds], lds ≥ M:
+ * the scales of one block of K for consecutive rows lie next to each other.  q 16-byte aligned, x 2-byte (16-byte and ldx % 8 == 0 is faster).
+ * hb_fp8_quantize: w fp32 (bf16 == 0) or bf16 (bf16 != 0) [N,K], dense, 16-byte aligned → q [N,K], s fp32 [ceil(N/128), ceil(K/128)]. */
+HB_API int hb_fp8_quant_rows(hb_ctx* ctx, const void* x_bf16, int ldx, int M, int K, uint8_t* q, int ldq, float* s, int lds, void* stream);
+HB_API int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t* q, float* s, void* stream);
+/* y[m,n] = Σ_b xs[b,m]·W.s[n/128,b]·Σ_{k in block b} xq[m,k]·W.w[n,k], written as bf16 (yb) or fp32 (yf): exactly one non-NULL, row stride ldy
+ * elements.  W of format HB_FMT_FP8_B128; xq / xs as hb_fp8_quant_rows writes them.  M ≥ 0 (0 does nothing) from one token to prompt chunks,
+ * any N.  Products are exact, sums fp32.  xq and W.w 16-byte aligned.  ws ≥ hb_fp8_gemm_ws_bytes(M, N, K), 256-byte aligned. */
+HB_API size_t hb_fp8_gemm_ws_bytes(int M, int N, int K);
+HB_API int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb_bf16, float* yf, int ldy, void* ws,
+                       void* stream);
+/* An expert of such weights as one record: codes of gate w1 [I,H], up w3 [I,H], down w2 [H,I], then their scales s1, s3 [I/128,H/128],
+ * s2 [H/128,I/128], to a multiple of 4096 bytes.  H and I multiples of 128. */
+typedef struct hb_fp8_rec_layout {
+  uint64_t w1, w3, w2, s1, s3, s2, total;
+} hb_fp8_rec_layout;
+HB_API int hb_fp8_rec_layout_make(int H, int I, hb_fp8_rec_layout* out);
+/* Routed experts of FP8 records for any number of rows (the operator of engine/include/hive/qwen/fn_moe.h:38-41 with 8-bit activations): per pair
+ * (row m, expert ids[m,k]) x[m] is quantised by hb_fp8_quant_rows' rule, g and u are its products with w1 and w3 (fp32), y = silu(g)·u (limit > 0:
+ * g ≤ limit, |u| ≤ limit first) is quantised by the same rule, d = bf16 of its product with w2, and
+ *   routed[m] = Σ_k w[m,k]·d (fp32, in k order).
+ * cmb == NULL: out fp32 [M,H] = routed.  Else cmb->out bf16 [M,H] = bf16(routed + gate·shared[m]), gate = sigmoid(lg[m·ld + col]) or 1 where
+ * cmb->lg is NULL, no shared term where cmb->shared is NULL; `out` is not used.  Records come from rec_tab[li·E + id] (16-byte aligned); ids outside
+ * [0,E) and NULL records contribute nothing.  A row's result does not depend on the rows beside it beyond fp32 summation order.
+ * E ≤ 1024, K ≤ 32, M·K < 2^30.  ws ≥ hb_moe_fp8_ws_bytes(M, K, E, H, I), 256-byte aligned. */
+HB_API size_t hb_moe_fp8_ws_bytes(int M, int K, int E, int H, int I);
+HB_API int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, const uint8_t* const* rec_tab, int li, int E, const void* x_bf16, int H, int I,
+                      float limit, float* out, const hb_pf_combine* cmb, void* ws, void* stream);
 
 /* ---- a whole MoE layer for any number of rows (the expert-dispatch scheduler) ---- */
 /* router → routed experts → always-on shared expert (one more NVFP4 record, NULL = none) → combine, like hb_moe_layer_decode, for

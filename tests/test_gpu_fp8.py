@@ -1,0 +1,359 @@
+"""GPU parity of the 8-bit block-scaled operators: quantisers (codes equal to the exact rule's), the product, the routed experts, against 64-bit forms."""
+import numpy as np
+import pytest
+
+import fp8_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def E():
+    import eke_hive_b200 as E
+    return E
+
+
+def gen(seed):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def rows(M, K, seed, ld=None):
+    """bf16 rows whose blocks have very different sizes, among them blocks of zeros."""
+    import torch
+    g = gen(seed)
+    x = torch.randn(M, ld or K, device="cuda", generator=g)
+    x = x * torch.exp2(torch.randint(-12, 12, (M, -(-(ld or K) // 128)), device="cuda", generator=g).float()).repeat_interleave(128, 1)[:, :(ld or K)]
+    x[torch.rand(x.shape, device="cuda", generator=g) < 0.05] = 0.0
+    x = x.to(torch.bfloat16)
+    x[M // 2, :128] = 0.0
+    return x[:, :K]
+
+
+def matrix(N, K, seed):
+    import torch
+    g = gen(seed)
+    q = (torch.randn(N, K, device="cuda", generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    s = (torch.rand(R.up(N), R.up(K), device="cuda", generator=g) + 0.5) * 2e-4
+    return q, s
+
+
+def record(E, H, I, seed, at=0):
+    """A record in a buffer of its own, `at` bytes (a multiple of 16) behind a 4096-byte boundary, and its parts in 64 bits."""
+    import torch
+    mats = [matrix(I, H, seed), matrix(I, H, seed + 1), matrix(H, I, seed + 2)]
+    buf = torch.zeros(E.Fp8RecLayout(H, I).total + at, dtype=torch.uint8, device="cuda")
+    return E.fp8_record(H, I, *mats, out=buf[at:]), [(q.double(), s.double()) for q, s in mats]
+
+
+# ---------------------------------------------------------------------------------------------------- quantisers
+@pytest.mark.parametrize("M,K,ld", [(1, 128, None), (1, 16, None), (3, 2048, None), (67, 1552, None), (5, 400, 408), (9, 272, 275), (513, 7168, None), (2, 17408, None)])
+def test_quant_rows_is_exact(E, M, K, ld):
+    import torch
+    x = rows(M, K, M + K, ld)
+    q, s = E.fp8_quant_rows(x)
+    q0, s0 = R.quant_rows(x.double())
+    assert torch.equal(R.codes_to_f64(q), q0)
+    assert torch.equal(s.double(), s0)
+
+
+def test_quant_rows_every_bf16_quotient_border(E):
+    """All pairs (amax, v) of bf16 mantissas, signs and a few exponents: ties between codes are seen as ties."""
+    import torch
+    man = 1.0 + torch.arange(128, device="cuda").float() / 128
+    x = torch.zeros(128, 8, 128, device="cuda")
+    for j, e in enumerate((0, -1, -2, -3, -5, -8, -10, -14)):
+        x[:, j, :] = man[None, :] * 2.0 ** e * torch.where(torch.arange(128, device="cuda") % 2 == 0, 1.0, -1.0)
+    x = torch.where(x.abs() > man[:, None, None], 0.5 * x, x)
+    x[:, :, 0] = man[:, None]
+    for scale in (1.0, 2.0 ** 100, 2.0 ** -100, 2.0 ** 126, 2.0 ** -120):
+        xb = (x.reshape(128, 1024) * scale).to(torch.bfloat16)
+        q, s = E.fp8_quant_rows(xb)
+        q0, s0 = R.quant_rows(xb.double())
+        assert torch.equal(R.codes_to_f64(q), q0), scale
+        assert torch.equal(s.double(), s0), scale
+
+
+def test_quant_rows_non_finite_blocks(E):
+    import torch
+    x = torch.randn(4, 512, device="cuda").to(torch.bfloat16)
+    x[0, 5] = float("nan"); x[1, 200] = float("inf"); x[2, 500] = -float("inf")
+    q, s = E.fp8_quant_rows(x)
+    nan = torch.isnan(s)
+    assert nan.nonzero().tolist() == [[0, 0], [1, 1], [3, 2]]
+    assert (q[0, :128] == 0).all() and (q[1, 128:256] == 0).all() and (q[2, 384:] == 0).all()
+    ok = E.fp8_quant_rows(x[3:4])
+    assert torch.equal(q[3], ok[0][0]) and torch.equal(s[:, 3], ok[1][:, 0])
+    W = matrix(130, 512, 3)
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, 130, 512, *W), q, s)
+    assert torch.isnan(y[:3]).all() and torch.isfinite(y[3]).all()
+
+
+def test_quant_rows_strides_and_rows_behind_the_last(E):
+    import torch
+    x = rows(5, 320, 1, 333)
+    q = torch.full((8, 400), 0x55, dtype=torch.uint8, device="cuda")
+    s = torch.full((3, 9), -7.0, device="cuda")
+    E.fp8_quant_rows(x, q=q[:5, :320], s=s[:, :5])
+    q0, s0 = E.fp8_quant_rows(x.contiguous())
+    assert torch.equal(q[:5, :320], q0) and torch.equal(s[:, :5], s0)
+    assert (q[5:] == 0x55).all() and (q[:, 320:] == 0x55).all() and (s[:, 5:] == -7).all()
+
+
+@pytest.mark.parametrize("N,K,dt", [(128, 128, "float32"), (1, 16, "float32"), (300, 1552, "float32"), (2111, 528, "bfloat16"), (129, 2048, "bfloat16"), (5120, 272, "float32")])
+def test_quantize_is_exact(E, N, K, dt):
+    import torch
+    w = (torch.randn(N, K, device="cuda", generator=gen(N)) * 0.02).to(getattr(torch, dt))
+    if N > 200:
+        w[:128, :128] = 0.0
+    q, s = E.fp8_quantize(w)
+    q0, s0 = R.quant_blocks(w)
+    assert torch.equal(R.codes_to_f64(q), q0)
+    assert torch.equal(s.double(), s0)
+
+
+# ---------------------------------------------------------------------------------------------------- the product
+GEMM = [(1, 128, 128), (1, 1, 16), (1, 5120, 2048), (2, 300, 400), (7, 4100, 1552), (13, 256, 7168), (16, 384, 640), (17, 130, 272), (33, 1000, 1024), (64, 512, 512), (65, 257, 2064),
+        (127, 640, 384), (128, 256, 256), (129, 255, 144), (200, 1500, 1000 // 16 * 16), (333, 513, 2048), (600, 260, 4096), (1030, 777, 528)]
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,N,K", GEMM)
+def test_gemm(E, M, N, K, dt):
+    import torch
+    q, s = matrix(N, K, N + K)
+    xq, xs = E.fp8_quant_rows(rows(M, K, M))
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q, s), xq, xs, out_dtype=getattr(torch, dt))
+    y0, a = R.gemm(R.codes_to_f64(xq), xs.double(), q.double(), s.double())
+    tol = R.sum_bound(K) * a
+    tol = tol + R.HALF[y.dtype] * (y0.abs() + tol)
+    bad = (y.double() - y0).abs() > tol
+    assert not bad.any(), (bad.sum().item(), bad.nonzero()[:4].tolist(), ((y.double() - y0).abs() / (a + 1e-300)).max().item())
+
+
+def test_gemm_strides_and_what_lies_around(E):
+    import torch
+    M, N, K = 37, 201, 336
+    q, s = matrix(N, K, 5)
+    W = E.GMat(E.FMT_FP8_B128, N, K, q, s)
+    xq, xs = E.fp8_quant_rows(rows(M, K, 6))
+    for dt in (torch.bfloat16, torch.float32):
+        ref = E.fp8_gemm(W, xq, xs, out_dtype=dt)
+        xq2 = torch.full((M + 3, 512), 0x7f, dtype=torch.uint8, device="cuda")          # NaN codes around the rows
+        xs2 = torch.full((3, M + 5), float("nan"), device="cuda")
+        y = torch.full((M + 2, 233), -7.0, dtype=dt, device="cuda")
+        xq2[:M, :K] = xq; xs2[:, :M] = xs
+        E.fp8_gemm(W, xq2[:M, :K], xs2[:, :M], y=y[:M, :N])
+        assert torch.equal(y[:M, :N], ref)
+        assert (y[M:] == -7).all() and (y[:, N:] == -7).all()
+
+
+def test_gemm_nan_codes_and_scales_stay_in_their_row_and_column(E):
+    import torch
+    M, N, K = 40, 300, 512
+    q, s = matrix(N, K, 5)
+    xq, xs = E.fp8_quant_rows(rows(M, K, 6))
+    ref = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q, s), xq, xs)
+    xq2, q2 = xq.clone(), q.clone()
+    xq2[3, 100] = 0x7f
+    q2.view(torch.uint8)[200, 7] = 0xff
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q2, s), xq2, xs)
+    nan = torch.isnan(y)
+    assert nan[3].all() and nan[:, 200].all() and nan.sum() == N + M - 1
+    assert torch.equal(y[~nan], ref[~nan])
+
+
+@pytest.mark.parametrize("N,K", [(5120, 2048), (640, 7168)])
+def test_gemm_twice_and_row_by_row(E, N, K):
+    """The same call gives the same bits."""
+    import torch
+    q, s = matrix(N, K, 9)
+    W = E.GMat(E.FMT_FP8_B128, N, K, q, s)
+    for M in (1, 5, 16, 40, 150):
+        xq, xs = E.fp8_quant_rows(rows(M, K, M))
+        a = E.fp8_gemm(W, xq, xs, out_dtype=torch.float32)
+        for _ in range(3):
+            assert torch.equal(a, E.fp8_gemm(W, xq, xs, out_dtype=torch.float32))
+
+
+def test_gemm_refusals(E):
+    import torch
+    q, s = matrix(64, 256, 1)
+    W = E.GMat(E.FMT_FP8_B128, 64, 256, q, s)
+    xq, xs = E.fp8_quant_rows(rows(4, 256, 2))
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(E.GMat(E.FMT_NVFP4, 64, 256, q, s), xq, xs)
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(E.GMat(E.FMT_FP8_B128, 64, 248, q, s), xq, xs)
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(W, xq[:, 8:], xs)                                                    # not 16-byte aligned
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(W, xq, xs, y=torch.empty(4, 60, device="cuda"))
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(W, xq, xs[:, :2].contiguous())                                       # fewer scales than rows
+    with pytest.raises(E.HbError):
+        E.fp8_gemm(W, xq, xs, ws=torch.empty(1024, dtype=torch.uint8, device="cuda")[8:])
+    with pytest.raises(E.HbError):
+        E.dense_gemv(W, rows(1, 256, 3), ws=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"))   # the bf16-activation GEMV has no such format
+    with pytest.raises(E.HbError):
+        E.fp8_quant_rows(rows(2, 264, 3))
+    assert E.fp8_gemm(W, xq[:0], xs[:, :0]).shape == (0, 64)
+    assert E.fp8_quant_rows(rows(4, 256, 2)[:0])[0].shape == (0, 256)
+
+
+# ---------------------------------------------------------------------------------------------------- routed experts
+def routing(M, K, Ex, seed, hot=None):
+    import torch
+    rng = np.random.default_rng(seed)
+    ids = np.stack([rng.permutation(Ex)[:K] for _ in range(M)]).astype(np.int32)
+    if hot is not None:
+        ids[:, 0] = hot
+        ids[:, 1:][ids[:, 1:] == hot] = (hot + 1) % Ex
+    return torch.from_numpy(ids).cuda(), torch.from_numpy(rng.uniform(0.05, 0.6, (M, K)).astype(np.float32)).cuda()
+
+
+def moe_check(E, M, H, I, Ex, K, seed, limit=0.0, hot=None, missing=(), shared=True, gate=True, edit=None):
+    import torch
+    recs = [record(E, H, I, 10 * e + seed, at=16 * (e % 7)) for e in range(Ex)]
+    tab = torch.tensor([0 if e in missing else r[0].data_ptr() for e, r in enumerate(recs)], dtype=torch.int64, device="cuda")
+    ref = [None if e in missing else r[1] for e, r in enumerate(recs)]
+    x = (torch.randn(M, H, device="cuda", generator=gen(seed)) * 2).to(torch.bfloat16)
+    ids, w = routing(M, K, Ex, seed, hot)
+    if edit:
+        edit(ids)
+    sh = (torch.randn(M, H, device="cuda", generator=gen(seed + 1)) * 0.3).to(torch.bfloat16)
+    lg = torch.randn(M, 3, device="cuda", generator=gen(seed + 2))
+    o0, tol, mag = R.moe(ids, w, ref, x, limit)
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, limit=limit, out_dtype=torch.float32)
+    err = (out.double() - o0).abs()
+    assert (err <= tol + 1e-30).all(), ((err / (tol + 1e-30)).max().item(), (err > tol).sum().item())
+    # tol adds up every rounding at its worst.  Over all outputs they do not conspire: d's rounding is off by 2^-8 of it at most, a code of y that falls the
+    # other way (one in 2^16, where g and u are off by 2^-20) by 2^-3 of a value, 2^-11 of d; twice the first covers both
+    assert err.norm() <= 2.0 ** -7 * mag.norm()
+    s0, stol, _ = R.moe(ids, w, ref, x, limit, sh if shared else None, lg[:, 1] if gate else None)
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, shared=sh if shared else None, lg=lg if shared and gate else None, col=1, limit=limit)
+    stol = stol + R.HALF[torch.bfloat16] * (s0.abs() + stol)
+    err = (out.double() - s0).abs()
+    assert (err <= stol + 1e-30).all(), (err / (stol + 1e-30)).max().item()
+    assert torch.equal(out, E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, shared=sh if shared else None, lg=lg if shared and gate else None, col=1, limit=limit))
+    return out
+
+
+@pytest.mark.parametrize("M,H,I,Ex,K", [(1, 128, 128, 1, 1), (1, 2048, 512, 12, 10), (2, 256, 384, 6, 3), (5, 640, 256, 4, 4), (16, 2048, 512, 32, 10), (17, 512, 128, 3, 2), (40, 384, 640, 5, 4),
+                                        (64, 1024, 256, 8, 8), (65, 256, 256, 2, 1), (130, 512, 384, 9, 4), (300, 256, 512, 2, 2), (700, 384, 256, 16, 5)])
+def test_moe(E, M, H, I, Ex, K):
+    moe_check(E, M, H, I, Ex, K, M + H)
+
+
+def test_moe_limit_and_gateless_shared(E):
+    moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
+    moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
+
+
+def test_moe_hot_expert_missing_records_and_invalid_ids(E):
+    import torch
+
+    def edit(ids):
+        ids[0, 1] = -1; ids[1, 0] = 7; ids[2, :] = -1; ids[3, :] = 1000                 # a row that nothing is left of, ids outside the table
+    moe_check(E, 150, 256, 256, 7, 3, 3, hot=2, missing=(4,), edit=edit)
+    moe_check(E, 12, 256, 256, 7, 3, 4, hot=2, missing=(4, 5), edit=edit)
+    out = moe_check(E, 6, 256, 128, 5, 2, 5, missing=(0, 1, 2, 3, 4), shared=False)     # no record at all: nothing is added
+    assert (out == 0).all()
+
+
+def test_moe_the_same_expert_twice_in_a_row(E):
+    def edit(ids):
+        ids[:, 1] = ids[:, 0]
+    moe_check(E, 30, 256, 128, 5, 3, 6, edit=edit)
+
+
+def test_moe_rows_behind_the_last_and_layers(E):
+    import torch
+    H, I, Ex, K, M = 256, 256, 4, 2, 21
+    recs = [record(E, H, I, 100 + e) for e in range(3 * Ex)]
+    tab = E.rec_table([r[0] for r in recs])
+    x = torch.randn(M, H, device="cuda", generator=gen(1)).to(torch.bfloat16)
+    ids, w = routing(M, K, Ex, 2)
+    for li in range(3):
+        o0, tol, _ = R.moe(ids, w, [r[1] for r in recs[li * Ex:(li + 1) * Ex]], x)
+        out = torch.full((M + 4, H), -7.0, device="cuda")
+        E.moe_fp8(ids, w, tab, li, Ex, x, H, I, out=out[:M])
+        assert ((out[:M].double() - o0).abs() <= tol).all() and (out[M:] == -7).all()
+
+
+def test_moe_refusals(E):
+    import torch
+    x = torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda")
+    ids, w = routing(2, 2, 4, 1)
+    tab = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for H, I in ((192, 256), (256, 192), (0, 128)):
+        with pytest.raises(E.HbError):
+            E.moe_fp8(ids, w, tab, 0, 4, x, H, I, out=torch.empty(2, 256, device="cuda"), ws=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(E.HbError):
+        E.moe_fp8(ids, w, tab, 0, 1025, x, 256, 256)
+    with pytest.raises(E.HbError):
+        E.moe_fp8(ids, w, tab, -1, 4, x, 256, 256)
+    with pytest.raises(E.HbError):
+        E.moe_fp8(ids, w, tab, 0, 4, x, 256, 256, ws=torch.empty(1 << 22, dtype=torch.uint8, device="cuda")[16:])
+    with pytest.raises(E.HbError):
+        E.Fp8RecLayout(200, 128)
+    assert E.moe_fp8(ids[:0], w[:0], tab, 0, 4, x[:0], 256, 256).shape == (0, 256)
+
+
+# ---------------------------------------------------------------------------------------------------- together
+def layer(E, lg, bias, x, tab, Ex, H, I, Wsh, K):
+    """Router, routed experts, a dense matrix for every row beside them."""
+    ids, w = E.router_grouped_topk(lg, K, 4, 2, bias=bias, scale=2.5)
+    sh = E.fp8_gemm(Wsh, *E.fp8_quant_rows(x))
+    return ids, w, E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, shared=sh)
+
+
+@pytest.mark.parametrize("M", [1, 11, 90])
+def test_layer_on_streams_and_in_graphs(E, M):
+    """Weights quantised here, routed, multiplied and summed; the same on another stream and replayed from a captured graph with other inputs."""
+    import torch
+    H, I, Ex, K = 512, 256, 16, 4
+    g = gen(M)
+    recs = [E.fp8_record(H, I, *(E.fp8_quantize(torch.randn(n, k, device="cuda", generator=g) * 0.05) for n, k in ((I, H), (I, H), (H, I)))) for _ in range(Ex)]
+    tab = E.rec_table(recs)
+    Wsh = E.GMat(E.FMT_FP8_B128, H, H, *E.fp8_quantize((torch.randn(H, H, device="cuda", generator=g) * 0.05).to(torch.bfloat16)))
+    bias = torch.randn(Ex, device="cuda", generator=g) * 0.05
+    ins = [(torch.randn(M, Ex, device="cuda", generator=g), torch.randn(M, H, device="cuda", generator=g).to(torch.bfloat16)) for _ in range(3)]
+    ref = [layer(E, lg, bias, x, tab, Ex, H, I, Wsh, K) for lg, x in ins]
+    L = E.Fp8RecLayout(H, I)
+    parts = []
+    for r in recs:
+        parts.append([(r[a:a + n * k].view(torch.float8_e4m3fn).view(n, k).double(), r[b:b + n * k // 4096].view(torch.float32).view(n // 128, k // 128).double())
+                      for a, b, n, k in ((L.w1, L.s1, I, H), (L.w3, L.s3, I, H), (L.w2, L.s2, H, I))])
+    for (lg, x), (ids, w, out) in zip(ins, ref):
+        i0, _ = R.route(lg.cpu().numpy(), bias.cpu().numpy(), K, 4, 2, 2, "sigmoid", True, 2.5)
+        assert np.array_equal(ids.cpu().numpy(), i0)
+        xq, xs = R.quant_rows(x.double())
+        s0, a = R.gemm(xq, xs, Wsh.w.view(torch.float8_e4m3fn).double(), Wsh.s.double())
+        o0, tol, _ = R.moe(ids, w, parts, x)
+        tol = tol + R.sum_bound(H) * a + 2.0 ** -8 * s0.abs()
+        o0 = o0 + s0
+        assert ((out.double() - o0).abs() <= tol + 2.0 ** -8 * (o0.abs() + tol)).all()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for (lg, x), r in zip(ins, ref):
+            got = layer(E, lg, bias, x, tab, Ex, H, I, Wsh, K)
+            assert all(torch.equal(a, b) for a, b in zip(got, r))
+    torch.cuda.current_stream().wait_stream(st)
+    graphs = []
+    for _ in range(2):                                                                   # two graphs, each with buffers of its own
+        lg, x = ins[0][0].clone(), ins[0][1].clone()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = layer(E, lg, bias, x, tab, Ex, H, I, Wsh, K)
+        graphs.append((gr, lg, x, got))
+    for i in (1, 2, 0):
+        for gr, lg, x, got in graphs:
+            lg.copy_(ins[i][0]); x.copy_(ins[i][1])
+            gr.replay()
+            assert all(torch.equal(a, b) for a, b in zip(got, ref[i]))
+    E.context().check_device()
+
