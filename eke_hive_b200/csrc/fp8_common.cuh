@@ -1,0 +1,40 @@
+// Shared by the 8-bit kernels: blocks of 128 values and the rule that quantises one.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "hb_common.cuh"
+
+namespace hb {
+
+constexpr int F8_B = 128;                              // values a scale covers
+__host__ __device__ constexpr int f8_blocks(int n) { return (n + F8_B - 1) / F8_B; }
+
+// ---- quantisation -------------------------------------------------------------------------------------------------------------------
+// The largest magnitude of a block as the bits of a float: they order like the magnitudes, infinities and NaN last.  From it the scale that
+// is stored (amax / 448) and the code of each value: e4m3(v · 448 / amax).  v · 448 of a bf16 value is exact in fp32; the quotient is worked out
+// from the reciprocal with one residual step, which gives the correctly rounded one (Markstein, "Computation of elementary functions on the
+// IBM RISC System/6000 processor", 1990), and exactly the quotient where fp32 holds it, so a tie between two codes is seen as one.
+// Blocks of very small or very large values are brought to the middle of the range by a power of two first: nothing over- or underflows
+// that could be more than a zero code.
+struct F8Block {
+  float f, d, r; bool live;                            // v·f is the value scaled, d = amax·f, r = 1 / d
+  __device__ __forceinline__ float init(uint32_t bits) {   // returns the scale
+    const float amax = __uint_as_float(bits);
+    live = bits > 0u && bits < 0x7f800000u;
+    f = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.f;
+    d = __fmul_rn(amax, f); r = live ? __frcp_rn(d) : 0.f;
+    return bits < 0x7f800000u ? __fdiv_rn(amax, 448.f) : __int_as_float(0x7fc00000);
+  }
+  __device__ __forceinline__ float quotient(float v) const {
+    const float t = __fmul_rn(__fmul_rn(v, f), 448.f), q = __fmul_rn(t, r);
+    return copysignf(__fmaf_rn(__fmaf_rn(-q, d, t), r, q), t);
+  }
+  __device__ __forceinline__ uint32_t pair(float a, float b) const {   // codes of two values, the first in the low byte
+    uint16_t o;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(quotient(b)), "f"(quotient(a)));
+    return live ? (uint32_t)o : 0u;
+  }
+};
+__device__ __forceinline__ uint32_t f8_mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+}  // namespace hb

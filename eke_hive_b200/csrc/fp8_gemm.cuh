@@ -1,0 +1,368 @@
+// The product of 8-bit rows and 8-bit weights with a scale per block of 128, on the 5th-generation tensor cores: one kernel for the dense
+// product, for the gate/up pass of routed experts (SwiGLU and the quantisation of its result in the epilogue) and for their down pass.
+//
+//   acc[n, m] += (ws[n / 128, b] · xs[b, m]) · Σ_{k in block b} w[n, k]·x[m, k]          for every block b of 128 values of K
+//
+// A block's sum is one accumulator tile of tcgen05.mma kind::f8f6f4 (e4m3 × e4m3: exact products, fp32 sums) in tensor memory; the scales are fp32
+// numbers of any value, which no MMA applies, so the epilogue warps read every block's sums back and add them, scaled, to sums of their own in registers.
+// The weights are the A operand (128 rows a tile, two tiles an item), the rows of x the B operand (N = up to BN of them): a lane of tensor memory is
+// a weight row, a column a row of x, so a call with few rows wastes no tensor-core columns, and what a thread ends up with is one output column
+// n for many rows m — in the gate/up pass gate and up of the same value.
+//
+// Work: items (tile of rows × 256 weight rows) of ceil(K / 128) steps.  Whole items go round the CTAs; what is left over, less than two rounds, is cut into
+// equal runs of steps, one a CTA, without regard to where an item ends.  A CTA that holds part of an item leaves its sums in the workspace; the last
+// one to arrive (a counter an item) adds all parts in the order of the CTAs — the same order in every run — and finishes the item.  So a product
+// with one row of x keeps all SMs streaming weights to the end.  Nobody waits for anybody.
+//
+// Per CTA (persistent, one per SM, 12 warps): warp 8 (one thread) loads the operand tiles by TMA under the 128-byte swizzle, warp 9 (one thread) issues the
+// MMAs, warp 10 multiplies the step's scales, warps 0-7 read the sums back (a warp reaches the 32 lanes of its number mod 4; warps 0-3 take the first half
+// of the columns, 4-7 the second) and end the items.  Two accumulator buffers: one fills while the other is read.  Every wait is bounded.
+#pragma once
+#include "fp8_common.cuh"
+#include "wmap.cuh"
+
+namespace hb {
+
+enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
+
+constexpr int F8_MAX_CTAS = 160;                       // grid at most; the workspace holds two partial items of each
+constexpr int F8_COUNTERS = 2 * F8_MAX_CTAS;           // items that are cut, at most
+constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
+constexpr int F8_A_BYTES = 128 * 128;                  // a tile of weights: 128 rows × 128 values
+
+template <int BN_>
+struct F8Cfg {
+  static constexpr int BN = BN_, CW = BN / 2;          // rows of x a tile may have; columns of tensor memory an epilogue warp reads of each weight tile
+  static constexpr int B_BYTES = BN * 128, STAGE = 2 * F8_A_BYTES + B_BYTES;
+  static constexpr int ST = 200 * 1024 / STAGE;        // ring of operand stages
+  static constexpr int TMEM = BN <= 16 ? 64 : 4 * BN;  // two buffers of two tiles
+  static constexpr int LD = CW < 32 ? CW : 32;         // columns read at a time
+  static constexpr int SMEM = 1024 + ST * STAGE + 2 * 2 * BN * 4 + 2 * 4 * CW * 4 + 512;
+  static_assert(F8_COUNTERS <= kErrCounterWords, "counters of the context");
+  static_assert(SMEM <= 227 * 1024 && TMEM <= 512 && STAGE % 1024 == 0, "shared memory, tensor memory, swizzle atoms");
+};
+
+struct F8Args {
+  const TileRef* tiles; const int* n_tiles;            // GU / DOWN: tiles of slots; PLAIN: ceil(M / per) tiles of `per` rows
+  int M, per, N, K, n_nt;                              // n_nt: items a tile has (GU: N / 128 with N = I, else ceil(N / 256))
+  const float* ws; const uint8_t* const* tab; uint64_t off_w, off_s0, off_s1; int row2;   // PLAIN: scales; else records, offsets of the codes and of the two tiles' scales, rows from the first tile's matrix to the second's (GU)
+  WmArgs wm;
+  const float* xs; int lds;                            // scales of the rows
+  float limit;
+  __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN
+  uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
+  float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256], arrivals (zero before and after)
+  uint32_t* err;
+};
+
+// The steps of a CTA, the same for all its warps: segments (item, first step, end).
+struct F8Sched {
+  int items, KB, G, dp, sk; long long U; int Gs;
+  long long u, u1; int i;
+  __device__ __forceinline__ void init(int items_, int KB_) {
+    items = items_; KB = KB_; G = gridDim.x;
+    const int waves = items / G, rem = items - waves * G;
+    dp = rem == 0 ? waves : max(waves - 1, 0);         // rounds of whole items, after the cut ones
+    sk = items - dp * G;
+    U = (long long)sk * KB;
+    Gs = (int)min((long long)G, max(U, 1ll));          // CTAs that get a run of steps: none is empty
+    u = start(blockIdx.x); u1 = start(blockIdx.x + 1);
+    i = 0;
+  }
+  __device__ __forceinline__ long long start(int c) const { return c >= Gs ? U : (long long)c * U / Gs; }
+  __device__ __forceinline__ bool next(int& item, int& kb0, int& kb1) {
+    if (u < u1) {
+      item = (int)(u / KB); kb0 = (int)(u - (long long)item * KB);
+      kb1 = (int)min((long long)KB, kb0 + (u1 - u));
+      u += kb1 - kb0;
+      return true;
+    }
+    if (i >= dp) return false;
+    item = sk + i * G + blockIdx.x; kb0 = 0; kb1 = KB; ++i;
+    return true;
+  }
+  __device__ __forceinline__ int owner(long long step) const { return (int)(((step + 1) * Gs - 1) / U); }
+};
+
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// a += d·s, two values at a time
+__device__ __forceinline__ void f8_fma2(float& a0, float& a1, uint32_t d0, uint32_t d1, float s0, float s1) {
+  asm("{\n .reg .b64 a, d, s;\n mov.b64 a, {%0, %1};\n mov.b64 d, {%2, %3};\n mov.b64 s, {%4, %5};\n fma.rn.f32x2 a, d, s, a;\n mov.b64 {%0, %1}, a;\n}"
+      : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
+}
+__device__ __forceinline__ bool named_bar_and(int id, int threads, bool v) {   // barrier of `threads` threads; true where all bring true
+  uint32_t o;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(o) : "r"(id), "r"(threads), "r"((uint32_t)v) : "memory");
+  return o != 0;
+}
+template <int W>
+__device__ __forceinline__ void f8_ld(uint32_t taddr, uint32_t (&r)[W]) {
+  if constexpr (W == 32) tc_ld32(taddr, r);
+  else if constexpr (W == 16) tc_ld16(taddr, r);
+  else tc_ld8(taddr, r);
+}
+
+template <int BN, int MODE>
+__global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+  using C = F8Cfg<BN>;
+  extern __shared__ uint8_t f8_raw[];
+  const uint32_t raw = smem_u32(f8_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = f8_raw + (base - raw);
+  float* scl = reinterpret_cast<float*>(sm + C::ST * C::STAGE);              // [2 buffers][2 tiles][BN]
+  uint32_t* amx = reinterpret_cast<uint32_t*>(scl + 4 * BN);                 // [2 halves][4 warps][CW]: magnitudes of y
+  uint64_t* full = reinterpret_cast<uint64_t*>(amx + 8 * C::CW);             // [ST] the stage's operands have landed
+  uint64_t* empty = full + C::ST;                                            // [ST] the MMAs that read them are done
+  uint64_t* acc_full = empty + C::ST;                                        // [2] the buffer's sums and scales are there
+  uint64_t* acc_empty = acc_full + 2;                                        // [2] the epilogue has read them
+  uint64_t* mma_done = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile uint32_t* last = tmem_slot + 1;
+  const int warp = warp_uniform(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 2); mbar_init(&acc_empty[s], 8); }
+    mbar_init(mma_done, 1);
+    mbar_fence_init();
+  }
+  if (warp == F8_W_MMA) { tmem_alloc(tmem_slot, C::TMEM); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch();
+  const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
+  F8Sched sch;
+  sch.init(n_tiles * a.n_nt, KB);
+  auto tile_of = [&](int ti) -> TileRef {
+    if (MODE != F8_PLAIN) return a.tiles[ti];
+    return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
+  };
+  int item, kb0, kb1;
+
+  if (warp == F8_W_TMA) {
+    // ------------------------------------------------------------------------------------------------ operand tiles, one thread
+    if (elect_one()) {
+      uint32_t s = 0, ph = 1;
+      bool ok = true;
+      WmReader wm;
+      if (MODE != F8_PLAIN) wm.init(a.wm);
+      while (ok && sch.next(item, kb0, kb1)) {
+        const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
+        const TileRef tl = tile_of(ti);
+        WmBox box;
+        if (MODE != F8_PLAIN && !wm.locate(a.tab[tl.expert] + a.off_w, box, a.err)) break;
+        const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, r1 = MODE == F8_GU ? r0 + a.row2 : r0 + 128;
+        const bool two = MODE == F8_GU || r1 < a.N;                            // a last item may have one tile: beyond it there is other memory
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
+          const uint32_t sb = base + s * C::STAGE;
+          mbar_expect_tx(&full[s], (two ? 2 : 1) * F8_A_BYTES + C::B_BYTES);
+          if (MODE == F8_PLAIN) {
+            tma_load_2d(sb, &tmW, kb * 128, r0, &full[s]);
+            if (two) tma_load_2d(sb + F8_A_BYTES, &tmW, kb * 128, r1, &full[s]);
+          } else {
+            wm.load(sb, box, kb * 128, r0, &full[s]);
+            wm.load(sb + F8_A_BYTES / 2, box, kb * 128, r0 + 64, &full[s]);
+            if (two) {
+              wm.load(sb + F8_A_BYTES, box, kb * 128, r1, &full[s]);
+              wm.load(sb + F8_A_BYTES + F8_A_BYTES / 2, box, kb * 128, r1 + 64, &full[s]);
+            }
+          }
+          tma_load_2d(sb + 2 * F8_A_BYTES, &tmX, kb * 128, tl.slot0, &full[s]);
+          if (++s == C::ST) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == F8_W_MMA) {
+    // ------------------------------------------------------------------------------------------------ MMA issue, one thread
+    if (elect_one()) {
+      uint32_t s = 0, ph = 0, it = 0;
+      bool ok = true;
+      while (ok && sch.next(item, kb0, kb1)) {
+        const int rows = tile_of(item / a.n_nt).rows;
+        // kind::f8f6f4: D fp32 (bit 4), A and B e4m3 (format 0 at bits 7 and 10), both K-major, N / 8 at bit 17, M / 16 at bit 24
+        const uint32_t idesc = (1u << 4) | ((uint32_t)((rows + 15) >> 4) << 18) | ((128u >> 4) << 24);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t buf = it & 1u;
+          if (!(ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x200u))) break;
+          if (!(ok = mbar_wait(&full[s], ph, a.err, 0x400u))) break;
+          tc_fence_after();
+          const uint32_t sb = base + s * C::STAGE, d = tmem + buf * (2 * BN);
+          const uint64_t ad = tc_desc_sw128(sb), bd = tc_desc_sw128(sb + 2 * F8_A_BYTES);
+#pragma unroll
+          for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)                                   // 32 values further along the swizzled rows
+              tc_mma_f8(d + u * BN, ad + u * (F8_A_BYTES >> 4) + 2 * j, bd + 2 * j, idesc, j);
+          tc_commit(&empty[s]);
+          tc_commit(&acc_full[buf]);
+          if (++s == C::ST) { s = 0; ph ^= 1u; }
+        }
+      }
+      tc_commit(mma_done);                                                     // nothing is in flight when tensor memory is freed
+      mbar_wait(mma_done, 0, a.err, 0x800u);
+    }
+  } else if (warp == F8_W_SCALE) {
+    // ------------------------------------------------------------------------------------------------ scales of a step: weight block × row, a step ahead
+    constexpr int NL = (BN + 31) / 32;
+    uint32_t it = 0;
+    bool ok = true;
+    while (ok && sch.next(item, kb0, kb1)) {
+      const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
+      const TileRef tl = tile_of(ti);
+      const float *w0, *w1;
+      if (MODE == F8_PLAIN) { w0 = a.ws + (size_t)(2 * nt) * KB; w1 = nt * 256 + 128 < a.N ? w0 + KB : w0; }
+      else {
+        const uint8_t* rec = a.tab[tl.expert];
+        const int b0 = MODE == F8_GU ? nt : 2 * nt, b1 = MODE == F8_GU ? nt : nt * 256 + 128 < a.N ? b0 + 1 : b0;
+        w0 = reinterpret_cast<const float*>(rec + a.off_s0) + (size_t)b0 * KB;
+        w1 = reinterpret_cast<const float*>(rec + a.off_s1) + (size_t)b1 * KB;
+      }
+      float nx[NL], n0, n1;
+      auto fetch = [&](int kb) {
+        n0 = __ldg(w0 + kb); n1 = __ldg(w1 + kb);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) nx[i] = lane + 32 * i < tl.rows ? __ldcg(a.xs + (size_t)kb * a.lds + tl.slot0 + lane + 32 * i) : 0.f;
+      };
+      fetch(kb0);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t buf = it & 1u;
+        float x[NL]; const float s0 = n0, s1 = n1;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x[i] = nx[i];
+        if (kb + 1 < kb1) fetch(kb + 1);
+        ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x2000u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float* d = scl + buf * (2 * BN);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (BN >= 32 || lane < BN) { d[lane + 32 * i] = x[i] * s0; d[BN + lane + 32 * i] = x[i] * s1; }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_full[buf]);
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has lanes [32 q, 32 q + 32), columns [h·CW, (h + 1)·CW)
+    const int h = warp >> 2, q = warp & 3, row = 32 * q + lane;
+    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + h * C::CW;
+    uint32_t it = 0;
+    bool ok = true;
+    while (ok && sch.next(item, kb0, kb1)) {
+      const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
+      const TileRef tl = tile_of(ti);
+      const int cols = min(max(tl.rows - h * C::CW, 0), C::CW);                // this warp's columns that hold rows of x
+      float acc[2][C::CW];
+#pragma unroll
+      for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t buf = it & 1u;
+        ok = mbar_wait(&acc_full[buf], (it >> 1) & 1u, a.err, 0x1000u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c0 = 0; c0 < C::CW; c0 += C::LD) {
+            if (c0 < cols) {
+              uint32_t r[C::LD];
+              f8_ld<C::LD>(trow + buf * (2 * BN) + u * BN + c0, r);
+              const float4* s4 = reinterpret_cast<const float4*>(scl + buf * (2 * BN) + u * BN + h * C::CW + c0);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < C::LD; c += 4) {
+                const float4 sv = s4[c / 4];
+                f8_fma2(acc[u][c0 + c], acc[u][c0 + c + 1], r[c], r[c + 1], sv.x, sv.y);
+                f8_fma2(acc[u][c0 + c + 2], acc[u][c0 + c + 3], r[c + 2], r[c + 3], sv.z, sv.w);
+              }
+            }
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
+      // ---- an item that other CTAs have parts of: leave the sums, the last one to arrive goes on with everybody's
+      if (!(ok = named_bar_and(1, 256, ok))) break;
+      if (kb1 - kb0 < KB) {
+        const long long s0 = (long long)item * KB;
+        const int c_first = sch.owner(s0), c_last = sch.owner(s0 + KB - 1);
+        auto part_of = [&](int c) { return a.part + ((size_t)c * 2 + (sch.start(c) / KB == item ? 0 : 1)) * (256 * BN) + (size_t)h * C::CW * 256 + row; };
+        float* mine = part_of(blockIdx.x);
+#pragma unroll
+        for (int c = 0; c < C::CW; ++c)
+          if (c < cols) { __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]); }
+        __threadfence();
+        named_bar_sync(1, 256);
+        if (threadIdx.x == 0) {
+          const bool all = atomicAdd(a.count + item, 1u) == (unsigned)(c_last - c_first);
+          if (all) a.count[item] = 0u;                                         // zero again for the next launch
+          *last = all;
+        }
+        named_bar_sync(1, 256);
+        const bool mine_to_end = *last != 0u;
+        named_bar_sync(1, 256);                                                // the flag has been read: the next item may write it
+        if (!mine_to_end) continue;
+        __threadfence();
+#pragma unroll
+        for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
+        for (int cc = c_first; cc <= c_last; ++cc) {
+          const float* p = part_of(cc);
+#pragma unroll
+          for (int c = 0; c < C::CW; ++c)
+            if (c < cols) { acc[0][c] += __ldcg(p + c * 256); acc[1][c] += __ldcg(p + c * 256 + 128); }
+        }
+      }
+      // ---- the item's results
+      if (MODE == F8_GU) {
+        uint32_t* am = amx + (h * 4) * C::CW;
+#pragma unroll
+        for (int c = 0; c < C::CW; ++c) {
+          float gv = acc[0][c], uv = acc[1][c];
+          if (a.limit > 0.f) { gv = fminf(gv, a.limit); uv = fminf(fmaxf(uv, -a.limit), a.limit); }
+          acc[0][c] = gv / (1.f + expf(-gv)) * uv;
+          const uint32_t mx = __reduce_max_sync(0xffffffffu, f8_mag(acc[0][c]));
+          if (lane == 0) am[q * C::CW + c] = mx;
+        }
+        named_bar_sync(2 + h, 128);
+#pragma unroll
+        for (int c = 0; c < C::CW; ++c) {
+          F8Block blk;
+          const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
+          const uint32_t code = blk.pair(acc[0][c], 0.f);
+          const int slot = tl.slot0 + h * C::CW + c;
+          if (c < cols) {
+            a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)code;
+            if (row == 0) a.ys[(size_t)nt * a.ldys + slot] = sc;
+          }
+        }
+        named_bar_sync(2 + h, 128);                                            // the magnitudes have been read
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int n = nt * 256 + u * 128 + row;
+          if (n < a.N) {
+#pragma unroll
+            for (int c = 0; c < C::CW; ++c)
+              if (c < cols) {
+                const size_t at = (size_t)(tl.slot0 + h * C::CW + c) * a.ldy + n;
+                if (MODE == F8_DOWN || a.yb) a.yb[at] = __float2bfloat16(acc[u][c]);
+                else a.yf[at] = acc[u][c];
+              }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == F8_W_MMA) { tc_fence_after(); tmem_dealloc(tmem, C::TMEM); }
+}
+
+}  // namespace hb

@@ -32,7 +32,8 @@ int hb_create(const hb_config* cfg, hb_ctx** out) {
   if (prop.major != 10) { delete c; return HB_ERR_NO_DEVICE; }          // the kernels are sm_100a only
   c->sm_count = prop.multiProcessorCount;
   c->smem_optin = (int)prop.sharedMemPerBlockOptin;
-  if (cudaMalloc(&c->dev_err, 256) != cudaSuccess || cudaMemset(c->dev_err, 0, 256) != cudaSuccess) { delete c; cudaGetLastError(); return HB_ERR_CUDA; }
+  constexpr size_t block = (kErrCounters + kErrCounterWords) * 4;
+  if (cudaMalloc(&c->dev_err, block) != cudaSuccess || cudaMemset(c->dev_err, 0, block) != cudaSuccess) { delete c; cudaGetLastError(); return HB_ERR_CUDA; }
   {
     const uint32_t polls = cfg && cfg->wait_polls ? cfg->wait_polls : (1u << 24);
     if (cudaMemcpy(c->dev_err + kErrWaitPolls, &polls, 4, cudaMemcpyHostToDevice) != cudaSuccess) { cudaFree(c->dev_err); delete c; cudaGetLastError(); return HB_ERR_CUDA; }
@@ -41,6 +42,7 @@ int hb_create(const hb_config* cfg, hb_ctx** out) {
   if (r == HB_OK) r = hbk_nvfp4_setup(c);
   if (r == HB_OK) r = hbk_dense_setup(c);
   if (r == HB_OK) r = hbk_moe_prefill_setup(c);
+  if (r == HB_OK) r = hbk_fp8_setup(c);
   if (r != HB_OK) { cudaFree(c->dev_err); delete c; return r; }
   *out = c;
   return HB_OK;
@@ -125,6 +127,7 @@ int hb_check_device(hb_ctx* ctx, void* stream) {
     HB_CUDA(ctx, cudaStreamSynchronize(as_stream(stream)));
   }
   HB_CUDA(ctx, cudaMemsetAsync(ctx->dev_err, 0, 4, as_stream(stream)));
+  HB_CUDA(ctx, cudaMemsetAsync(ctx->dev_err + kErrCounters, 0, kErrCounterWords * 4, as_stream(stream)));   // a product that gave up left its counts where they were
   if (v & 0x80000000u)
     return hb_fail(ctx, HB_ERR_DEVICE_FLAG, "device error word 0x%x: range check 0x%x failed with value %d (debug build)", v, site[0], (int)site[1]);
   return hb_fail(ctx, HB_ERR_DEVICE_FLAG, "device error word 0x%x (bits 0x1-0x80: a pipeline wait inside a decode or prefill kernel; 0x400-0x2000: the decode layer kernel's tables and grid barrier; "

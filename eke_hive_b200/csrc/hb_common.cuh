@@ -18,6 +18,9 @@ constexpr int kErrWaitPolls = 17;
 constexpr int kErrPlanMeet = 18;
 constexpr int kErrBoundSite = 20;     // [20], [21]: first failed range check of a -DHB_BOUNDS build (site code, offending value)      // [18], [19]: the meeting counters of the prefill plan kernel
 
+constexpr int kErrCounters = 64;      // behind the block: arrival counters of products that are cut along K (fp8_gemm.cuh), zero between launches
+constexpr int kErrCounterWords = 320;
+
 struct hb_ctx {
   int device = 0;
   int sm_count = 0;

@@ -104,3 +104,4 @@ int hbk_moe_dtc_down_run(hb_ctx* ctx, int P, int H, int I, void* ws, const hb::R
 // dense GEMV (k_dense.cu)
 int hbk_dense_setup(hb_ctx* ctx);
 int hbk_moe_prefill_setup(hb_ctx* ctx);
+int hbk_fp8_setup(hb_ctx* ctx);

@@ -1,82 +1,39 @@
 // 8-bit floats with a scale per block of 128: the quantisers of activations and weights, the product, the routed experts.
-#include <cuda_fp8.h>
-
-#include "hb_common.cuh"
+#include "fp8_gemm.cuh"
 #include "hb_kernels.h"
-#include "tc_common.cuh"
 
 namespace hb {
 
-constexpr int F8_B = 128;                              // values a scale covers
-__host__ __device__ constexpr int f8_blocks(int n) { return (n + F8_B - 1) / F8_B; }
-
-// ---- quantisation -------------------------------------------------------------------------------------------------------------------
-// The largest magnitude of a block as the bits of a float: they order like the magnitudes, infinities and NaN last.  From it the scale that
-// is stored (amax / 448) and the code of each value: e4m3(v · 448 / amax).  v · 448 of a bf16 value is exact in fp32; the quotient is worked out
-// from the reciprocal with one residual step, which gives the correctly rounded one (Markstein, "Computation of elementary functions on the
-// IBM RISC System/6000 processor", 1990), and exactly the quotient where fp32 holds it, so a tie between two codes is seen as one.
-// Blocks of very small or very large values are brought to the middle of the range by a power of two first: nothing over- or underflows
-// that could be more than a zero code.
-struct F8Block {
-  float f, d, r; bool live;                            // v·f is the value scaled, d = amax·f, r = 1 / d
-  __device__ __forceinline__ float init(uint32_t bits) {   // returns the scale
-    const float amax = __uint_as_float(bits);
-    live = bits > 0u && bits < 0x7f800000u;
-    f = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.f;
-    d = __fmul_rn(amax, f); r = live ? __frcp_rn(d) : 0.f;
-    return bits < 0x7f800000u ? __fdiv_rn(amax, 448.f) : __int_as_float(0x7fc00000);
-  }
-  __device__ __forceinline__ float quotient(float v) const {
-    const float t = __fmul_rn(__fmul_rn(v, f), 448.f), q = __fmul_rn(t, r);
-    return copysignf(__fmaf_rn(__fmaf_rn(-q, d, t), r, q), t);
-  }
-  __device__ __forceinline__ uint32_t pair(float a, float b) const {   // codes of two values, the first in the low byte
-    uint16_t o;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(quotient(b)), "f"(quotient(a)));
-    return live ? (uint32_t)o : 0u;
-  }
-};
-__device__ __forceinline__ uint32_t f8_mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 // Rows: 16 lanes take a block of 128 values, 8 each.  dest == nullptr: row m of q / s; else row m goes to slots dest[m·nd + j], j < nd, negative ones
-// skipped (the rows of a routed layer are quantised once and written into expert order).  Source: bf16, or silu(g)·u of two fp32 matrices.
+// skipped (the rows of a routed layer are quantised once and written into expert order).
 struct F8RowsArgs {
-  const __nv_bfloat16* x; int ldx;
-  const float* g; const float* u; float limit;         // x == nullptr: y = silu(g)·u, both [M,K]
-  int M, K; const int* m_dev;                          // m_dev: rows there really are (device), at most M
+  const __nv_bfloat16* x; int ldx, M, K;
   const int* dest; int nd;
   uint8_t* q; int ldq; float* s; int lds;
+  WmStamp wm;                                          // with dest: the first CTA stamps the weight maps of the call's GEMMs instead
 };
-__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const F8RowsArgs a) {
+__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const __grid_constant__ F8RowsArgs a) {
   griddep_wait();
+  if (a.dest && blockIdx.x == 0) { wm_stamp(a.wm); return; }
+  const int cta = blockIdx.x - (a.dest ? 1 : 0), ctas = gridDim.x - (a.dest ? 1 : 0);
   const int nb = f8_blocks(a.K), l16 = threadIdx.x & 15;
   const uint32_t half = 0xffffu << (threadIdx.x & 16);
-  const int M = a.m_dev ? min(a.M, *a.m_dev) : a.M;
-  const long long total = (long long)M * nb;
-  for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i < total; i += (long long)gridDim.x * 16) {
+  const long long total = (long long)a.M * nb;
+  for (long long i = (long long)cta * 16 + (threadIdx.x >> 4); i < total; i += (long long)ctas * 16) {
     const int m = (int)(i / nb), b = (int)(i - (long long)m * nb), k = b * F8_B + l16 * 8;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
     if (k < a.K) {                                                             // K is a multiple of 16: eight values are inside or outside together
-      if (a.x) {
-        const __nv_bfloat16* p = a.x + (size_t)m * a.ldx + k;
-        if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      const __nv_bfloat16* p = a.x + (size_t)m * a.ldx + k;
+      if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(ww[j] << 16); v[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __bfloat162float(p[j]);
-        }
+        for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(ww[j] << 16); v[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float gv = a.g[(size_t)m * a.K + k + j], uv = a.u[(size_t)m * a.K + k + j];
-          if (a.limit > 0.f) { gv = fminf(gv, a.limit); uv = fminf(fmaxf(uv, -a.limit), a.limit); }
-          v[j] = gv / (1.f + expf(-gv)) * uv;
-        }
+        for (int j = 0; j < 8; ++j) v[j] = __bfloat162float(p[j]);
       }
     }
     uint32_t mx = 0u;
@@ -142,61 +99,6 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
   }
 }
 
-// ---- the product, simple form: 64 rows × 64 tokens a CTA, fp32 on the CUDA cores --------------------------------------------------------
-struct F8GemmArgs {
-  const uint8_t* w; const float* ws;                   // one matrix, or (tab) the expert's at these offsets
-  const uint8_t* const* tab; uint64_t off_w, off_s;
-  const TileRef* tiles; const int* n_tiles;            // tab: tiles of slots
-  const uint8_t* xq; int ldq; const float* xs; int lds;
-  int M, N, K;
-  __nv_bfloat16* yb; float* yf; int ldy;
-};
-__global__ void __launch_bounds__(256) fp8_gemm_simple_kernel(const F8GemmArgs a) {
-  __shared__ float xa[32][65], wa[32][65];
-  TileRef t{(int)blockIdx.y * 64, min(64, a.M - (int)blockIdx.y * 64), 0};
-  const uint8_t* w = a.w; const float* ws = a.ws;
-  if (a.tab) {
-    if ((int)blockIdx.y >= *a.n_tiles) return;
-    t = a.tiles[blockIdx.y];
-    w = a.tab[t.expert] + a.off_w; ws = reinterpret_cast<const float*>(a.tab[t.expert] + a.off_s);
-  }
-  const int n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, nb = f8_blocks(a.K);
-  float acc[4][4] = {}, part[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 32) {
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      const int r = i >> 5, k = k0 + (i & 31);
-      xa[i & 31][r] = r < t.rows && k < a.K ? e4m3_to_f32(a.xq[(size_t)(t.slot0 + r) * a.ldq + k]) : 0.f;
-      wa[i & 31][r] = n0 + r < a.N && k < a.K ? e4m3_to_f32(w[(size_t)(n0 + r) * a.K + k]) : 0.f;
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(xa[k][ty * 4 + i], wa[k][tx + 16 * j], part[i][j]);
-    __syncthreads();
-    if ((k0 & 127) == 96 || k0 + 32 >= a.K) {
-      const float sw = ws[(size_t)(n0 >> 7) * nb + (k0 >> 7)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float sx = ty * 4 + i < t.rows ? a.xs[(size_t)(k0 >> 7) * a.lds + t.slot0 + ty * 4 + i] * sw : 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { acc[i][j] = fmaf(part[i][j], sx, acc[i][j]); part[i][j] = 0.f; }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = ty * 4 + i, n = n0 + tx + 16 * j;
-      if (r >= t.rows || n >= a.N) continue;
-      const size_t at = (size_t)(t.slot0 + r) * a.ldy + n;
-      if (a.yb) a.yb[at] = __float2bfloat16(acc[i][j]);
-      else a.yf[at] = acc[i][j];
-    }
-}
-
 // ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)] (+ gate·shared[m]) --------------------------------------------
 __global__ void __launch_bounds__(256) fp8_sum_kernel(const __nv_bfloat16* __restrict__ part, const int* __restrict__ pos_of, const float* __restrict__ w, int K, int H,
                                                       float* __restrict__ out, const __nv_bfloat16* __restrict__ shared, const float* __restrict__ lg, int ld, int col,
@@ -219,29 +121,71 @@ __global__ void __launch_bounds__(256) fp8_sum_kernel(const __nv_bfloat16* __res
 using namespace hb;
 
 namespace {
-constexpr int F8_BM = 64;                              // tokens of a tile
+using F8Kernel = void (*)(const F8Args, const CUtensorMap, const CUtensorMap);
+struct F8Pick { F8Kernel fn; int smem; };
+template <int MODE>
+F8Pick f8_kernel(int bn) {
+  switch (bn) {
+    case 16: return {fp8_gemm_kernel<16, MODE>, F8Cfg<16>::SMEM};
+    case 32: return {fp8_gemm_kernel<32, MODE>, F8Cfg<32>::SMEM};
+    case 64: return {fp8_gemm_kernel<64, MODE>, F8Cfg<64>::SMEM};
+    default: return {fp8_gemm_kernel<128, MODE>, F8Cfg<128>::SMEM};
+  }
+}
+int f8_grid(const hb_ctx* ctx) {
+  const int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
+  return n < F8_MAX_CTAS ? n : F8_MAX_CTAS;
+}
+size_t f8_part_bytes(int bn) { return (size_t)F8_MAX_CTAS * 2 * 256 * bn * 4; }
+// rows of a tile for a product of M rows
+int f8_bn_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+// pairs of a tile by what an expert gets on average: runs that are longer are cut into tiles, which read the expert's weights again
+int f8_bn_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 16ll * E ? 32 : P <= 40ll * E ? 64 : 128; }
+// map of a byte matrix [n_rows][row_bytes], rows ld bytes apart, in boxes of 128 bytes × box_rows under the 128-byte swizzle; bytes and rows past the
+// end read as zero codes
+int f8_map(hb_ctx* ctx, CUtensorMap* m, const void* base, size_t row_bytes, size_t ld, size_t n_rows, int box_rows) {
+  TcEncodeFn fn = tc_encode_fn();
+  HB_REQUIRE(ctx, fn, HB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)n_rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  HB_REQUIRE(ctx, r == CUDA_SUCCESS, HB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %zu rows of %zu bytes at %p", (int)r, n_rows, row_bytes, base);
+  return HB_OK;
+}
+
 struct F8Ws {
-  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; float* g; float* u; uint8_t* yq; float* ys; __nv_bfloat16* part;
+  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; uint8_t* yq; float* ys; __nv_bfloat16* part; float* cut; uint8_t* wmaps;
 };
 size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   size_t off = 0;
   auto take = [&](size_t b) { void* r = ws ? static_cast<char*>(ws) + off : nullptr; off += hb_align256(b); return r; };
   const size_t P = (size_t)M * K;
+  const int bn = f8_bn_pairs((long long)P, E);
   F8Ws t;
   t.hist = (int*)take(hbk_pf_plan_hist_bytes(E)); t.n_slots = (int*)take(4); t.n_tiles = (int*)take(4);
-  t.tiles = (TileRef*)take((P / F8_BM + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
+  t.tiles = (TileRef*)take((P / bn + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
   t.xq = (uint8_t*)take(P * H); t.xs = (float*)take(P * f8_blocks(H) * 4);
-  t.g = (float*)take(P * I * 4); t.u = (float*)take(P * I * 4);
   t.yq = (uint8_t*)take(P * I); t.ys = (float*)take(P * f8_blocks(I) * 4);
   t.part = (__nv_bfloat16*)take(P * H * 2);
+  t.cut = (float*)take(f8_part_bytes(bn));
+  t.wmaps = (uint8_t*)take(wm_bytes(2 * H) + wm_bytes(2 * I));               // (the maps count e2m1 columns, two to a byte)
   if (w) *w = t;
   return off;
 }
+unsigned int* f8_counters(hb_ctx* ctx) { return reinterpret_cast<unsigned int*>(ctx->dev_err) + kErrCounters; }
 int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
   const long long units = (long long)a.M * f8_blocks(a.K), ctas = (units + 15) / 16, cap = (long long)ctx->sm_count * 32;
-  return hb_launch(ctx, "fp8_quant_rows", !(ctx->flags & HB_FLAG_NO_PDL), fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(256), 0, st, a);
+  return hb_launch(ctx, "fp8_quant_rows", !(ctx->flags & HB_FLAG_NO_PDL), fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap) + (a.dest ? 1 : 0)), dim3(256), 0, st, a);
 }
 }  // namespace
+
+int hbk_fp8_setup(hb_ctx* ctx) {
+  for (int bn : {16, 32, 64, 128})
+    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)})
+      HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+  return HB_OK;
+}
 
 extern "C" {
 
@@ -269,7 +213,7 @@ int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t*
   return hb_launch(ctx, "fp8_quantize", false, fp8_quantize_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float*>(w), N, K, q, s);
 }
 
-size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? 256 : 0; }
+size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(f8_bn_rows(M)) : 0; }
 
 int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb, float* yf, int ldy, void* ws, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
@@ -281,10 +225,17 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "fp8_gemm: ws NULL or not 256-byte aligned");
-  F8GemmArgs a{};
-  a.w = W->w; a.ws = reinterpret_cast<const float*>(W->s); a.xq = xq; a.ldq = ldq; a.xs = xs; a.lds = lds; a.M = M; a.N = W->N; a.K = W->K;
-  a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy;
-  return hb_launch(ctx, "fp8_gemm", false, fp8_gemm_simple_kernel, dim3((W->N + 63) / 64, (M + 63) / 64), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), a);
+  const int bn = f8_bn_rows(M), nt = (M + bn - 1) / bn;
+  F8Args a{};
+  a.M = M; a.per = ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
+  HB_REQUIRE(ctx, (long long)nt * a.n_nt < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d", M, W->N);
+  a.ws = reinterpret_cast<const float*>(W->s); a.xs = xs; a.lds = lds;
+  a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.count = f8_counters(ctx); a.err = ctx->dev_err;
+  CUtensorMap tw, tx;
+  int r;
+  if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, bn))) return r;
+  const F8Pick k = f8_kernel<F8_PLAIN>(bn);
+  return hb_launch(ctx, "fp8_gemm", !(ctx->flags & HB_FLAG_NO_PDL), k.fn, dim3(f8_grid(ctx)), dim3(F8_THREADS), (size_t)k.smem, reinterpret_cast<cudaStream_t>(stream), a, tw, tx);
 }
 
 int hb_fp8_rec_layout_make(int H, int I, hb_fp8_rec_layout* L) {
@@ -316,24 +267,25 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   const uint8_t* const* tab = rec_tab + (size_t)li * E;
   F8Ws W;
   f8_carve(ws, M, K, E, H, I, &W);
-  const int P = M * K;
+  const int P = M * K, bn = f8_bn_pairs(P, E), grid = f8_grid(ctx);
+  const bool pdl = !(ctx->flags & HB_FLAG_NO_PDL);
   int r;
-  if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, F8_BM, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
   F8RowsArgs q{};
   q.x = reinterpret_cast<const __nv_bfloat16*>(x); q.ldx = H; q.M = M; q.K = H; q.dest = W.pos_of; q.nd = K; q.q = W.xq; q.ldq = H; q.s = W.xs; q.lds = P;
+  if ((r = hbk_wm_stamp_args(ctx, tab, E, nullptr, 2 * H, 2 * I, W.wmaps, &q.wm))) return r;
+  CUtensorMap tx, ty;
+  if ((r = f8_map(ctx, &tx, W.xq, H, H, P, bn)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, bn))) return r;
+  if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, bn, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
   if ((r = f8_rows(ctx, q, st))) return r;
-  const unsigned tiles = (unsigned)(P / F8_BM + (E < P ? E : P));
-  F8GemmArgs a{};
-  a.tab = tab; a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.xq = W.xq; a.ldq = H; a.xs = W.xs; a.lds = P; a.N = I; a.K = H; a.ldy = I;
-  a.off_w = L.w1; a.off_s = L.s1; a.yf = W.g;
-  if ((r = hb_launch(ctx, "fp8_gemm_gate", false, fp8_gemm_simple_kernel, dim3((I + 63) / 64, tiles), dim3(256), 0, st, a))) return r;
-  a.off_w = L.w3; a.off_s = L.s3; a.yf = W.u;
-  if ((r = hb_launch(ctx, "fp8_gemm_up", false, fp8_gemm_simple_kernel, dim3((I + 63) / 64, tiles), dim3(256), 0, st, a))) return r;
-  F8RowsArgs y{};
-  y.g = W.g; y.u = W.u; y.limit = limit; y.M = P; y.m_dev = W.n_slots; y.K = I; y.nd = 1; y.q = W.yq; y.ldq = I; y.s = W.ys; y.lds = P;
-  if ((r = f8_rows(ctx, y, st))) return r;
-  a.off_w = L.w2; a.off_s = L.s2; a.yf = nullptr; a.yb = W.part; a.xq = W.yq; a.ldq = I; a.xs = W.ys; a.N = H; a.K = I; a.ldy = H;
-  if ((r = hb_launch(ctx, "fp8_gemm_down", false, fp8_gemm_simple_kernel, dim3((H + 63) / 64, tiles), dim3(256), 0, st, a))) return r;
+  F8Args a{};
+  a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.count = f8_counters(ctx); a.err = ctx->dev_err;
+  a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.wm = wm_args(W.wmaps, 2 * H);
+  a.xs = W.xs; a.lds = P; a.yq = W.yq; a.ys = W.ys; a.ldys = P;
+  const F8Pick kg = f8_kernel<F8_GU>(bn), kd = f8_kernel<F8_DOWN>(bn);
+  if ((r = hb_launch(ctx, "fp8_gemm_gu", pdl, kg.fn, dim3(grid), dim3(F8_THREADS), (size_t)kg.smem, st, a, tx, tx))) return r;
+  a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.wm = wm_args(W.wmaps + wm_bytes(2 * H), 2 * I);
+  a.xs = W.ys; a.yb = W.part; a.ldy = H;
+  if ((r = hb_launch(ctx, "fp8_gemm_down", pdl, kd.fn, dim3(grid), dim3(F8_THREADS), (size_t)kd.smem, st, a, ty, ty))) return r;
   return hb_launch(ctx, "fp8_sum", false, fp8_sum_kernel, dim3(M), dim3(256), 0, st, (const __nv_bfloat16*)W.part, (const int*)W.pos_of, w, K, H, out,
                    cmb ? reinterpret_cast<const __nv_bfloat16*>(cmb->shared) : (const __nv_bfloat16*)nullptr, cmb && cmb->shared ? cmb->lg : (const float*)nullptr, cmb ? cmb->ld : 0,
                    cmb ? cmb->col : 0, cmb ? reinterpret_cast<__nv_bfloat16*>(cmb->out) : (__nv_bfloat16*)nullptr);

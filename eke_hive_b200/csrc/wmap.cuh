@@ -67,7 +67,7 @@ struct WmReader {
     b.map = nullptr; b.row = 0; b.far = w;
     if (row + (1ull << 24) < (1ull << 31)) {
       b.map = reinterpret_cast<const CUtensorMap*>(a.base + kWmHead) + (rem >> 4); b.row = (int)row;
-      const uint32_t bit = rem & ((1u << a.gshift) - 1u) ? 0u : 1u << (rem >> a.gshift);
+      const uint32_t bit = (rem & ((1u << a.gshift) - 1u)) || (rem >> a.gshift) > 31u ? 0u : 1u << (rem >> a.gshift);
       if (!(seen & bit)) { tmap_acquire(b.map); seen |= bit; }
     }
     return true;
