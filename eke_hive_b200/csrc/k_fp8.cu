@@ -99,20 +99,54 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
   }
 }
 
-// ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)] (+ gate·shared[m]) --------------------------------------------
-__global__ void __launch_bounds__(256) fp8_sum_kernel(const __nv_bfloat16* __restrict__ part, const int* __restrict__ pos_of, const float* __restrict__ w, int K, int H,
-                                                      float* __restrict__ out, const __nv_bfloat16* __restrict__ shared, const float* __restrict__ lg, int ld, int col,
-                                                      __nv_bfloat16* __restrict__ cout) {
-  const int m = blockIdx.x;
-  const float gate = lg ? 1.f / (1.f + expf(-lg[(size_t)m * ld + col])) : 1.f;
-  for (int n = threadIdx.x; n < H; n += 256) {
-    float acc = 0.f;
-    for (int k = 0; k < K; ++k) {
-      const int slot = pos_of[(size_t)m * K + k];
-      if (slot >= 0) acc = fmaf(w[(size_t)m * K + k], __bfloat162float(part[(size_t)slot * H + n]), acc);
+// ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)], k in order (+ gate·shared[m]) ----------------------------------
+// A thread owns eight columns of a row, 16 bytes of every pair's part; the row's slots and weights are fetched together in front of the parts.
+constexpr int F8_SUM_THREADS = 128;
+struct F8SumArgs {
+  const __nv_bfloat16* part; const int* pos_of; const float* w; int M, K, H; float* out;
+  const __nv_bfloat16* shared; const float* lg; int ld, col; __nv_bfloat16* cout;
+};
+__global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs a) {
+  griddep_wait();
+  const int chunks = a.H / 8;
+  const long long total = (long long)a.M * chunks;
+  for (long long i = (long long)blockIdx.x * F8_SUM_THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * F8_SUM_THREADS) {
+    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 8;
+    const float gate = a.lg ? 1.f / (1.f + expf(-__ldg(a.lg + (size_t)m * a.ld + a.col))) : 1.f;
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+      uint4 v[8]; float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int slot = k0 + k < a.K ? __ldcg(a.pos_of + (size_t)m * a.K + k0 + k) : -1;
+        w[k] = slot >= 0 ? __ldg(a.w + (size_t)m * a.K + k0 + k) : 0.f;
+        v[k] = slot >= 0 ? __ldcs(reinterpret_cast<const uint4*>(a.part + (size_t)slot * a.H + n)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(w[k], __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(w[k], __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
+      }
     }
-    if (!cout) out[(size_t)m * H + n] = acc;
-    else cout[(size_t)m * H + n] = __float2bfloat16(shared ? fmaf(gate, __bfloat162float(shared[(size_t)m * H + n]), acc) : acc);
+    const size_t o = (size_t)m * a.H + n;
+    if (!a.cout) {
+      *reinterpret_cast<float4*>(a.out + o) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(a.out + o + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      continue;
+    }
+    if (a.shared) {
+      const uint4 sv = __ldg(reinterpret_cast<const uint4*>(a.shared + o));
+      const uint32_t u[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(gate, __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(gate, __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
+    }
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]); p[j] = *reinterpret_cast<const uint32_t*>(&b); }
+    *reinterpret_cast<uint4*>(a.cout + o) = make_uint4(p[0], p[1], p[2], p[3]);
   }
 }
 
@@ -286,9 +320,13 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.wm = wm_args(W.wmaps + wm_bytes(2 * H), 2 * I);
   a.xs = W.ys; a.yb = W.part; a.ldy = H;
   if ((r = hb_launch(ctx, "fp8_gemm_down", pdl, kd.fn, dim3(grid), dim3(F8_THREADS), (size_t)kd.smem, st, a, ty, ty))) return r;
-  return hb_launch(ctx, "fp8_sum", false, fp8_sum_kernel, dim3(M), dim3(256), 0, st, (const __nv_bfloat16*)W.part, (const int*)W.pos_of, w, K, H, out,
-                   cmb ? reinterpret_cast<const __nv_bfloat16*>(cmb->shared) : (const __nv_bfloat16*)nullptr, cmb && cmb->shared ? cmb->lg : (const float*)nullptr, cmb ? cmb->ld : 0,
-                   cmb ? cmb->col : 0, cmb ? reinterpret_cast<__nv_bfloat16*>(cmb->out) : (__nv_bfloat16*)nullptr);
+  F8SumArgs su{W.part, W.pos_of, w, M, K, H, out, nullptr, nullptr, 0, 0, nullptr};
+  if (cmb) {
+    su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
+    if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
+  }
+  const long long ctas = ((long long)M * (H / 8) + F8_SUM_THREADS - 1) / F8_SUM_THREADS, cap = (long long)ctx->sm_count * 16;
+  return hb_launch(ctx, "fp8_sum", pdl, fp8_sum_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(F8_SUM_THREADS), 0, st, su);
 }
 
 }  // extern "C"

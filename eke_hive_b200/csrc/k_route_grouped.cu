@@ -3,28 +3,27 @@
 //   a group's value = the sum of its group_top (1 or 2) largest c; the topk_group groups of the largest values stay,
 //   the k experts of the largest c among theirs are picked, best first (ties: the smaller index, for groups and experts),
 //   w = s of the pick, divided by (the picks' sum + 1e-20) when renorm is set, times scale.
-// The selection is that of exact arithmetic as far as 64 bits tell: scores, sums and comparisons are fp64.
+// The selection is that of 64-bit arithmetic.
 #include "hb_common.cuh"
 #include "hb_kernels.h"
 
 namespace hb {
 
+// One warp takes a row.  The scores are worked out in fp32 with an error bound, and so is the selection; wherever two neighbours of the result (two
+// picks next to each other, the last pick and the best expert left out, the last group kept and the best one dropped) are closer than
+// their bounds, and are not equal by their inputs, 64 bits decide: between experts for the candidates alone, a lane each; between groups, and for scores at
+// the end of fp32's range, the warp does the whole row again.  64 bits for every row took 37 us for 8192 rows of 256 experts and 12 us for one.
 constexpr int RG_WARPS = 4;
 
 struct RouteGroupedArgs {
   const float* logits; int ld, M, E, k, n_group, topk_group, group_top, sigmoid, renorm; const float* bias; float scale; int32_t* ids; float* w;
 };
 
-// a before b: the larger value, the smaller index among equals; NaN comes after everything
+// a before b: the larger value, the smaller index among equals
 __device__ __forceinline__ bool rg_before(double a, int ia, double b, int ib) { return a > b || (a == b && ia < ib); }
 
-__global__ void __launch_bounds__(RG_WARPS * 32) route_grouped_kernel(const RouteGroupedArgs a) {
-  extern __shared__ double rg_sm[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = blockIdx.x * RG_WARPS + warp;
-  griddep_wait();
-  if (m >= a.M) return;
-  double* c = rg_sm + (size_t)warp * a.E;
-  const float* lr = a.logits + (size_t)m * a.ld;
+// A row in 64 bits; c: E doubles of shared memory of the warp's own.  Lane l < k gets pick l.
+__device__ __noinline__ void route_grouped_row64(const RouteGroupedArgs& a, const float* lr, double* c, int lane, int& id, float& w) {
   auto logit = [&](int e) -> double { const float v = lr[e]; return v == v ? (double)v : -INFINITY; };   // NaN counts as -inf
   double mx = -INFINITY, sum = 0.0;
   if (!a.sigmoid) {
@@ -35,11 +34,11 @@ __global__ void __launch_bounds__(RG_WARPS * 32) route_grouped_kernel(const Rout
   }
   auto score = [&](int e) -> double {
     if (a.sigmoid) return 1.0 / (1.0 + exp(-logit(e)));
-    return mx == -INFINITY ? 0.0 : exp(logit(e) - mx) / sum;                 // a row without a finite logit: all scores 0
+    return mx == -INFINITY ? 0.0 : exp(logit(e) - mx) / sum;                     // a row without a finite logit: all scores 0
   };
   for (int e = lane; e < a.E; e += 32) {
     const double v = score(e) + (a.bias ? (double)a.bias[e] : 0.0);
-    c[e] = v == v ? v : -INFINITY;                                               // NaN is picked last
+    c[e] = v == v ? v : -INFINITY;
   }
   __syncwarp();
   const int size = a.E / a.n_group;
@@ -57,7 +56,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) route_grouped_kernel(const Rout
   }
   uint32_t gone = 0u;                                                            // bit j: expert lane + 32 j is not to be had
   for (int j = 0, e = lane; e < a.E; ++j, e += 32) if (!((keep >> (e / size)) & 1u)) gone |= 1u << j;
-  int id = 0;
+  id = 0;
   for (int r = 0; r < a.k; ++r) {
     double b = -INFINITY; int at = 0x7fffffff;
     for (int j = 0, e = lane; e < a.E; ++j, e += 32) {
@@ -75,7 +74,183 @@ __global__ void __launch_bounds__(RG_WARPS * 32) route_grouped_kernel(const Rout
   if (!(s == s)) s = 0.0;
   for (int r = 0; r < a.k; ++r) tot += __shfl_sync(0xffffffffu, s, r);
   if (a.renorm) s /= tot + 1e-20;
-  if (lane < a.k) { a.ids[(size_t)m * a.k + lane] = id; a.w[(size_t)m * a.k + lane] = (float)(s * (double)a.scale); }
+  w = (float)(s * (double)a.scale);
+}
+
+__device__ __forceinline__ uint32_t rg_key(float v) {                            // orders like the value; 0 is below everything
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float rg_val(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+
+// The row in fp32; R: experts a lane holds (e = lane + 32 j).  Returns false where fp32 does not settle the selection.
+template <int R>
+__device__ __forceinline__ bool route_grouped_row32(const RouteGroupedArgs& a, const float* lr, float* c, int lane, int& id, float& w) {
+  float s[R]; uint32_t key[R];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int e = lane + 32 * j;
+    s[j] = e < a.E ? __ldg(lr + e) : -INFINITY;
+    if (!(s[j] == s[j])) s[j] = -INFINITY;
+    mx = fmaxf(mx, s[j]);
+  }
+  // Error of a score, against the other scores of the row.  sigmoid: expf (a step), 1 + e and the reciprocal (half a step each), relative; with a bias it counts against scores up to 1.
+  // softmax: l - max = -d is off by half a step of d, expf and the product by a few, the sum (the same for all) by some 40 half steps.  Without a bias
+  // the sum does not count, and d < 63 (err() sees to it): (63 + 6) half steps, relative.  With one: e^-d (d + 46) half steps of the largest score.
+  float eps = 0x1p-22f;
+  bool safe = true;
+  if (a.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) s[j] = __frcp_rn(1.f + expf(-s[j]));
+  } else {
+    mx = rg_val(__reduce_max_sync(0xffffffffu, rg_key(mx)));
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < R; ++j) { s[j] = expf(s[j] - mx); sum += s[j]; }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float r = __frcp_rn(sum);
+#pragma unroll
+    for (int j = 0; j < R; ++j) s[j] *= r;
+    eps = a.bias ? r * 0x1p-18f : 0x1p-17f;
+    safe = mx > -INFINITY && mx < INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int e = lane + 32 * j;
+    const float v = e < a.E ? s[j] + (a.bias ? __ldg(a.bias + e) : 0.f) : 0.f;
+    if (e < a.E) c[e] = v;
+    key[j] = e < a.E ? rg_key(v) : 0u;
+  }
+  __syncwarp();
+  // bound of the error of a value v = score + bias; scores below 2^-90 have none where they stand alone
+  auto err = [&](float v) { return a.bias ? fmaf(fabsf(v), 0x1p-23f, eps) : v > 0x1p-90f ? v * (eps + 0x1p-23f) : INFINITY; };
+  if (a.topk_group < a.n_group) {
+    const int size = a.E / a.n_group;
+    int T = 1, lg = 0;                                                           // lanes a group gets: a power of two
+    while (2 * T * a.n_group <= 32) { T *= 2; ++lg; }
+    const int g = lane >> lg, t = lane & (T - 1);
+    float t1 = -INFINITY, t2 = -INFINITY;
+    if (g < a.n_group) {
+#pragma unroll 4
+      for (int i = t; i < size; i += T) { const float x = c[g * size + i]; t2 = fmaxf(t2, fminf(t1, x)); t1 = fmaxf(t1, x); }
+    }
+    for (int o = T >> 1; o > 0; o >>= 1) {
+      const float o1 = __shfl_xor_sync(0xffffffffu, t1, o), o2 = __shfl_xor_sync(0xffffffffu, t2, o);
+      t2 = fmaxf(fmaxf(t2, o2), fminf(t1, o1)); t1 = fmaxf(t1, o1);
+    }
+    const bool two = a.group_top == 2 && size > 1;
+    float v = two ? t1 + t2 : t1, ve = two ? err(t1) + err(t2) + fabsf(v) * 0x1p-23f : err(t1);
+    v = __shfl_sync(0xffffffffu, v, (lane << lg) & 31); ve = __shfl_sync(0xffffffffu, ve, (lane << lg) & 31);   // lane g: group g
+    int rank = 0;
+    for (int i = 0; i < a.n_group; ++i) { const float ov = __shfl_sync(0xffffffffu, v, i); rank += ov > v || (ov == v && i < lane); }
+    const bool in = lane < a.n_group;
+    const uint32_t keep = __ballot_sync(0xffffffffu, in && rank < a.topk_group);
+    // the lowest a kept group can be against the highest a dropped one can be
+    const float lo = rg_val(__reduce_min_sync(0xffffffffu, in && rank < a.topk_group ? rg_key(v - ve) : 0xffffffffu));
+    const float hi = rg_val(__reduce_max_sync(0xffffffffu, in && rank >= a.topk_group ? rg_key(v + ve) : 0u));
+    safe = safe && lo > hi;
+    const uint32_t mul = 0xffffffffu / (uint32_t)size + 1u;                      // e / size for e < 2^10
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const uint32_t e = lane + 32 * j;
+      if (!((keep >> ((size == 1 ? e : __umulhi(e, mul)) & 31u)) & 1u)) key[j] = 0u;
+    }
+  }
+  // k picks and the best one left out, lane r the r-th
+  uint32_t mykey = 0u; id = 0;
+  auto pick = [&](int r) -> uint32_t {
+    uint32_t best = 0u; int at = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) if (key[j] > best) { best = key[j]; at = j; }
+    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t e = __reduce_min_sync(0xffffffffu, best == m && m ? (uint32_t)(lane + 32 * at) : 0x7fffffffu);
+    if (lane == r) { mykey = m; id = (int)e; }
+    if ((e & 31u) == (uint32_t)lane && m) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) if (j == (int)(e >> 5)) key[j] = 0u;
+    }
+    return m;
+  };
+#pragma unroll 1
+  for (int r = 0; r <= a.k; ++r) pick(r);
+  auto inputs = [&](float& l, float& b) {                                        // of the lane's pick
+    l = mykey ? __ldg(lr + id) : -INFINITY;
+    if (!(l == l)) l = -INFINITY;
+    b = mykey && a.bias ? __ldg(a.bias + id) : 0.f;
+  };
+  float l, b;
+  inputs(l, b);
+  const float v = rg_val(mykey), vn = __shfl_down_sync(0xffffffffu, v, 1);
+  const float ln = __shfl_down_sync(0xffffffffu, l, 1), bn = __shfl_down_sync(0xffffffffu, b, 1);
+  const bool next = __shfl_down_sync(0xffffffffu, mykey, 1) != 0u;               // (there may be no expert left to be left out)
+  const bool close = lane < a.k && next && !(v - vn > err(v) + err(vn)) && !(l == ln && b == bn);
+  safe = safe && !__any_sync(0xffffffffu, lane < a.k && mykey == 0u);
+  if (!safe) return false;
+  if (__any_sync(0xffffffffu, close)) {
+    // Neighbours too close for fp32: everyone that may belong among the picks, a lane each, put in order in 64 bits
+    int n = a.k + 1;
+    const float vk = __shfl_sync(0xffffffffu, v, a.k - 1);
+    for (bool more = true; more;) {
+      const float vl = rg_val(__shfl_sync(0xffffffffu, mykey, n - 1));
+      if (__shfl_sync(0xffffffffu, mykey, n - 1) == 0u) { --n; break; }
+      if (vk - vl > err(vk) + err(vl)) break;
+      if (n == 32) return false;
+      pick(n++);
+    }
+    inputs(l, b);
+    double d = 0.0;
+    if (a.sigmoid) d = 1.0 / (1.0 + exp(-(double)l));
+    else {
+      d = exp((double)l - (double)mx);                                           // without a bias the sum changes no order
+      if (a.bias) {
+        double sum = 0.0;
+        for (int e = lane; e < a.E; e += 32) { const float x = __ldg(lr + e); if (x == x) sum += exp((double)x - (double)mx); }
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        d /= sum;
+      }
+    }
+    d += (double)b;
+    int rank = 0;
+    for (int i = 0; i < n; ++i) { const double od = __shfl_sync(0xffffffffu, d, i); const int oi = __shfl_sync(0xffffffffu, id, i); rank += rg_before(od, oi, d, id); }
+    __syncwarp();
+    int* ids = reinterpret_cast<int*>(c);
+    if (lane < n) { ids[rank] = id; ids[32 + rank] = (int)mykey; }
+    __syncwarp();
+    if (lane < a.k) { id = ids[lane]; mykey = (uint32_t)ids[32 + lane]; }
+    __syncwarp();
+    inputs(l, b);
+  }
+  float sc = 0.f;
+  if (lane < a.k) sc = a.sigmoid ? __frcp_rn(1.f + expf(-l)) : a.bias ? 0.f : rg_val(mykey);
+  if (!a.sigmoid && a.bias) {                                                    // the softmax score of a pick, from the lane that has it
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < R; ++j) { const int e = lane + 32 * j; if (e < a.E) c[e] = s[j]; }
+    __syncwarp();
+    if (lane < a.k) sc = c[id];
+  }
+  if (__any_sync(0xffffffffu, lane < a.k && l > -INFINITY && sc < 0x1p-100f)) return false;   // a score near the end of fp32's range is itself not exact
+  float tot = 0.f;
+  for (int r = 0; r < a.k; ++r) tot += __shfl_sync(0xffffffffu, sc, r);
+  w = (a.renorm ? __fdiv_rn(sc, tot + 1e-20f) : sc) * a.scale;
+  return true;
+}
+
+template <int R>
+__global__ void __launch_bounds__(RG_WARPS * 32) route_grouped_kernel(const RouteGroupedArgs a) {
+  extern __shared__ double rg_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = blockIdx.x * RG_WARPS + warp;
+  griddep_wait();
+  if (m >= a.M) return;
+  double* c = rg_sm + (size_t)warp * max(a.E, 32);
+  const float* lr = a.logits + (size_t)m * a.ld;
+  int id; float w;
+  if (!route_grouped_row32<R>(a, lr, reinterpret_cast<float*>(c), lane, id, w)) {
+    __syncwarp();
+    route_grouped_row64(a, lr, c, lane, id, w);
+  }
+  if (lane < a.k) { a.ids[(size_t)m * a.k + lane] = id; a.w[(size_t)m * a.k + lane] = w; }
 }
 
 }  // namespace hb
@@ -95,6 +270,7 @@ extern "C" int hb_route_grouped_topk(hb_ctx* ctx, const float* logits, int ld, i
   HB_REQUIRE(ctx, (group_top == 1 || group_top == 2) && (score == HB_SCORE_SOFTMAX || score == HB_SCORE_SIGMOID), HB_ERR_INVALID,
              "route_grouped_topk: group_top=%d (1 or 2) score=%d", group_top, score);
   RouteGroupedArgs a{logits, ld, M, E, k, n_group, topk_group, group_top, score == HB_SCORE_SIGMOID, renorm, bias, scale, ids, w};
-  return hb_launch(ctx, "route_grouped", !(ctx->flags & HB_FLAG_NO_PDL), route_grouped_kernel, dim3((M + RG_WARPS - 1) / RG_WARPS), dim3(RG_WARPS * 32),
-                   (size_t)RG_WARPS * E * 8, reinterpret_cast<cudaStream_t>(stream), a);
+  auto fn = E <= 128 ? route_grouped_kernel<4> : E <= 256 ? route_grouped_kernel<8> : E <= 512 ? route_grouped_kernel<16> : route_grouped_kernel<32>;
+  return hb_launch(ctx, "route_grouped", !(ctx->flags & HB_FLAG_NO_PDL), fn, dim3((M + RG_WARPS - 1) / RG_WARPS), dim3(RG_WARPS * 32),
+                   (size_t)RG_WARPS * (E > 32 ? E : 32) * 8, reinterpret_cast<cudaStream_t>(stream), a);
 }

@@ -34,8 +34,17 @@ def _p(t):
     return int(t)
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
+def _stream(device: int | None = None):
+    # the stream's handle without the Python object around it: a third of what a call costs on the host
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
+
+
+def _here(t: torch.Tensor, ctx: "Context | None"):
+    """(context, stream handle) of a call on tensor t: t, the context and the current device have to be the same device."""
+    d = torch.cuda.current_device()
+    if t.device.index != d or (ctx is not None and ctx.device != d):
+        raise HbError(-1, f"tensor on {t.device}, context on cuda:{d if ctx is None else ctx.device}, current device cuda:{d}: they have to be the same")
+    return ctx or context(d), torch._C._cuda_getCurrentRawStream(d)
 
 
 class Context:
@@ -201,14 +210,16 @@ def router_grouped_topk(logits: torch.Tensor, k: int, n_group: int = 1, topk_gro
                         renorm: bool = True, scale: float = 1.0, E: int | None = None, ids=None, w=None, ctx: Context | None = None):
     """hb_route_grouped_topk: top-k among the experts of the topk_group best of n_group groups; score "sigmoid" or "softmax", selection on
     score + bias, weights from the score alone.  logits fp32 [M, ld]; returns ids int32 [M, k], w fp32 [M, k]."""
-    ctx = ctx or context()
-    M, ld = logits.shape[0], logits.stride(0)
-    E = logits.shape[1] if E is None else E
-    ids = torch.empty((M, k), dtype=torch.int32, device=logits.device) if ids is None else ids
-    w = torch.empty((M, k), dtype=torch.float32, device=logits.device) if w is None else w
-    ctx.check(_L().hb_route_grouped_topk(ctx.handle, _p(logits), ld, M, E, k, n_group, topk_group, group_top, {"softmax": 0, "sigmoid": 1}[score], _p(bias),
-                                         int(renorm), scale, _p(ids), _p(w), _stream()))
+    ctx, st = _here(logits, ctx)
+    M, cols = logits.shape
+    ids = logits.new_empty((M, k), dtype=torch.int32) if ids is None else ids
+    w = logits.new_empty((M, k)) if w is None else w
+    ctx.check(_L().hb_route_grouped_topk(ctx.handle, _p(logits), _rows(logits), M, cols if E is None else E, k, n_group, topk_group, group_top, _SCORE[score],
+                                         _p(bias), renorm, scale, _p(ids), _p(w), st))
     return ids, w
+
+
+_SCORE = {"softmax": 0, "sigmoid": 1}
 
 
 def rec_table(recs: list[torch.Tensor | None]) -> torch.Tensor:
@@ -399,23 +410,24 @@ def _rows(t):
 
 def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     """hb_fp8_quant_rows: x bf16 [M, K] → (codes u8 [M, K], scales fp32 [ceil(K/128), M])."""
-    ctx = ctx or context()
+    ctx, st = _here(x, ctx)
     assert x.dtype == torch.bfloat16
     M, K = x.shape
-    q = torch.empty((M, K), dtype=torch.uint8, device=x.device) if q is None else q
-    s = torch.empty((-(-K // 128), M), dtype=torch.float32, device=x.device) if s is None else s
-    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, _p(x), _rows(x), M, K, _p(q), _rows(q), _p(s), _rows(s), _stream()))
+    q = x.new_empty((M, K), dtype=torch.uint8) if q is None else q
+    s = x.new_empty((-(-K // 128), M), dtype=torch.float32) if s is None else s
+    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, _p(x), _rows(x), M, K, _p(q), _rows(q), _p(s), _rows(s), st))
     return q, s
 
 
 def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     """hb_fp8_quantize: a weight fp32 or bf16 [N, K] → (codes u8 [N, K], scales fp32 [ceil(N/128), ceil(K/128)])."""
-    ctx = ctx or context()
-    assert w.dtype in (torch.float32, torch.bfloat16) and w.is_contiguous()
+    ctx, st = _here(w, ctx)
+    bf16 = w.dtype == torch.bfloat16
+    assert (bf16 or w.dtype == torch.float32) and w.is_contiguous()
     N, K = w.shape
-    q = torch.empty((N, K), dtype=torch.uint8, device=w.device) if q is None else q
-    s = torch.empty((-(-N // 128), -(-K // 128)), dtype=torch.float32, device=w.device) if s is None else s
-    ctx.check(_L().hb_fp8_quantize(ctx.handle, _p(w), int(w.dtype == torch.bfloat16), N, K, _p(q), _p(s), _stream()))
+    q = w.new_empty((N, K), dtype=torch.uint8) if q is None else q
+    s = w.new_empty((-(-N // 128), -(-K // 128)), dtype=torch.float32) if s is None else s
+    ctx.check(_L().hb_fp8_quantize(ctx.handle, _p(w), bf16, N, K, _p(q), _p(s), st))
     return q, s
 
 
@@ -425,12 +437,12 @@ def fp8_gemm_ws_bytes(M: int, N: int, K: int) -> int:
 
 def fp8_gemm(W: GMat, xq, xs, out_dtype=torch.bfloat16, y=None, ws=None, ctx: Context | None = None):
     """hb_fp8_gemm: y [M, N] (bf16 or fp32) = rows quantised by fp8_quant_rows times the block-scaled matrix W (FMT_FP8_B128)."""
-    ctx = ctx or context()
+    ctx, st = _here(xq, ctx)
     M = xq.shape[0]
-    y = torch.empty((M, W.N), dtype=out_dtype, device=xq.device) if y is None else y
-    ws = torch.empty(fp8_gemm_ws_bytes(M, W.N, W.K), dtype=torch.uint8, device=xq.device) if ws is None else ws
+    y = xs.new_empty((M, W.N), dtype=out_dtype) if y is None else y
+    ws = xq.new_empty(_L().hb_fp8_gemm_ws_bytes(M, W.N, W.K), dtype=torch.uint8) if ws is None else ws
     yb, yf = (_p(y), None) if y.dtype == torch.bfloat16 else (None, _p(y))
-    ctx.check(_L().hb_fp8_gemm(ctx.handle, C.byref(W.c), _p(xq), _rows(xq), _p(xs), _rows(xs), M, yb, yf, _rows(y), _p(ws), _stream()))
+    ctx.check(_L().hb_fp8_gemm(ctx.handle, C.byref(W.c), _p(xq), _rows(xq), _p(xs), _rows(xs), M, yb, yf, _rows(y), _p(ws), st))
     return y
 
 
@@ -467,14 +479,15 @@ def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg
             ws=None, ctx: Context | None = None):
     """hb_moe_fp8: routed experts of FP8 records for any number of rows; ids int32 / w fp32 [M, K], x bf16 [M, H].  bf16 out adds the gated shared
     rows where given; out_dtype (or out.dtype) float32 gives the routed sum alone."""
-    ctx = ctx or context()
+    ctx, st = _here(x, ctx)
     M, K = ids.shape
     assert x.is_contiguous() and ids.is_contiguous() and w.is_contiguous()
-    out = torch.empty((M, H), dtype=out_dtype, device=x.device) if out is None else out
-    ws = torch.empty(moe_fp8_ws_bytes(M, K, E, H, I), dtype=torch.uint8, device=x.device) if ws is None else ws
+    out = x.new_empty((M, H), dtype=out_dtype) if out is None else out
+    ws = x.new_empty(_L().hb_moe_fp8_ws_bytes(M, K, E, H, I), dtype=torch.uint8) if ws is None else ws
+    assert out.is_contiguous() and (shared is None or shared.is_contiguous())
     assert out.dtype == torch.bfloat16 or (shared is None and lg is None), "shared rows are added to a bf16 output"
     cmb = C.byref(PfCombine(_p(shared), _p(lg), 0 if lg is None else lg.stride(0), col, _p(out))) if out.dtype == torch.bfloat16 else None
-    ctx.check(_L().hb_moe_fp8(ctx.handle, _p(ids), _p(w), M, K, _p(rec_tab), li, E, _p(x), H, I, limit, None if cmb else _p(out), cmb, _p(ws), _stream()))
+    ctx.check(_L().hb_moe_fp8(ctx.handle, _p(ids), _p(w), M, K, _p(rec_tab), li, E, _p(x), H, I, limit, None if cmb else _p(out), cmb, _p(ws), st))
     return out
 
 
