@@ -28,6 +28,9 @@ enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
 constexpr int F8_MAX_CTAS = 160;                       // grid at most; the workspace holds two partial items of each
 constexpr int F8_COUNTERS = 2 * F8_MAX_CTAS;           // items that are cut, at most
 constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
+constexpr int F8_STG_PITCH = 80, F8_STG_BYTES = 32 * F8_STG_PITCH;   // a warp's staging: 32 rows of 64 bytes (pitch: 16-byte accesses without bank conflicts)
+constexpr int F8_REGS = 168, F8_REGS_SUM = 216, F8_REGS_REST = 72;   // a thread's at launch (hbk_fp8_setup checks it), then of the sums' and of the other warps
+static_assert(8 * F8_REGS_SUM + 4 * F8_REGS_REST <= 12 * F8_REGS, "register split");
 constexpr int F8_A_BYTES = 128 * 128;                  // a tile of weights: 128 rows × 128 values
 
 template <int BN_>
@@ -37,7 +40,9 @@ struct F8Cfg {
   static constexpr int ST = 200 * 1024 / STAGE;        // ring of operand stages
   static constexpr int TMEM = BN <= 16 ? 64 : 4 * BN;  // two buffers of two tiles
   static constexpr int LD = CW < 32 ? CW : 32;         // columns read at a time
-  static constexpr int SMEM = 1024 + ST * STAGE + 2 * 2 * BN * 4 + 2 * 4 * CW * 4 + 512;
+  static constexpr int NCH = 2 * CW / LD;              // reads a step takes: even
+  static constexpr bool SPLIT = BN >= 64;              // the sums need more registers than a twelfth of the file: the other warps give some of theirs
+  static constexpr int SMEM = 1024 + ST * STAGE + 4 * 2 * BN * 4 + 8 * CW * 4 + 512;
   static_assert(F8_COUNTERS <= kErrCounterWords, "counters of the context");
   static_assert(SMEM <= 227 * 1024 && TMEM <= 512 && STAGE % 1024 == 0, "shared memory, tensor memory, swizzle atoms");
 };
@@ -56,32 +61,32 @@ struct F8Args {
 };
 
 // The steps of a CTA, the same for all its warps: segments (item, first step, end).
-struct F8Sched {
-  int items, KB, G, dp, sk; long long U; int Gs;
-  long long u, u1; int i;
-  __device__ __forceinline__ void init(int items_, int KB_) {
-    items = items_; KB = KB_; G = gridDim.x;
-    const int waves = items / G, rem = items - waves * G;
-    dp = rem == 0 ? waves : max(waves - 1, 0);         // rounds of whole items, after the cut ones
+struct F8Sched {                                       // (32 bits: at most 320 cut items of at most 2^16 steps, times 160 CTAs)
+  uint32_t KB, G, me, dp, sk, U, Gs, u, u1, i;
+  // even: with fewer items than CTAs cut every one into the same number of runs and leave CTAs without work
+  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool even) {
+    KB = KB_; G = G_; me = me_;
+    const uint32_t waves = items / G, rem = items - waves * G;
+    dp = rem == 0u ? waves : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
     sk = items - dp * G;
-    U = (long long)sk * KB;
-    Gs = (int)min((long long)G, max(U, 1ll));          // CTAs that get a run of steps: none is empty
-    u = start(blockIdx.x); u1 = start(blockIdx.x + 1);
-    i = 0;
+    U = sk * KB;
+    Gs = min(even && waves == 0u && items > 0u ? G / items * items : G, max(U, 1u));   // CTAs that get a run of steps: none is empty
+    u = start(me); u1 = start(me + 1u);
+    i = 0u;
   }
-  __device__ __forceinline__ long long start(int c) const { return c >= Gs ? U : (long long)c * U / Gs; }
+  __device__ __forceinline__ uint32_t start(uint32_t c) const { return c >= Gs ? U : c * U / Gs; }
   __device__ __forceinline__ bool next(int& item, int& kb0, int& kb1) {
     if (u < u1) {
-      item = (int)(u / KB); kb0 = (int)(u - (long long)item * KB);
-      kb1 = (int)min((long long)KB, kb0 + (u1 - u));
-      u += kb1 - kb0;
+      item = (int)(u / KB); kb0 = (int)(u - (uint32_t)item * KB);
+      kb1 = (int)min(KB, kb0 + (u1 - u));
+      u += (uint32_t)(kb1 - kb0);
       return true;
     }
     if (i >= dp) return false;
-    item = sk + i * G + blockIdx.x; kb0 = 0; kb1 = KB; ++i;
+    item = (int)(sk + i * G + me); kb0 = 0; kb1 = (int)KB; ++i;
     return true;
   }
-  __device__ __forceinline__ int owner(long long step) const { return (int)(((step + 1) * Gs - 1) / U); }
+  __device__ __forceinline__ uint32_t owner(uint32_t step) const { return ((step + 1u) * Gs - 1u) / U; }
 };
 
 __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -95,10 +100,71 @@ __device__ __forceinline__ void f8_fma2(float& a0, float& a1, uint32_t d0, uint3
   asm("{\n .reg .b64 a, d, s;\n mov.b64 a, {%0, %1};\n mov.b64 d, {%2, %3};\n mov.b64 s, {%4, %5};\n fma.rn.f32x2 a, d, s, a;\n mov.b64 {%0, %1}, a;\n}"
       : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
 }
+__device__ __forceinline__ float f8_swiglu(float g, float u, float limit) {
+  if (limit > 0.f) { g = fminf(g, limit); u = fminf(fmaxf(u, -limit), limit); }
+  return g / (1.f + expf(-g)) * u;
+}
+__device__ __forceinline__ uint4 f8_pack8(const float* v) {                     // eight values as bf16
+  uint32_t p[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]); p[j] = *reinterpret_cast<const uint32_t*>(&b); }
+  return make_uint4(p[0], p[1], p[2], p[3]);
+}
+// A warp's staged 32 rows × 64 bytes to memory, eight rows an instruction (a lane has a row: its own stores would touch 32 rows each).  to: the first
+// row's place; bytes: how much of a row there is room for; es: bytes of an element.
+__device__ __forceinline__ void f8_flush(const uint8_t* stg, uint8_t* to, size_t ld, int rows, int bytes, int es, int lane) {
+  __syncwarp();
+  const int c = (lane & 3) * 16;
+  const bool wide = ((reinterpret_cast<uintptr_t>(to) | ld) & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2);
+    const uint4 v = *reinterpret_cast<const uint4*>(stg + r * F8_STG_PITCH + c);
+    if (r >= rows) continue;
+    uint8_t* p = to + (size_t)r * ld + c;
+    if (wide && c + 16 <= bytes) *reinterpret_cast<uint4*>(p) = v;
+    else if (c < bytes) {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (es == 4) { if (c + 4 * j < bytes) *reinterpret_cast<uint32_t*>(p + 4 * j) = w[j]; }
+        else {
+          if (c + 4 * j < bytes) *reinterpret_cast<uint16_t*>(p + 4 * j) = (uint16_t)(w[j] & 0xffffu);
+          if (c + 4 * j + 2 < bytes) *reinterpret_cast<uint16_t*>(p + 4 * j + 2) = (uint16_t)(w[j] >> 16);
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+template <int W>
+__device__ __forceinline__ void f8_add(float* acc, const uint32_t (&d)[W], const float* s) {
+#pragma unroll
+  for (int c = 0; c < W; c += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(s + c);
+    f8_fma2(acc[c], acc[c + 1], d[c], d[c + 1], v.x, v.y);
+    f8_fma2(acc[c + 2], acc[c + 3], d[c + 2], d[c + 3], v.z, v.w);
+  }
+}
+template <int W>
+__device__ __forceinline__ void f8_add(float* acc, const uint32_t (&d)[W], float s) {
+#pragma unroll
+  for (int c = 0; c < W; c += 2) f8_fma2(acc[c], acc[c + 1], d[c], d[c + 1], s, s);
+}
 __device__ __forceinline__ bool named_bar_and(int id, int threads, bool v) {   // barrier of `threads` threads; true where all bring true
   uint32_t o;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(o) : "r"(id), "r"(threads), "r"((uint32_t)v) : "memory");
   return o != 0;
+}
+// The columns asked for before have arrived; the registers are named so that nothing that reads them is moved in front of it.
+template <int W>
+__device__ __forceinline__ void f8_landed(uint32_t (&r)[W], uint32_t (&p)[W]) {
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < W; i += 8) {
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+    asm volatile("" : "+r"(p[i]), "+r"(p[i + 1]), "+r"(p[i + 2]), "+r"(p[i + 3]), "+r"(p[i + 4]), "+r"(p[i + 5]), "+r"(p[i + 6]), "+r"(p[i + 7]));
+  }
 }
 template <int W>
 __device__ __forceinline__ void f8_ld(uint32_t taddr, uint32_t (&r)[W]) {
@@ -113,8 +179,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   extern __shared__ uint8_t f8_raw[];
   const uint32_t raw = smem_u32(f8_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* sm = f8_raw + (base - raw);
-  float* scl = reinterpret_cast<float*>(sm + C::ST * C::STAGE);              // [2 buffers][2 tiles][BN]
-  uint32_t* amx = reinterpret_cast<uint32_t*>(scl + 4 * BN);                 // [2 halves][4 warps][CW]: magnitudes of y
+  // Scales of a step [step mod 4][2 tiles][BN]: a warp may still read those of a step whose sums it has taken out, while the next two's are written
+  float* scl = reinterpret_cast<float*>(sm + C::ST * C::STAGE);
+  uint32_t* amx = reinterpret_cast<uint32_t*>(scl + 8 * BN);                 // magnitudes of y: [2 halves][4 warps][CW]
   uint64_t* full = reinterpret_cast<uint64_t*>(amx + 8 * C::CW);             // [ST] the stage's operands have landed
   uint64_t* empty = full + C::ST;                                            // [ST] the MMAs that read them are done
   uint64_t* acc_full = empty + C::ST;                                        // [2] the buffer's sums and scales are there
@@ -138,13 +205,15 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   griddep_launch();
   const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  sch.init(n_tiles * a.n_nt, KB);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
   auto tile_of = [&](int ti) -> TileRef {
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
   };
   int item, kb0, kb1;
 
+  if (warp >= 8) {
+  if constexpr (C::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_REGS_REST));
   if (warp == F8_W_TMA) {
     // ------------------------------------------------------------------------------------------------ operand tiles, one thread
     if (elect_one()) {
@@ -198,7 +267,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
 #pragma unroll
           for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)                                   // 32 values further along the swizzled rows
+            for (uint32_t j = 0; j < 4; ++j)                                 // 32 values further along the swizzled rows
               tc_mma_f8(d + u * BN, ad + u * (F8_A_BYTES >> 4) + 2 * j, bd + 2 * j, idesc, j);
           tc_commit(&empty[s]);
           tc_commit(&acc_full[buf]);
@@ -240,7 +309,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
         ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x2000u);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        float* d = scl + buf * (2 * BN);
+        float* d = scl + (it & 3u) * (2 * BN);
 #pragma unroll
         for (int i = 0; i < NL; ++i)
           if (BN >= 32 || lane < BN) { d[lane + 32 * i] = x[i] * s0; d[BN + lane + 32 * i] = x[i] * s1; }
@@ -248,8 +317,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
         if (lane == 0) mbar_arrive(&acc_full[buf]);
       }
     }
-  } else if (warp < 8) {
-    // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has lanes [32 q, 32 q + 32), columns [h·CW, (h + 1)·CW)
+  }
+  } else {
+    if constexpr (C::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
+    // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has lanes [32 q, 32 q + 32) and of each weight
+    // tile's columns [h·CW, (h + 1)·CW): a lane is a weight row, a column a row of x with a scale of its own, read from shared memory by all lanes together
     const int h = warp >> 2, q = warp & 3, row = 32 * q + lane;
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + h * C::CW;
     uint32_t it = 0;
@@ -258,91 +330,125 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
       const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
       const TileRef tl = tile_of(ti);
       const int cols = min(max(tl.rows - h * C::CW, 0), C::CW);                // this warp's columns that hold rows of x
+      const bool active = cols > 0;
       float acc[2][C::CW];
 #pragma unroll
       for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t buf = it & 1u;
-        ok = mbar_wait(&acc_full[buf], (it >> 1) & 1u, a.err, 0x1000u);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      // Read i of a buffer: columns (i mod NCH / 2)·LD of tile i / (NCH / 2).  A wait for reads waits for all that are under way, so two go out together,
+      // each as soon as the registers it writes have been added up (one at a time, each behind the other's additions: 730 clocks a step of 256 columns)
+      uint32_t ra[C::LD], rb[C::LD];
+      auto arrived = [&](uint32_t n) {
+        const bool o = mbar_wait(&acc_full[n & 1u], (n >> 1) & 1u, a.err, 0x1000u);
         tc_fence_after();
+        return (bool)__all_sync(0xffffffffu, o);
+      };
+      auto read2 = [&](uint32_t t, int n) {
+        constexpr int half = C::NCH / 2;
+        f8_ld<C::LD>(t + (n / half) * BN + (n % half) * C::LD, ra);
+        f8_ld<C::LD>(t + ((n + 1) / half) * BN + ((n + 1) % half) * C::LD, rb);
+      };
+      if ((ok = arrived(it)) && active) read2(trow + (it & 1u) * (2 * BN), 0);
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+        const uint32_t buf = it & 1u, tb = trow + buf * (2 * BN);
+        const float* sb = scl + (it & 3u) * (2 * BN) + h * C::CW;
+        constexpr int half = C::NCH / 2;
+        auto add = [&](float* to, const uint32_t (&d)[C::LD], int u, int c0) {
+          f8_add<C::LD>(to, d, sb + u * BN + c0);
+        };
+        if (active) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int c0 = 0; c0 < C::CW; c0 += C::LD) {
-            if (c0 < cols) {
-              uint32_t r[C::LD];
-              f8_ld<C::LD>(trow + buf * (2 * BN) + u * BN + c0, r);
-              const float4* s4 = reinterpret_cast<const float4*>(scl + buf * (2 * BN) + u * BN + h * C::CW + c0);
-              tc_wait_ld();
-#pragma unroll
-              for (int c = 0; c < C::LD; c += 4) {
-                const float4 sv = s4[c / 4];
-                f8_fma2(acc[u][c0 + c], acc[u][c0 + c + 1], r[c], r[c + 1], sv.x, sv.y);
-                f8_fma2(acc[u][c0 + c + 2], acc[u][c0 + c + 3], r[c + 2], r[c + 3], sv.z, sv.w);
-              }
+          for (int i = 0; i < C::NCH; i += 2) {
+            f8_landed<C::LD>(ra, rb);
+            const bool end = i + 2 == C::NCH;
+            if (end) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[buf]);                     // the buffer's sums are in registers
             }
+            add(&acc[i / half][(i % half) * C::LD], ra, i / half, (i % half) * C::LD);
+            const bool more = !end || (kb + 1 < kb1 && (ok = arrived(it + 1)));
+            const uint32_t nb = end ? trow + (buf ^ 1u) * (2 * BN) : tb;
+            const int n = end ? 0 : i + 2;
+            if (more) f8_ld<C::LD>(nb + (n / half) * BN + (n % half) * C::LD, ra);
+            add(&acc[(i + 1) / half][((i + 1) % half) * C::LD], rb, (i + 1) / half, ((i + 1) % half) * C::LD);
+            if (more) f8_ld<C::LD>(nb + ((n + 1) / half) * BN + ((n + 1) % half) * C::LD, rb);
           }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        } else {
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          if (kb + 1 < kb1) ok = arrived(it + 1);
+        }
       }
       // ---- an item that other CTAs have parts of: leave the sums, the last one to arrive goes on with everybody's
       if (!(ok = named_bar_and(1, 256, ok))) break;
       if (kb1 - kb0 < KB) {
-        const long long s0 = (long long)item * KB;
-        const int c_first = sch.owner(s0), c_last = sch.owner(s0 + KB - 1);
-        auto part_of = [&](int c) { return a.part + ((size_t)c * 2 + (sch.start(c) / KB == item ? 0 : 1)) * (256 * BN) + (size_t)h * C::CW * 256 + row; };
-        float* mine = part_of(blockIdx.x);
+        const uint32_t s0 = (uint32_t)item * (uint32_t)KB, c_first = sch.owner(s0), c_last = sch.owner(s0 + KB - 1);
+        // a part: [column][tile][lane]; a CTA's first run is its part 0
+        auto part_of = [&](uint32_t c, uint32_t st) { return a.part + ((size_t)c * 2 + (c == c_first && st != s0 ? 1 : 0)) * (256 * BN) + (size_t)h * C::CW * 256 + row; };
+        float* mine = part_of(blockIdx.x, sch.start(blockIdx.x));
 #pragma unroll
         for (int c = 0; c < C::CW; ++c)
-          if (c < cols) { __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]); }
-        __threadfence();
+          if (active && c < cols) { __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]); }
         named_bar_sync(1, 256);
         if (threadIdx.x == 0) {
-          const bool all = atomicAdd(a.count + item, 1u) == (unsigned)(c_last - c_first);
+          __threadfence();                                                     // everybody's sums are out before this CTA is counted
+          const bool all = atomicAdd(a.count + item, 1u) == c_last - c_first;
           if (all) a.count[item] = 0u;                                         // zero again for the next launch
+          __threadfence();
           *last = all;
         }
         named_bar_sync(1, 256);
         const bool mine_to_end = *last != 0u;
         named_bar_sync(1, 256);                                                // the flag has been read: the next item may write it
         if (!mine_to_end) continue;
-        __threadfence();
 #pragma unroll
         for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
-        for (int cc = c_first; cc <= c_last; ++cc) {
-          const float* p = part_of(cc);
+        // parts and columns fetched together; a value's parts are added in order
+        constexpr int NP = C::CW <= 8 ? 8 : 2, GC = C::CW < 32 ? C::CW : 16;
+        const float* first = part_of(c_first, sch.start(c_first));
+        const float* rest = part_of(c_first, s0);                              // the later CTAs' parts are their first ones: 2 · 256 · BN apart
+        for (uint32_t cc = c_first; cc <= c_last; cc += NP) {
 #pragma unroll
-          for (int c = 0; c < C::CW; ++c)
-            if (c < cols) { acc[0][c] += __ldcg(p + c * 256); acc[1][c] += __ldcg(p + c * 256 + 128); }
+          for (int g = 0; g < C::CW; g += GC) {
+            if (!active || g >= cols) break;
+            float t[NP][2][GC];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+              const float* p = cc + i == c_first ? first : rest + (size_t)(cc + i - c_first) * (2 * 256 * BN);
+#pragma unroll
+              for (int c = 0; c < GC; ++c) {
+                const bool on = g + c < cols && cc + i <= c_last;
+                t[i][0][c] = on ? __ldcg(p + (g + c) * 256) : 0.f; t[i][1][c] = on ? __ldcg(p + (g + c) * 256 + 128) : 0.f;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+              for (int c = 0; c < GC; ++c) { acc[0][g + c] += t[i][0][c]; acc[1][g + c] += t[i][1][c]; }
+          }
         }
       }
       // ---- the item's results
-      if (MODE == F8_GU) {
-        uint32_t* am = amx + (h * 4) * C::CW;
+      if constexpr (MODE == F8_GU) {
+          uint32_t* am = amx + (h * 4) * C::CW;
 #pragma unroll
-        for (int c = 0; c < C::CW; ++c) {
-          float gv = acc[0][c], uv = acc[1][c];
-          if (a.limit > 0.f) { gv = fminf(gv, a.limit); uv = fminf(fmaxf(uv, -a.limit), a.limit); }
-          acc[0][c] = gv / (1.f + expf(-gv)) * uv;
-          const uint32_t mx = __reduce_max_sync(0xffffffffu, f8_mag(acc[0][c]));
-          if (lane == 0) am[q * C::CW + c] = mx;
-        }
-        named_bar_sync(2 + h, 128);
-#pragma unroll
-        for (int c = 0; c < C::CW; ++c) {
-          F8Block blk;
-          const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
-          const uint32_t code = blk.pair(acc[0][c], 0.f);
-          const int slot = tl.slot0 + h * C::CW + c;
-          if (c < cols) {
-            a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)code;
-            if (row == 0) a.ys[(size_t)nt * a.ldys + slot] = sc;
+          for (int c = 0; c < C::CW; ++c) {
+            acc[0][c] = f8_swiglu(acc[0][c], acc[1][c], a.limit);
+            const uint32_t mx = __reduce_max_sync(0xffffffffu, f8_mag(acc[0][c]));
+            if (lane == 0) am[q * C::CW + c] = mx;
           }
-        }
-        named_bar_sync(2 + h, 128);                                            // the magnitudes have been read
+          named_bar_sync(2 + h, 128);
+#pragma unroll
+          for (int c = 0; c < C::CW; ++c) {
+            F8Block blk;
+            const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
+            const uint32_t code = blk.pair(acc[0][c], 0.f);
+            const int slot = tl.slot0 + h * C::CW + c;
+            if (c < cols) {
+              a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)code;
+              if (row == 0) a.ys[(size_t)nt * a.ldys + slot] = sc;
+            }
+          }
+          named_bar_sync(2 + h, 128);                                          // the magnitudes have been read
       } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {

@@ -1,5 +1,5 @@
 // 8-bit floats with a scale per block of 128: the quantisers of activations and weights, the product, the routed experts.
-#include "fp8_gemm.cuh"
+#include "fp8_pair.cuh"
 #include "hb_kernels.h"
 
 namespace hb {
@@ -157,24 +157,29 @@ using namespace hb;
 namespace {
 using F8Kernel = void (*)(const F8Args, const CUtensorMap, const CUtensorMap);
 struct F8Pick { F8Kernel fn; int smem; };
+// rows: of a tile, at most (16, 32, 64: one CTA's tile; 256: a pair's)
 template <int MODE>
-F8Pick f8_kernel(int bn) {
-  switch (bn) {
+F8Pick f8_kernel(int rows) {
+  switch (rows) {
     case 16: return {fp8_gemm_kernel<16, MODE>, F8Cfg<16>::SMEM};
     case 32: return {fp8_gemm_kernel<32, MODE>, F8Cfg<32>::SMEM};
     case 64: return {fp8_gemm_kernel<64, MODE>, F8Cfg<64>::SMEM};
-    default: return {fp8_gemm_kernel<128, MODE>, F8Cfg<128>::SMEM};
+    default: return {fp8_pair_kernel<MODE>, F8P_SMEM};
   }
 }
-int f8_grid(const hb_ctx* ctx) {
-  const int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
-  return n < F8_MAX_CTAS ? n : F8_MAX_CTAS;
+template <int MODE>
+int f8_launch(hb_ctx* ctx, const char* name, int rows, const F8Args& a, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t st) {
+  const F8Pick k = f8_kernel<MODE>(rows);
+  int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
+  if (n > F8_MAX_CTAS) n = F8_MAX_CTAS;
+  if (rows == F8P_ROWS) n = n < 2 ? 2 : n & ~1;
+  return hb_launch_cluster(ctx, name, true, rows == F8P_ROWS ? 2 : 1, k.fn, dim3(n), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
 }
-size_t f8_part_bytes(int bn) { return (size_t)F8_MAX_CTAS * 2 * 256 * bn * 4; }
+size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows > 64 ? 128 : rows) * 4; }
 // rows of a tile for a product of M rows
-int f8_bn_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+int f8_rows_for(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : F8P_ROWS; }
 // pairs of a tile by what an expert gets on average: runs that are longer are cut into tiles, which read the expert's weights again
-int f8_bn_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 16ll * E ? 32 : P <= 40ll * E ? 64 : 128; }
+int f8_rows_for_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 16ll * E ? 32 : P <= 48ll * E ? 64 : F8P_ROWS; }
 // map of a byte matrix [n_rows][row_bytes], rows ld bytes apart, in boxes of 128 bytes × box_rows under the 128-byte swizzle; bytes and rows past the
 // end read as zero codes
 int f8_map(hb_ctx* ctx, CUtensorMap* m, const void* base, size_t row_bytes, size_t ld, size_t n_rows, int box_rows) {
@@ -195,7 +200,7 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   size_t off = 0;
   auto take = [&](size_t b) { void* r = ws ? static_cast<char*>(ws) + off : nullptr; off += hb_align256(b); return r; };
   const size_t P = (size_t)M * K;
-  const int bn = f8_bn_pairs((long long)P, E);
+  const int bn = f8_rows_for_pairs((long long)P, E);
   F8Ws t;
   t.hist = (int*)take(hbk_pf_plan_hist_bytes(E)); t.n_slots = (int*)take(4); t.n_tiles = (int*)take(4);
   t.tiles = (TileRef*)take((P / bn + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
@@ -210,14 +215,19 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
 unsigned int* f8_counters(hb_ctx* ctx) { return reinterpret_cast<unsigned int*>(ctx->dev_err) + kErrCounters; }
 int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
   const long long units = (long long)a.M * f8_blocks(a.K), ctas = (units + 15) / 16, cap = (long long)ctx->sm_count * 32;
-  return hb_launch(ctx, "fp8_quant_rows", !(ctx->flags & HB_FLAG_NO_PDL), fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap) + (a.dest ? 1 : 0)), dim3(256), 0, st, a);
+  return hb_launch(ctx, "fp8_quant_rows", true, fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap) + (a.dest ? 1 : 0)), dim3(256), 0, st, a);
 }
 }  // namespace
 
 int hbk_fp8_setup(hb_ctx* ctx) {
-  for (int bn : {16, 32, 64, 128})
-    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)})
+  for (int bn : {16, 32, 64, F8P_ROWS})
+    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {
+      cudaFuncAttributes at;
+      HB_CUDA(ctx, cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(k.fn)));
+      // a warp that asks for more registers than the block was launched with would wait for good
+      HB_REQUIRE(ctx, bn < 64 || at.numRegs >= F8_REGS, HB_ERR_CUDA, "fp8_gemm: built with %d registers a thread, its warps share out %d", at.numRegs, F8_REGS);
       HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    }
   return HB_OK;
 }
 
@@ -247,7 +257,7 @@ int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t*
   return hb_launch(ctx, "fp8_quantize", false, fp8_quantize_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float*>(w), N, K, q, s);
 }
 
-size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(f8_bn_rows(M)) : 0; }
+size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(f8_rows_for(M)) : 0; }
 
 int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb, float* yf, int ldy, void* ws, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
@@ -255,21 +265,22 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, W && W->w && W->s && xq && xs && (!yb != !yf), HB_ERR_INVALID, "fp8_gemm: NULL argument, or not exactly one output");
   HB_REQUIRE(ctx, W->fmt == HB_FMT_FP8_B128 && W->N > 0 && W->K > 0 && W->K % 16 == 0 && M > 0, HB_ERR_UNSUPPORTED, "fp8_gemm: FP8_B128 matrix with K %% 16 == 0 wanted (fmt %d N=%d K=%d M=%d)",
              W->fmt, W->N, W->K, M);
+  HB_REQUIRE(ctx, W->K <= 1 << 23, HB_ERR_UNSUPPORTED, "fp8_gemm: K=%d (<= 2^23)", W->K);
   HB_REQUIRE(ctx, ldq >= W->K && ldq % 16 == 0 && lds >= M && ldy >= W->N, HB_ERR_INVALID, "fp8_gemm: ldq=%d (>= K=%d, %% 16) lds=%d (>= M=%d) ldy=%d (>= N=%d)", ldq, W->K, lds, M, ldy, W->N);
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "fp8_gemm: ws NULL or not 256-byte aligned");
-  const int bn = f8_bn_rows(M), nt = (M + bn - 1) / bn;
+  const int rows = f8_rows_for(M), nt = (M + rows - 1) / rows;
   F8Args a{};
   a.M = M; a.per = ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
   HB_REQUIRE(ctx, (long long)nt * a.n_nt < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d", M, W->N);
   a.ws = reinterpret_cast<const float*>(W->s); a.xs = xs; a.lds = lds;
   a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.count = f8_counters(ctx); a.err = ctx->dev_err;
   CUtensorMap tw, tx;
+  const bool pair = rows == F8P_ROWS;
   int r;
-  if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, bn))) return r;
-  const F8Pick k = f8_kernel<F8_PLAIN>(bn);
-  return hb_launch(ctx, "fp8_gemm", !(ctx->flags & HB_FLAG_NO_PDL), k.fn, dim3(f8_grid(ctx)), dim3(F8_THREADS), (size_t)k.smem, reinterpret_cast<cudaStream_t>(stream), a, tw, tx);
+  if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, pair ? 64 : 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, pair ? 128 : rows))) return r;
+  return f8_launch<F8_PLAIN>(ctx, "fp8_gemm", rows, a, tw, tx, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int hb_fp8_rec_layout_make(int H, int I, hb_fp8_rec_layout* L) {
@@ -301,32 +312,30 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   const uint8_t* const* tab = rec_tab + (size_t)li * E;
   F8Ws W;
   f8_carve(ws, M, K, E, H, I, &W);
-  const int P = M * K, bn = f8_bn_pairs(P, E), grid = f8_grid(ctx);
-  const bool pdl = !(ctx->flags & HB_FLAG_NO_PDL);
+  const int P = M * K, rows = f8_rows_for_pairs(P, E), box = rows == F8P_ROWS ? 128 : rows;
   int r;
   F8RowsArgs q{};
   q.x = reinterpret_cast<const __nv_bfloat16*>(x); q.ldx = H; q.M = M; q.K = H; q.dest = W.pos_of; q.nd = K; q.q = W.xq; q.ldq = H; q.s = W.xs; q.lds = P;
   if ((r = hbk_wm_stamp_args(ctx, tab, E, nullptr, 2 * H, 2 * I, W.wmaps, &q.wm))) return r;
   CUtensorMap tx, ty;
-  if ((r = f8_map(ctx, &tx, W.xq, H, H, P, bn)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, bn))) return r;
-  if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, bn, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
+  if ((r = f8_map(ctx, &tx, W.xq, H, H, P, box)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, box))) return r;
+  if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, rows, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
   if ((r = f8_rows(ctx, q, st))) return r;
   F8Args a{};
   a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.count = f8_counters(ctx); a.err = ctx->dev_err;
   a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.wm = wm_args(W.wmaps, 2 * H);
   a.xs = W.xs; a.lds = P; a.yq = W.yq; a.ys = W.ys; a.ldys = P;
-  const F8Pick kg = f8_kernel<F8_GU>(bn), kd = f8_kernel<F8_DOWN>(bn);
-  if ((r = hb_launch(ctx, "fp8_gemm_gu", pdl, kg.fn, dim3(grid), dim3(F8_THREADS), (size_t)kg.smem, st, a, tx, tx))) return r;
+  if ((r = f8_launch<F8_GU>(ctx, "fp8_gemm_gu", rows, a, tx, tx, st))) return r;
   a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.wm = wm_args(W.wmaps + wm_bytes(2 * H), 2 * I);
   a.xs = W.ys; a.yb = W.part; a.ldy = H;
-  if ((r = hb_launch(ctx, "fp8_gemm_down", pdl, kd.fn, dim3(grid), dim3(F8_THREADS), (size_t)kd.smem, st, a, ty, ty))) return r;
+  if ((r = f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, ty, ty, st))) return r;
   F8SumArgs su{W.part, W.pos_of, w, M, K, H, out, nullptr, nullptr, 0, 0, nullptr};
   if (cmb) {
     su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
     if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
   }
   const long long ctas = ((long long)M * (H / 8) + F8_SUM_THREADS - 1) / F8_SUM_THREADS, cap = (long long)ctx->sm_count * 16;
-  return hb_launch(ctx, "fp8_sum", pdl, fp8_sum_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(F8_SUM_THREADS), 0, st, su);
+  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(F8_SUM_THREADS), 0, st, su);
 }
 
 }  // extern "C"
