@@ -9,7 +9,8 @@
 // back half 0, warps 4-7 half 1, and while one half's MMAs run the other half is read.  Gate/up: a half is 64 gate rows (loaded by CTA 0) and the 64 up
 // rows that belong to them (CTA 1), so a thread has both for its row of x.
 //
-// Warp 8 (one thread) loads, warp 9 (one thread, in CTA 0) issues the MMAs of both CTAs and announces finished buffers and free stages to both.  Work is cut
+// Warp 8 (one thread) loads, warps 9 and 10 (one thread each, in CTA 0) issue the MMAs of both CTAs, a half each, and announce finished buffers and free
+// stages to both.  Work is cut
 // and put together as in fp8_gemm.cuh, a pair of CTAs in the place of a CTA; each CTA looks after the parts of its own 128 rows.
 #pragma once
 #include "fp8_gemm.cuh"
@@ -76,9 +77,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a,
   const int warp = warp_uniform(), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < F8P_ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < F8P_ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
     for (int s = 0; s < 4; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, 2);
     mbar_fence_init();
   }
   if (warp == F8_W_MMA) tmem_alloc2(tmem_slot, 512);
@@ -138,29 +139,27 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a,
           if (++s == F8P_ST) { s = 0; ph ^= 1u; }
         }
       }
-    } else if (warp == F8_W_MMA && rank == 0) {
-      // ---------------------------------------------------------------------------------------------- MMA issue, one thread of CTA 0
+    } else if ((warp == F8_W_MMA || warp == F8_W_MMA + 1) && rank == 0) {
+      // ---------------------------------------------------------------------------------------------- MMA issue, one thread of CTA 0 for each half (one for both spent
+      // 700 clocks a step on its waits and instructions)
       if (elect_one()) {
+        const uint32_t h = warp - F8_W_MMA;
         uint32_t s = 0, ph = 0, it = 0;
         bool ok = true;
         // kind::f8f6f4: D fp32 (bit 4), A and B e4m3, both K-major, N / 8 = 16 at bit 17, M / 16 = 16 at bit 24
         constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((256u >> 4) << 24);
-        const uint64_t ad0 = tc_desc_sw128(base), bd0 = tc_desc_sw128(base + 128 * 128);
+        const uint64_t ad0 = tc_desc_sw128(base), bd0 = tc_desc_sw128(base + 128 * 128 + h * (64 * 128));
         while (ok && sch.next(item, kb0, kb1)) {
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const uint32_t buf = it & 1u, par = ((it >> 1) & 1u) ^ 1u;
+            const uint32_t buf = it & 1u;
             if (!(ok = mbar_wait(&full[s], ph, a.err, 0x400u))) break;
+            if (!(ok = mbar_wait(&acc_empty[h * 2 + buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x200u))) break;
+            tc_fence_after();
             const uint64_t ad = ad0 + s * (uint32_t)(F8P_STAGE >> 4), bd = bd0 + s * (uint32_t)(F8P_STAGE >> 4);
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              if (!(ok = mbar_wait(&acc_empty[h * 2 + buf], par, a.err, 0x200u))) break;
-              tc_fence_after();
-#pragma unroll
-              for (uint32_t j = 0; j < 4; ++j)                                 // 32 values further along the swizzled rows
-                tc_mma2_f8(tmem + buf * 256 + h * 128, ad + 2 * j, bd + h * (64 * 128 >> 4) + 2 * j, idesc, j);
-              tc_commit2(&acc_full[h * 2 + buf]);
-            }
-            if (!ok) break;
+            for (uint32_t j = 0; j < 4; ++j)                                   // 32 values further along the swizzled rows
+              tc_mma2_f8(tmem + buf * 256 + h * 128, ad + 2 * j, bd + 2 * j, idesc, j);
+            tc_commit2(&acc_full[h * 2 + buf]);
             tc_commit2(&empty[s]);
             if (++s == F8P_ST) { s = 0; ph ^= 1u; }
           }
