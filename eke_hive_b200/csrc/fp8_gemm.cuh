@@ -89,6 +89,9 @@ struct F8Sched {                                       // (32 bits: at most 320 
   __device__ __forceinline__ uint32_t owner(uint32_t step) const { return ((step + 1u) * Gs - 1u) / U; }
 };
 
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(tmap), "r"(c0), "r"(c1) : "memory");
+}
 __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -201,11 +204,24 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int KB = f8_blocks(a.K);
+  F8Sched sch;
+  if (MODE == F8_PLAIN) {
+    // While the kernel in front ends: the first stages' weights on their way to L2.  (Nothing is read; what is written there until then, L2 has.)
+    sch.init((uint32_t)((a.M + a.per - 1) / a.per) * a.n_nt, KB, gridDim.x, blockIdx.x, false);
+    if (warp == F8_W_TMA && elect_one()) {
+      F8Sched ahead = sch;
+      int it0, k0, k1;
+      if (ahead.next(it0, k0, k1)) {
+        const int r0 = it0 % a.n_nt * 256;
+        for (int kb = k0; kb < min(k1, k0 + C::ST); ++kb) { tma_prefetch_2d(&tmW, kb * 128, r0); if (r0 + 128 < a.N) tma_prefetch_2d(&tmW, kb * 128, r0 + 128); }
+      }
+    }
+    __syncwarp();
+  }
   griddep_wait();
   griddep_launch();
-  const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
-  F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
+  if (MODE != F8_PLAIN) sch.init((uint32_t)*a.n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
   auto tile_of = [&](int ti) -> TileRef {
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};

@@ -4,55 +4,155 @@
 
 namespace hb {
 
-// Rows: 16 lanes take a block of 128 values, 8 each.  dest == nullptr: row m of q / s; else row m goes to slots dest[m·nd + j], j < nd, negative ones
-// skipped (the rows of a routed layer are quantised once and written into expert order).
+// Rows: 16 lanes take a block of 128 values, 8 each.  Without destinations row m becomes row m of q / s.  With them (a routed layer's rows are quantised once
+// and written into expert order) row m goes to the slots of its nd pairs, those that have one.
 struct F8RowsArgs {
   const __nv_bfloat16* x; int ldx, M, K;
-  const int* dest; int nd;
+  const int* dest; int nd;                             // [M, nd], negative: none; nd == 0: no destinations
   uint8_t* q; int ldq; float* s; int lds;
-  WmStamp wm;                                          // with dest: the first CTA stamps the weight maps of the call's GEMMs instead
 };
-__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const __grid_constant__ F8RowsArgs a) {
-  griddep_wait();
-  if (a.dest && blockIdx.x == 0) { wm_stamp(a.wm); return; }
-  const int cta = blockIdx.x - (a.dest ? 1 : 0), ctas = gridDim.x - (a.dest ? 1 : 0);
+// Block b of row m; slot: of lane l16 < nd's pair, or -1.
+__device__ __forceinline__ void f8_quant_unit(const F8RowsArgs& a, int m, int b, int slot) {
+  const int l16 = threadIdx.x & 15, k = b * F8_B + l16 * 8, sh = threadIdx.x & 16;
+  const uint32_t half = 0xffffu << sh;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (k < a.K) {                                                               // K is a multiple of 16: eight values are inside or outside together
+    const __nv_bfloat16* p = a.x + (size_t)m * a.ldx + k;
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(ww[j] << 16); v[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __bfloat162float(p[j]);
+    }
+  }
+  uint32_t mx = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) mx = max(mx, f8_mag(v[j]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(half, mx, o));
+  F8Block blk;
+  const float sc = blk.init(mx);
+  const uint2 c = make_uint2(blk.pair(v[0], v[1]) | blk.pair(v[2], v[3]) << 16, blk.pair(v[4], v[5]) | blk.pair(v[6], v[7]) << 16);
+  if (a.nd == 0) {
+    if (k < a.K) *reinterpret_cast<uint2*>(a.q + (size_t)m * a.ldq + k) = c;
+    if (l16 == 0) a.s[(size_t)b * a.lds + m] = sc;
+    return;
+  }
+  if (slot >= 0) a.s[(size_t)b * a.lds + slot] = sc;
+  for (uint32_t on = __ballot_sync(half, slot >= 0) >> sh & 0xffffu; on; on &= on - 1u) {
+    const int to = __shfl_sync(half, slot, (__ffs(on) - 1) + sh);
+    if (k < a.K) *reinterpret_cast<uint2*>(a.q + (size_t)to * a.ldq + k) = c;
+  }
+}
+// CTA `cta` of `ctas`: every ctas-th run of 16 blocks
+__device__ __forceinline__ void f8_quant_rows(const F8RowsArgs& a, int cta, int ctas) {
   const int nb = f8_blocks(a.K), l16 = threadIdx.x & 15;
   const uint32_t half = 0xffffu << (threadIdx.x & 16);
   const long long total = (long long)a.M * nb;
   for (long long i = (long long)cta * 16 + (threadIdx.x >> 4); i < total; i += (long long)ctas * 16) {
-    const int m = (int)(i / nb), b = (int)(i - (long long)m * nb), k = b * F8_B + l16 * 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (k < a.K) {                                                             // K is a multiple of 16: eight values are inside or outside together
-      const __nv_bfloat16* p = a.x + (size_t)m * a.ldx + k;
-      if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(ww[j] << 16); v[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __bfloat162float(p[j]);
-      }
-    }
-    uint32_t mx = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) mx = max(mx, f8_mag(v[j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(half, mx, o));
-    F8Block blk;
-    const float sc = blk.init(mx);
-    const uint2 c = make_uint2(blk.pair(v[0], v[1]) | blk.pair(v[2], v[3]) << 16, blk.pair(v[4], v[5]) | blk.pair(v[6], v[7]) << 16);
-    for (int j = 0; j < (a.dest ? a.nd : 1); ++j) {
-      const int slot = a.dest ? a.dest[(size_t)m * a.nd + j] : m;
-      if (slot < 0) continue;
-      if (k < a.K) *reinterpret_cast<uint2*>(a.q + (size_t)slot * a.ldq + k) = c;
-      if (l16 == 0) a.s[(size_t)b * a.lds + slot] = sc;
+    const int m = (int)(i / nb), b = (int)(i - (long long)m * nb);
+    if (a.nd == 0) { f8_quant_unit(a, m, b, -1); continue; }
+    for (int d = 0; d < a.nd; d += 16) {                                       // (more than 16 destinations: once more)
+      const int slot = d + l16 < a.nd ? __ldg(a.dest + (size_t)m * a.nd + d + l16) : -1;
+      if (__any_sync(half, slot >= 0)) f8_quant_unit(a, m, b, slot);           // a row nobody here wants is not read
     }
   }
 }
+__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const F8RowsArgs a) {
+  griddep_wait();
+  griddep_launch();
+  f8_quant_rows(a, blockIdx.x, gridDim.x);
+}
 
+// The front of a routed layer's call in one launch.  The first CTAs stamp the weight maps of the GEMMs.  Calls of at most F8_PREP_PAIRS pairs are planned here too: a
+// pair's slot is the number of pairs with a smaller expert plus the number of earlier ones with its own, which every CTA counts for the pairs it needs over
+// the whole list in shared memory — no histogram, no meeting of CTAs, no launch in between (the plan kernel for long lists and the quantiser
+// behind it took 19 of a one-row call's 75 us).  One CTA writes the plan down, the others quantise.
+constexpr int F8_PREP_PAIRS = 1024, F8_PREP_STAMP = 4;
+struct F8PrepArgs {
+  F8RowsArgs rows; WmStamp wm;
+  const int32_t* ids; int P, E, bm; const uint8_t* const* tab;                 // P == 0: rows.dest has been worked out before
+  int* pos_of; TileRef* tiles; int* n_tiles;
+};
+__global__ void __launch_bounds__(256) fp8_prep_kernel(const __grid_constant__ F8PrepArgs a) {
+  __shared__ int4 e4[F8_PREP_PAIRS / 4];
+  __shared__ int slots[512];
+  __shared__ uint32_t flag[F8_PREP_PAIRS / 32];
+  int* e_s = reinterpret_cast<int*>(e4);
+  griddep_wait();
+  griddep_launch();
+  if (blockIdx.x < F8_PREP_STAMP) { wm_stamp(a.wm, blockIdx.x, F8_PREP_STAMP); return; }
+  if (a.P == 0) { f8_quant_rows(a.rows, blockIdx.x - F8_PREP_STAMP, gridDim.x - F8_PREP_STAMP); return; }
+  constexpr int NONE = 0x7fffffff;
+  const int t = threadIdx.x, P = a.P, P4 = (P + 3) / 4;
+  for (int p = t; p < P4 * 4; p += 256) {
+    const int e = p < P ? __ldg(a.ids + p) : -1;
+    e_s[p] = e >= 0 && e < a.E && __ldg(reinterpret_cast<const unsigned long long*>(a.tab) + e) != 0ull ? e : NONE;
+  }
+  if (t < F8_PREP_PAIRS / 32) flag[t] = 0u;
+  __syncthreads();
+  struct At { int slot, rank, run; };
+  auto place = [&](int p) -> At {
+    const int e = e_s[p];
+    int less = 0, before = 0, run = 0;
+#pragma unroll 4
+    for (int i = 0; i < P4; ++i) {
+      const int4 v = e4[i];
+      less += (v.x < e) + (v.y < e) + (v.z < e) + (v.w < e);
+      const int c = (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+      run += c;
+      if (4 * i + 4 <= p) before += c;
+      else before += (v.x == e && 4 * i < p) + (v.y == e && 4 * i + 1 < p) + (v.z == e && 4 * i + 2 < p);
+    }
+    return e == NONE ? At{-1, 0, 0} : At{less + before, before, run};
+  };
+  if (blockIdx.x == F8_PREP_STAMP) {
+    // a tile starts at every tper-th pair of a run; its number is that of the starts in front of it
+    At at[F8_PREP_PAIRS / 256]; int tper[F8_PREP_PAIRS / 256];
+#pragma unroll
+    for (int i = 0; i < F8_PREP_PAIRS / 256; ++i) {
+      const int p = t + 256 * i;
+      if (p >= P) break;
+      at[i] = place(p);
+      a.pos_of[p] = at[i].slot;
+      if (at[i].slot < 0) continue;
+      const int nt = (at[i].run + a.bm - 1) / a.bm;
+      tper[i] = (at[i].run + nt - 1) / nt;
+      if (at[i].rank % tper[i] == 0) atomicOr(&flag[at[i].slot >> 5], 1u << (at[i].slot & 31));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < F8_PREP_PAIRS / 256; ++i) {
+      const int p = t + 256 * i;
+      if (p >= P) break;
+      if (at[i].slot < 0 || at[i].rank % tper[i] != 0) continue;
+      int n = __popc(flag[at[i].slot >> 5] & ((1u << (at[i].slot & 31)) - 1u));
+      for (int w = 0; w < at[i].slot >> 5; ++w) n += __popc(flag[w]);
+      TileRef tl; tl.slot0 = at[i].slot; tl.rows = min(tper[i], at[i].run - at[i].rank); tl.expert = e_s[p];
+      a.tiles[n] = tl;
+    }
+    if (t == 0) { int n = 0; for (int w = 0; w < F8_PREP_PAIRS / 32; ++w) n += __popc(flag[w]); *a.n_tiles = n; }
+    return;
+  }
+  // 16 blocks of 128 values a CTA: their rows' slots first
+  const int nb = f8_blocks(a.rows.K), u0 = (blockIdx.x - F8_PREP_STAMP - 1) * 16, total = a.rows.M * nb, nd = a.rows.nd;
+  const int m0 = u0 / nb, m1 = min(u0 + 15, total - 1) / nb;
+  for (int i = t; i < (m1 - m0 + 1) * nd; i += 256) slots[i] = place(m0 * nd + i).slot;
+  __syncthreads();
+  const int u = u0 + (t >> 4), l16 = t & 15;
+  if (u < total) {
+    const int m = u / nb;
+    for (int d = 0; d < nd; d += 16) {
+      const int slot = d + l16 < nd ? slots[(m - m0) * nd + d + l16] : -1;
+      if (__any_sync(0xffffu << (t & 16), slot >= 0)) f8_quant_unit(a.rows, m, u - m * nb, slot);
+    }
+  }
+}
 // Weights: a CTA takes a block of 128 × 128, sixteen lanes a row of it, eight rows a thread.
 template <class T>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ w, int N, int K, uint8_t* __restrict__ q, float* __restrict__ s) {
@@ -100,7 +200,8 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
 }
 
 // ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)], k in order (+ gate·shared[m]) ----------------------------------
-// A thread owns eight columns of a row, 16 bytes of every pair's part; the row's slots and weights are fetched together in front of the parts.
+// A warp takes 256 columns of a row, a lane eight of them (16 bytes of every pair's part).  Lane k looks up pair k; only pairs that have a slot are gone
+// through, four parts fetched at a time.
 constexpr int F8_SUM_THREADS = 128;
 struct F8SumArgs {
   const __nv_bfloat16* part; const int* pos_of; const float* w; int M, K, H; float* out;
@@ -108,45 +209,48 @@ struct F8SumArgs {
 };
 __global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs a) {
   griddep_wait();
-  const int chunks = a.H / 8;
+  const int chunks = (a.H + 255) / 256, lane = threadIdx.x & 31;
   const long long total = (long long)a.M * chunks;
-  for (long long i = (long long)blockIdx.x * F8_SUM_THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * F8_SUM_THREADS) {
-    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 8;
+  constexpr int WARPS = F8_SUM_THREADS / 32;
+  for (long long i = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); i < total; i += (long long)gridDim.x * WARPS) {
+    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 256 + lane * 8;
+    const bool in = n < a.H;                                                   // H is a multiple of 128
+    const size_t o = (size_t)m * a.H + n;
+    const int slot = lane < a.K ? __ldg(a.pos_of + (size_t)m * a.K + lane) : -1;
+    const float wk = slot >= 0 ? __ldg(a.w + (size_t)m * a.K + lane) : 0.f;
+    const uint4 sv = a.shared && in ? __ldg(reinterpret_cast<const uint4*>(a.shared + o)) : make_uint4(0u, 0u, 0u, 0u);
     const float gate = a.lg ? 1.f / (1.f + expf(-__ldg(a.lg + (size_t)m * a.ld + a.col))) : 1.f;
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int k0 = 0; k0 < a.K; k0 += 8) {
-      uint4 v[8]; float w[8];
+    auto add = [&](const uint4& v, float f) {
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int slot = k0 + k < a.K ? __ldcg(a.pos_of + (size_t)m * a.K + k0 + k) : -1;
-        w[k] = slot >= 0 ? __ldg(a.w + (size_t)m * a.K + k0 + k) : 0.f;
-        v[k] = slot >= 0 ? __ldcs(reinterpret_cast<const uint4*>(a.part + (size_t)slot * a.H + n)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(f, __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(f, __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
+    };
+    for (uint32_t on = __ballot_sync(0xffffffffu, slot >= 0); on;) {
+      uint4 v[4]; float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = on ? __ffs(on) - 1 : 0;
+        const int sl = __shfl_sync(0xffffffffu, slot, k);
+        f[j] = __shfl_sync(0xffffffffu, wk, k);
+        v[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (!on) f[j] = 0.f;
+        else if (in) v[j] = __ldcs(reinterpret_cast<const uint4*>(a.part + (size_t)sl * a.H + n));
+        on &= on - 1u;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(w[k], __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(w[k], __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
-      }
+      for (int j = 0; j < 4; ++j) add(v[j], f[j]);
     }
-    const size_t o = (size_t)m * a.H + n;
+    if (!in) continue;
     if (!a.cout) {
       *reinterpret_cast<float4*>(a.out + o) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       *reinterpret_cast<float4*>(a.out + o + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
       continue;
     }
-    if (a.shared) {
-      const uint4 sv = __ldg(reinterpret_cast<const uint4*>(a.shared + o));
-      const uint32_t u[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(gate, __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(gate, __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
-    }
-    uint32_t p[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]); p[j] = *reinterpret_cast<const uint32_t*>(&b); }
-    *reinterpret_cast<uint4*>(a.cout + o) = make_uint4(p[0], p[1], p[2], p[3]);
+    if (a.shared) add(sv, gate);
+    *reinterpret_cast<uint4*>(a.cout + o) = f8_pack8(acc);
   }
 }
 
@@ -215,7 +319,7 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
 unsigned int* f8_counters(hb_ctx* ctx) { return reinterpret_cast<unsigned int*>(ctx->dev_err) + kErrCounters; }
 int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
   const long long units = (long long)a.M * f8_blocks(a.K), ctas = (units + 15) / 16, cap = (long long)ctx->sm_count * 32;
-  return hb_launch(ctx, "fp8_quant_rows", true, fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap) + (a.dest ? 1 : 0)), dim3(256), 0, st, a);
+  return hb_launch(ctx, "fp8_quant_rows", true, fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(256), 0, st, a);
 }
 }  // namespace
 
@@ -241,7 +345,7 @@ int hb_fp8_quant_rows(hb_ctx* ctx, const void* x, int ldx, int M, int K, uint8_t
   HB_REQUIRE(ctx, ldx >= K && ldq >= K && ldq % 16 == 0 && lds >= M, HB_ERR_INVALID, "fp8_quant_rows: ldx=%d ldq=%d (>= K=%d, ldq %% 16) lds=%d (>= M=%d)", ldx, ldq, K, lds, M);
   HB_REQUIRE(ctx, hb_aligned(x, 2) && hb_aligned(q, 16) && hb_aligned(s, 4), HB_ERR_INVALID, "fp8_quant_rows: q must be 16-byte aligned, x and s to their elements");
   F8RowsArgs a{};
-  a.x = reinterpret_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.M = M; a.K = K; a.nd = 1; a.q = q; a.ldq = ldq; a.s = s; a.lds = lds;
+  a.x = reinterpret_cast<const __nv_bfloat16*>(x); a.ldx = ldx; a.M = M; a.K = K; a.q = q; a.ldq = ldq; a.s = s; a.lds = lds;
   return f8_rows(ctx, a, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -314,13 +418,22 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   f8_carve(ws, M, K, E, H, I, &W);
   const int P = M * K, rows = f8_rows_for_pairs(P, E), box = rows == F8P_ROWS ? 128 : rows;
   int r;
-  F8RowsArgs q{};
+  F8PrepArgs pr{};
+  F8RowsArgs& q = pr.rows;
   q.x = reinterpret_cast<const __nv_bfloat16*>(x); q.ldx = H; q.M = M; q.K = H; q.dest = W.pos_of; q.nd = K; q.q = W.xq; q.ldq = H; q.s = W.xs; q.lds = P;
-  if ((r = hbk_wm_stamp_args(ctx, tab, E, nullptr, 2 * H, 2 * I, W.wmaps, &q.wm))) return r;
+  if ((r = hbk_wm_stamp_args(ctx, tab, E, nullptr, 2 * H, 2 * I, W.wmaps, &pr.wm))) return r;
   CUtensorMap tx, ty;
   if ((r = f8_map(ctx, &tx, W.xq, H, H, P, box)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, box))) return r;
-  if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, rows, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
-  if ((r = f8_rows(ctx, q, st))) return r;
+  const long long units = (long long)M * f8_blocks(H), cap = (long long)ctx->sm_count * 32;
+  long long ctas = (units + 15) / 16;
+  if (P <= F8_PREP_PAIRS) {
+    pr.ids = ids; pr.P = P; pr.E = E; pr.bm = rows; pr.tab = tab; pr.pos_of = W.pos_of; pr.tiles = W.tiles; pr.n_tiles = W.n_tiles;
+    ++ctas;
+  } else {
+    if (ctas > cap) ctas = cap;
+    if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, rows, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
+  }
+  if ((r = hb_launch(ctx, "fp8_prep", true, fp8_prep_kernel, dim3(F8_PREP_STAMP + (unsigned)ctas), dim3(256), 0, st, pr))) return r;
   F8Args a{};
   a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.count = f8_counters(ctx); a.err = ctx->dev_err;
   a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.wm = wm_args(W.wmaps, 2 * H);
@@ -334,8 +447,8 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
     su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
     if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
   }
-  const long long ctas = ((long long)M * (H / 8) + F8_SUM_THREADS - 1) / F8_SUM_THREADS, cap = (long long)ctx->sm_count * 16;
-  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(F8_SUM_THREADS), 0, st, su);
+  const long long sums = ((long long)M * ((H + 255) / 256) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32);
+  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(sums < cap / 2 ? sums : cap / 2)), dim3(F8_SUM_THREADS), 0, st, su);
 }
 
 }  // extern "C"
