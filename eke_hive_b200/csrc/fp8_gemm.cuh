@@ -19,7 +19,7 @@
 // of the columns, 4-7 the second) and end the items.  Two accumulator buffers: one fills while the other is read.  Every wait is bounded.
 #pragma once
 #include "fp8_common.cuh"
-#include "wmap.cuh"
+#include "tc_common.cuh"
 
 namespace hb {
 
@@ -28,6 +28,68 @@ enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
 constexpr int F8_MAX_CTAS = 160;                       // grid at most; the workspace holds two partial items of each
 constexpr int F8_COUNTERS = 2 * F8_MAX_CTAS;           // items that are cut, at most
 constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
+// Plan of a short list of pairs (at most F8_PLAN_PAIRS), worked out by every CTA that needs it for itself: a pair's slot is the number of pairs with a smaller
+// expert plus the number of earlier ones with its own, counted over the whole list in shared memory — no histogram, no meeting of CTAs, no launch of its own.
+constexpr int F8_PLAN_PAIRS = 1024;
+struct F8Plan { const int32_t* ids; int P, E, bm; const uint8_t* const* tab; };   // bm: pairs of a tile, at most
+struct F8At { int slot, rank, run, expert; };          // slot -1: the pair contributes nothing
+// ids with a record, the others NONE, to shared memory (room for P rounded up to four); the caller synchronises behind it
+__device__ __forceinline__ void f8_plan_load(const F8Plan& a, int* e_s, int threads) {
+  for (int p = threadIdx.x; p < (a.P + 3) / 4 * 4; p += threads) {
+    const int e = p < a.P ? __ldg(a.ids + p) : -1;
+    e_s[p] = e >= 0 && e < a.E && __ldg(reinterpret_cast<const unsigned long long*>(a.tab) + e) != 0ull ? e : 0x7fffffff;
+  }
+}
+__device__ __forceinline__ F8At f8_plan_at(const F8Plan& a, const int* e_s, int p) {
+  const int e = e_s[p];
+  int less = 0, before = 0, run = 0;
+#pragma unroll 4
+  for (int i = 0; i < (a.P + 3) / 4; ++i) {
+    const int4 v = reinterpret_cast<const int4*>(e_s)[i];
+    less += (v.x < e) + (v.y < e) + (v.z < e) + (v.w < e);
+    const int c = (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+    run += c;
+    before += 4 * i + 4 <= p ? c : (v.x == e && 4 * i < p) + (v.y == e && 4 * i + 1 < p) + (v.z == e && 4 * i + 2 < p);
+  }
+  return e == 0x7fffffff ? F8At{-1, 0, 0, 0} : F8At{less + before, before, run, e};
+}
+// The tile list; tmp: 16-byte aligned room for 5 KB that may be written over.  A run of pairs is cut into tiles of equal size; a tile starts at every tper-th
+// pair of a run, and its number is that of the starts at smaller slots.  Returns the number of tiles; the caller synchronises before the list is read.
+// slots: where pair p's slot goes (or nullptr).
+__device__ __forceinline__ int f8_plan_tiles(const F8Plan& a, uint8_t* tmp, TileRef* tiles, int threads, int* slots = nullptr) {
+  int* e_s = reinterpret_cast<int*>(tmp);
+  uint32_t* flag = reinterpret_cast<uint32_t*>(e_s + F8_PLAN_PAIRS);
+  f8_plan_load(a, e_s, threads);
+  for (int i = threadIdx.x; i < F8_PLAN_PAIRS / 32; i += threads) flag[i] = 0u;
+  __syncthreads();
+  auto first = [&](const F8At& at, int& rows) {
+    const int nt = (at.run + a.bm - 1) / a.bm, tper = (at.run + nt - 1) / nt;
+    rows = min(tper, at.run - at.rank);
+    return at.rank % tper == 0;
+  };
+  F8At mine{-1, 0, 0, 0};                              // of the thread's first pair: lists this short are the rule
+  for (int p = threadIdx.x; p < a.P; p += threads) {
+    const F8At at = f8_plan_at(a, e_s, p);
+    if (p == (int)threadIdx.x) mine = at;
+    if (slots) slots[p] = at.slot;
+    int rows;
+    if (at.slot >= 0 && first(at, rows)) atomicOr(&flag[at.slot >> 5], 1u << (at.slot & 31));
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.P; p += threads) {
+    const F8At at = p == (int)threadIdx.x ? mine : f8_plan_at(a, e_s, p);
+    int rows;
+    if (at.slot < 0 || !first(at, rows)) continue;
+    int n = __popc(flag[at.slot >> 5] & ((1u << (at.slot & 31)) - 1u));
+    for (int w = 0; w < at.slot >> 5; ++w) n += __popc(flag[w]);
+    tiles[n] = TileRef{at.slot, rows, at.expert};
+  }
+  int n = 0;
+  for (int w = 0; w < (a.P + 31) / 32; ++w) n += __popc(flag[w]);
+  __syncthreads();                                     // tmp has been read
+  return n;
+}
+
 constexpr int F8_STG_PITCH = 80, F8_STG_BYTES = 32 * F8_STG_PITCH;   // a warp's staging: 32 rows of 64 bytes (pitch: 16-byte accesses without bank conflicts)
 constexpr int F8_REGS = 168, F8_REGS_SUM = 216, F8_REGS_REST = 72;   // a thread's at launch (hbk_fp8_setup checks it), then of the sums' and of the other warps
 static_assert(8 * F8_REGS_SUM + 4 * F8_REGS_REST <= 12 * F8_REGS, "register split");
@@ -42,22 +104,41 @@ struct F8Cfg {
   static constexpr int LD = CW < 32 ? CW : 32;         // columns read at a time
   static constexpr int NCH = 2 * CW / LD;              // reads a step takes: even
   static constexpr bool SPLIT = BN >= 64;              // the sums need more registers than a twelfth of the file: the other warps give some of theirs
-  static constexpr int SMEM = 1024 + ST * STAGE + 4 * 2 * BN * 4 + 8 * CW * 4 + 512;
+  static constexpr int SMEM = 1024 + ST * STAGE + 4 * 2 * BN * 4 + 8 * CW * 4 + 512 + F8_PLAN_PAIRS * (int)sizeof(TileRef);   // (the tile list: GU)
   static_assert(F8_COUNTERS <= kErrCounterWords, "counters of the context");
-  static_assert(SMEM <= 227 * 1024 && TMEM <= 512 && STAGE % 1024 == 0, "shared memory, tensor memory, swizzle atoms");
+  static_assert(ST < 8 && SMEM <= 227 * 1024 && TMEM <= 512 && STAGE % 1024 == 0, "shared memory, tensor memory, swizzle atoms");
 };
 
 struct F8Args {
   const TileRef* tiles; const int* n_tiles;            // GU / DOWN: tiles of slots; PLAIN: ceil(M / per) tiles of `per` rows
+  F8Plan plan;                                         // GU with plan.P > 0: the tiles are worked out here
   int M, per, N, K, n_nt;                              // n_nt: items a tile has (GU: N / 128 with N = I, else ceil(N / 256))
   const float* ws; const uint8_t* const* tab; uint64_t off_w, off_s0, off_s1; int row2;   // PLAIN: scales; else records, offsets of the codes and of the two tiles' scales, rows from the first tile's matrix to the second's (GU)
-  WmArgs wm;
+  uint8_t* maps;                                       // GU / DOWN: room for F8_MAPS tensor maps a CTA
   const float* xs; int lds;                            // scales of the rows
   float limit;
   __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN
   uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
   float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256], arrivals (zero before and after)
   uint32_t* err;
+};
+
+// Tensor maps of expert records, made by the thread that loads through them: a record's address is known on the device only, and the map of a matrix
+// is one map for all experts but for its address.  A CTA's slots go round; one is written again when F8_MAPS items, of at least one stage each, have gone by, more
+// than there are stages: what was loaded through it has been multiplied.
+constexpr int F8_MAPS = 8;
+struct F8Maps {
+  uint8_t* slots; uint32_t n;
+  __device__ __forceinline__ const void* make(const CUtensorMap& tpl, const void* addr) {
+    uint8_t* to = slots + (size_t)(n++ % F8_MAPS) * sizeof(CUtensorMap);
+    const uint4* from = reinterpret_cast<const uint4*>(&tpl);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(to)[j] = from[j];
+    asm volatile("tensormap.replace.tile.global_address.global.b1024.b64 [%0], %1;" ::"l"(to), "l"(addr) : "memory");
+    asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
+    tmap_acquire(to);
+    return to;
+  }
 };
 
 // The steps of a CTA, the same for all its warps: segments (item, first step, end).
@@ -177,7 +258,7 @@ __device__ __forceinline__ void f8_ld(uint32_t taddr, uint32_t (&r)[W]) {
 }
 
 template <int BN, int MODE>
-__global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+__global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
   using C = F8Cfg<BN>;
   extern __shared__ uint8_t f8_raw[];
   const uint32_t raw = smem_u32(f8_raw), base = (raw + 1023u) & ~1023u;
@@ -192,6 +273,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   uint64_t* mma_done = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile uint32_t* last = tmem_slot + 1;
+  TileRef* tile_s = reinterpret_cast<TileRef*>(tmem_slot + 4);
   const int warp = warp_uniform(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -200,29 +282,25 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
     mbar_fence_init();
   }
   if (warp == F8_W_MMA) { tmem_alloc(tmem_slot, C::TMEM); tmem_relinquish(); }
+  // What comes before griddep_wait runs beside the end of the kernel in front.  Routed: that one is this library's, and all that was there before it (routing,
+  // table, records, for long lists and for the down pass the tiles) is complete, as it announced itself after its own wait; the tiles are found and the first
+  // stages' weights loaded here.  Dense: the kernel in front is anybody's, and only sends weights on their way to L2.
+  const bool own_plan = MODE == F8_GU && a.plan.P > 0;
+  int n_tiles = 0;
+  if (own_plan) {
+    n_tiles = f8_plan_tiles(a.plan, sm, tile_s, F8_THREADS);
+    fence_proxy_async_smem();                                                  // its scratch becomes operand stages
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int KB = f8_blocks(a.K);
+  if (!own_plan) n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  if (MODE == F8_PLAIN) {
-    // While the kernel in front ends: the first stages' weights on their way to L2.  (Nothing is read; what is written there until then, L2 has.)
-    sch.init((uint32_t)((a.M + a.per - 1) / a.per) * a.n_nt, KB, gridDim.x, blockIdx.x, false);
-    if (warp == F8_W_TMA && elect_one()) {
-      F8Sched ahead = sch;
-      int it0, k0, k1;
-      if (ahead.next(it0, k0, k1)) {
-        const int r0 = it0 % a.n_nt * 256;
-        for (int kb = k0; kb < min(k1, k0 + C::ST); ++kb) { tma_prefetch_2d(&tmW, kb * 128, r0); if (r0 + 128 < a.N) tma_prefetch_2d(&tmW, kb * 128, r0 + 128); }
-      }
-    }
-    __syncwarp();
-  }
-  griddep_wait();
-  griddep_launch();
-  if (MODE != F8_PLAIN) sch.init((uint32_t)*a.n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
   auto tile_of = [&](int ti) -> TileRef {
+    if (own_plan) return tile_s[ti];
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
   };
@@ -234,32 +312,38 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
     // ------------------------------------------------------------------------------------------------ operand tiles, one thread
     if (elect_one()) {
       uint32_t s = 0, ph = 1;
-      bool ok = true;
-      WmReader wm;
-      if (MODE != F8_PLAIN) wm.init(a.wm);
+      bool ok = true, waited = false;
+      F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
       while (ok && sch.next(item, kb0, kb1)) {
         const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
         const TileRef tl = tile_of(ti);
-        WmBox box;
-        if (MODE != F8_PLAIN && !wm.locate(a.tab[tl.expert] + a.off_w, box, a.err)) break;
-        const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, r1 = MODE == F8_GU ? r0 + a.row2 : r0 + 128;
-        const bool two = MODE == F8_GU || r1 < a.N;                            // a last item may have one tile: beyond it there is other memory
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
-          const uint32_t sb = base + s * C::STAGE;
-          mbar_expect_tx(&full[s], (two ? 2 : 1) * F8_A_BYTES + C::B_BYTES);
-          if (MODE == F8_PLAIN) {
-            tma_load_2d(sb, &tmW, kb * 128, r0, &full[s]);
-            if (two) tma_load_2d(sb + F8_A_BYTES, &tmW, kb * 128, r1, &full[s]);
-          } else {
-            wm.load(sb, box, kb * 128, r0, &full[s]);
-            wm.load(sb + F8_A_BYTES / 2, box, kb * 128, r0 + 64, &full[s]);
-            if (two) {
-              wm.load(sb + F8_A_BYTES, box, kb * 128, r1, &full[s]);
-              wm.load(sb + F8_A_BYTES + F8_A_BYTES / 2, box, kb * 128, r1 + 64, &full[s]);
-            }
+        const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab[tl.expert] + a.off_w);
+        const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, r1 = MODE == F8_GU ? r0 + a.row2 : r0 + 128;   // rows past the last read as zero codes
+        auto weights = [&](uint32_t st, int kb) {
+          mbar_expect_tx(&full[st], C::STAGE);
+          tma_load_2d(base + st * C::STAGE, mw, kb * 128, r0, &full[st]);
+          tma_load_2d(base + st * C::STAGE + F8_A_BYTES, mw, kb * 128, r1, &full[st]);
+        };
+        auto rows = [&](uint32_t st, int kb) { tma_load_2d(base + st * C::STAGE + 2 * F8_A_BYTES, &tmX, kb * 128, tl.slot0, &full[st]); };
+        int kb = kb0;
+        if (!waited) {
+          const int n = min(kb1 - kb0, C::ST);
+          for (int i = 0; i < n; ++i) {
+            if (MODE != F8_PLAIN) weights(i, kb0 + i);
+            else { tma_prefetch_2d(&tmW, (kb0 + i) * 128, r0); tma_prefetch_2d(&tmW, (kb0 + i) * 128, r1); }
           }
-          tma_load_2d(sb + 2 * F8_A_BYTES, &tmX, kb * 128, tl.slot0, &full[s]);
+          griddep_wait();
+          waited = true;
+          if (MODE != F8_PLAIN) {
+            for (int i = 0; i < n; ++i) rows(i, kb0 + i);
+            kb += n;
+            s = n == C::ST ? 0 : n; ph = n == C::ST ? 0 : 1;
+          }
+        }
+        for (; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
+          weights(s, kb);
+          rows(s, kb);
           if (++s == C::ST) { s = 0; ph ^= 1u; }
         }
       }
@@ -296,6 +380,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   } else if (warp == F8_W_SCALE) {
     // ------------------------------------------------------------------------------------------------ scales of a step: weight block × row, a step ahead
     constexpr int NL = (BN + 31) / 32;
+    griddep_wait();
     uint32_t it = 0;
     bool ok = true;
     while (ok && sch.next(item, kb0, kb1)) {
@@ -336,6 +421,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
   }
   } else {
     if constexpr (C::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
+    griddep_wait();
+    griddep_launch();
     // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has lanes [32 q, 32 q + 32) and of each weight
     // tile's columns [h·CW, (h + 1)·CW): a lane is a weight row, a column a row of x with a scale of its own, read from shared memory by all lanes together
     const int h = warp >> 2, q = warp & 3, row = 32 * q + lane;
@@ -445,26 +532,27 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const F8Args a,
       }
       // ---- the item's results
       if constexpr (MODE == F8_GU) {
-          uint32_t* am = amx + (h * 4) * C::CW;
+        uint32_t* am = amx + (h * 4) * C::CW;
 #pragma unroll
-          for (int c = 0; c < C::CW; ++c) {
+        for (int c = 0; c < C::CW; ++c) {
+          if (c < cols) {
             acc[0][c] = f8_swiglu(acc[0][c], acc[1][c], a.limit);
             const uint32_t mx = __reduce_max_sync(0xffffffffu, f8_mag(acc[0][c]));
             if (lane == 0) am[q * C::CW + c] = mx;
           }
-          named_bar_sync(2 + h, 128);
+        }
+        named_bar_sync(2 + h, 128);
 #pragma unroll
-          for (int c = 0; c < C::CW; ++c) {
+        for (int c = 0; c < C::CW; ++c) {
+          if (c < cols) {
             F8Block blk;
             const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
-            const uint32_t code = blk.pair(acc[0][c], 0.f);
             const int slot = tl.slot0 + h * C::CW + c;
-            if (c < cols) {
-              a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)code;
-              if (row == 0) a.ys[(size_t)nt * a.ldys + slot] = sc;
-            }
+            a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)blk.pair(acc[0][c], 0.f);
+            if (row == 0) a.ys[(size_t)nt * a.ldys + slot] = sc;
           }
-          named_bar_sync(2 + h, 128);                                          // the magnitudes have been read
+        }
+        named_bar_sync(2 + h, 128);                                            // the magnitudes have been read
       } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {

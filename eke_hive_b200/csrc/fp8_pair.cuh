@@ -21,7 +21,7 @@ constexpr int F8P_ROWS = 256;                          // rows of x a tile may h
 constexpr int F8P_STAGE = 2 * 128 * 128, F8P_ST = 6;   // a stage of one CTA: 128 rows of x, 128 weight rows (64 of each half), 128 values each
 constexpr int F8P_STG = 8 * F8_STG_BYTES;
 constexpr int F8P_SMEM = 1024 + F8P_ST * F8P_STAGE + F8P_STG + 2 * 128 * 4 + 512;
-static_assert(F8P_SMEM <= 227 * 1024, "shared memory");
+static_assert(F8P_ST < F8_MAPS && F8P_SMEM <= 227 * 1024, "map slots, shared memory");
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
@@ -62,7 +62,7 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
 }
 
 template <int MODE>
-__global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+__global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
   extern __shared__ uint8_t f8p_raw[];
   const uint32_t raw = smem_u32(f8p_raw), base = (raw + 1023u) & ~1023u;       // the same offset in both CTAs
   uint8_t* sm = f8p_raw + (base - raw);
@@ -88,8 +88,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a,
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  griddep_wait();
-  griddep_launch();
+  // before griddep_wait: as in fp8_gemm.cuh (the tiles come from the kernel in front of the one in front)
   const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + F8P_ROWS - 1) / F8P_ROWS : *a.n_tiles;
   F8Sched sch;
   sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / 2, blockIdx.x / 2, true);
@@ -105,31 +104,36 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a,
       // ---------------------------------------------------------------------------------------------- operand tiles, one thread of each CTA
       if (elect_one()) {
         uint32_t s = 0, ph = 1;
-        bool ok = true;
-        WmReader wm;
-        if (MODE != F8_PLAIN) wm.init(a.wm);
+        bool ok = true, waited = false;
+        F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
         const uint32_t full0 = mapa_u32(smem_u32(full), 0);
         while (ok && sch.next(item, kb0, kb1)) {
           const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
           const TileRef tl = tile_of(ti);
-          WmBox box;
-          if (MODE != F8_PLAIN && !wm.locate(a.tab[tl.expert] + a.off_w, box, a.err)) break;
-          if (MODE != F8_PLAIN && !box.map) { atomicOr(a.err, 0x400000u); break; }   // out of a map's reach: the copies of a far box count in their own CTA only
-          // this CTA's 64 rows of each half
+          const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab[tl.expert] + a.off_w);
+          // this CTA's 64 rows of each half; rows past the last read as zero codes
           const int r0 = MODE == F8_GU ? nt * 128 + (int)rank * a.row2 : nt * 256 + (int)rank * 64, r1 = r0 + (MODE == F8_GU ? 64 : 128);
-          const bool two = MODE == F8_GU || nt * 256 + 128 < a.N;              // a last item may have one half: beyond it there is other memory
-          for (int kb = kb0; kb < kb1; ++kb) {
+          auto weights = [&](uint32_t st, int kb) {
+            const uint32_t wb = base + st * F8P_STAGE + 128 * 128, bar = full0 + st * 8;
+            if (rank == 0) mbar_expect_tx(&full[st], 2 * F8P_STAGE);
+            tma_load_2d_pair(wb, mw, kb * 128, r0, bar);
+            tma_load_2d_pair(wb + 64 * 128, mw, kb * 128, r1, bar);
+          };
+          auto rows = [&](uint32_t st, int kb) { tma_load_2d_pair(base + st * F8P_STAGE, &tmX, kb * 128, tl.slot0 + (int)rank * 128, full0 + st * 8); };
+          int kb = kb0;
+          if (!waited) {
+            const int n = MODE == F8_PLAIN ? 0 : min(kb1 - kb0, F8P_ST);
+            for (int i = 0; i < n; ++i) weights(i, kb0 + i);
+            griddep_wait();
+            waited = true;
+            for (int i = 0; i < n; ++i) rows(i, kb0 + i);
+            kb += n;
+            s = n == F8P_ST ? 0 : n; ph = n == F8P_ST ? 0 : 1;
+          }
+          for (; kb < kb1; ++kb) {
             if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
-            const uint32_t sb = base + s * F8P_STAGE, wb = sb + 128 * 128, bar = full0 + s * 8;
-            if (rank == 0) mbar_expect_tx(&full[s], 2 * (128 * 128 + (two ? 2 : 1) * 64 * 128));
-            tma_load_2d_pair(sb, &tmX, kb * 128, tl.slot0 + (int)rank * 128, bar);
-            if (MODE == F8_PLAIN) {
-              tma_load_2d_pair(wb, &tmW, kb * 128, r0, bar);
-              if (two) tma_load_2d_pair(wb + 64 * 128, &tmW, kb * 128, r1, bar);
-            } else {
-              tma_load_2d_pair(wb, box.map, kb * 128, box.row + r0, bar);
-              if (two) tma_load_2d_pair(wb + 64 * 128, box.map, kb * 128, box.row + r1, bar);
-            }
+            weights(s, kb);
+            rows(s, kb);
             if (++s == F8P_ST) { s = 0; ph ^= 1u; }
           }
         }
@@ -169,6 +173,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const F8Args a,
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
+    griddep_wait();
+    griddep_launch();
     // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has rows [32 q, 32 q + 32) of half h, a row a lane
     const int h = warp >> 2, q = warp & 3, row = 32 * q + lane;
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + h * 128;

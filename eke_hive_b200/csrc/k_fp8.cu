@@ -69,80 +69,28 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const F8RowsArgs a)
   f8_quant_rows(a, blockIdx.x, gridDim.x);
 }
 
-// The front of a routed layer's call in one launch.  The first CTAs stamp the weight maps of the GEMMs.  Calls of at most F8_PREP_PAIRS pairs are planned here too: a
-// pair's slot is the number of pairs with a smaller expert plus the number of earlier ones with its own, which every CTA counts for the pairs it needs over
-// the whole list in shared memory — no histogram, no meeting of CTAs, no launch in between (the plan kernel for long lists and the quantiser
-// behind it took 19 of a one-row call's 75 us).  One CTA writes the plan down, the others quantise.
-constexpr int F8_PREP_PAIRS = 1024, F8_PREP_STAMP = 4;
-struct F8PrepArgs {
-  F8RowsArgs rows; WmStamp wm;
-  const int32_t* ids; int P, E, bm; const uint8_t* const* tab;                 // P == 0: rows.dest has been worked out before
-  int* pos_of; TileRef* tiles; int* n_tiles;
-};
-__global__ void __launch_bounds__(256) fp8_prep_kernel(const __grid_constant__ F8PrepArgs a) {
-  __shared__ int4 e4[F8_PREP_PAIRS / 4];
+// The front of a routed layer's call with a short list of pairs, in one launch: CTA 0 writes the plan down (the slots for the sum at the end, the tiles for the down
+// pass; the gate/up pass finds them for itself), the others work out the slots of their rows and quantise.  (A plan kernel and the quantiser behind it took 19 of a
+// one-row call's 75 us.)
+struct F8PrepArgs { F8RowsArgs rows; F8Plan plan; int* pos_of; TileRef* tiles; int* n_tiles; };
+__global__ void __launch_bounds__(256) fp8_prep_kernel(const F8PrepArgs a) {
+  __shared__ __align__(16) uint8_t tmp[F8_PLAN_PAIRS * 4 + F8_PLAN_PAIRS / 8];
   __shared__ int slots[512];
-  __shared__ uint32_t flag[F8_PREP_PAIRS / 32];
-  int* e_s = reinterpret_cast<int*>(e4);
+  const int t = threadIdx.x;
   griddep_wait();
   griddep_launch();
-  if (blockIdx.x < F8_PREP_STAMP) { wm_stamp(a.wm, blockIdx.x, F8_PREP_STAMP); return; }
-  if (a.P == 0) { f8_quant_rows(a.rows, blockIdx.x - F8_PREP_STAMP, gridDim.x - F8_PREP_STAMP); return; }
-  constexpr int NONE = 0x7fffffff;
-  const int t = threadIdx.x, P = a.P, P4 = (P + 3) / 4;
-  for (int p = t; p < P4 * 4; p += 256) {
-    const int e = p < P ? __ldg(a.ids + p) : -1;
-    e_s[p] = e >= 0 && e < a.E && __ldg(reinterpret_cast<const unsigned long long*>(a.tab) + e) != 0ull ? e : NONE;
-  }
-  if (t < F8_PREP_PAIRS / 32) flag[t] = 0u;
-  __syncthreads();
-  struct At { int slot, rank, run; };
-  auto place = [&](int p) -> At {
-    const int e = e_s[p];
-    int less = 0, before = 0, run = 0;
-#pragma unroll 4
-    for (int i = 0; i < P4; ++i) {
-      const int4 v = e4[i];
-      less += (v.x < e) + (v.y < e) + (v.z < e) + (v.w < e);
-      const int c = (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
-      run += c;
-      if (4 * i + 4 <= p) before += c;
-      else before += (v.x == e && 4 * i < p) + (v.y == e && 4 * i + 1 < p) + (v.z == e && 4 * i + 2 < p);
-    }
-    return e == NONE ? At{-1, 0, 0} : At{less + before, before, run};
-  };
-  if (blockIdx.x == F8_PREP_STAMP) {
-    // a tile starts at every tper-th pair of a run; its number is that of the starts in front of it
-    At at[F8_PREP_PAIRS / 256]; int tper[F8_PREP_PAIRS / 256];
-#pragma unroll
-    for (int i = 0; i < F8_PREP_PAIRS / 256; ++i) {
-      const int p = t + 256 * i;
-      if (p >= P) break;
-      at[i] = place(p);
-      a.pos_of[p] = at[i].slot;
-      if (at[i].slot < 0) continue;
-      const int nt = (at[i].run + a.bm - 1) / a.bm;
-      tper[i] = (at[i].run + nt - 1) / nt;
-      if (at[i].rank % tper[i] == 0) atomicOr(&flag[at[i].slot >> 5], 1u << (at[i].slot & 31));
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < F8_PREP_PAIRS / 256; ++i) {
-      const int p = t + 256 * i;
-      if (p >= P) break;
-      if (at[i].slot < 0 || at[i].rank % tper[i] != 0) continue;
-      int n = __popc(flag[at[i].slot >> 5] & ((1u << (at[i].slot & 31)) - 1u));
-      for (int w = 0; w < at[i].slot >> 5; ++w) n += __popc(flag[w]);
-      TileRef tl; tl.slot0 = at[i].slot; tl.rows = min(tper[i], at[i].run - at[i].rank); tl.expert = e_s[p];
-      a.tiles[n] = tl;
-    }
-    if (t == 0) { int n = 0; for (int w = 0; w < F8_PREP_PAIRS / 32; ++w) n += __popc(flag[w]); *a.n_tiles = n; }
+  if (blockIdx.x == 0) {
+    const int n = f8_plan_tiles(a.plan, tmp, a.tiles, 256, a.pos_of);
+    if (t == 0) *a.n_tiles = n;
     return;
   }
-  // 16 blocks of 128 values a CTA: their rows' slots first
-  const int nb = f8_blocks(a.rows.K), u0 = (blockIdx.x - F8_PREP_STAMP - 1) * 16, total = a.rows.M * nb, nd = a.rows.nd;
+  // 16 blocks of 128 values a CTA
+  int* e_s = reinterpret_cast<int*>(tmp);
+  f8_plan_load(a.plan, e_s, 256);
+  __syncthreads();
+  const int nb = f8_blocks(a.rows.K), u0 = (blockIdx.x - 1) * 16, total = a.rows.M * nb, nd = a.rows.nd;
   const int m0 = u0 / nb, m1 = min(u0 + 15, total - 1) / nb;
-  for (int i = t; i < (m1 - m0 + 1) * nd; i += 256) slots[i] = place(m0 * nd + i).slot;
+  for (int i = t; i < (m1 - m0 + 1) * nd; i += 256) slots[i] = f8_plan_at(a.plan, e_s, m0 * nd + i).slot;
   __syncthreads();
   const int u = u0 + (t >> 4), l16 = t & 15;
   if (u < total) {
@@ -153,6 +101,7 @@ __global__ void __launch_bounds__(256) fp8_prep_kernel(const __grid_constant__ F
     }
   }
 }
+
 // Weights: a CTA takes a block of 128 × 128, sixteen lanes a row of it, eight rows a thread.
 template <class T>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ w, int N, int K, uint8_t* __restrict__ q, float* __restrict__ s) {
@@ -208,7 +157,7 @@ struct F8SumArgs {
   const __nv_bfloat16* shared; const float* lg; int ld, col; __nv_bfloat16* cout;
 };
 __global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs a) {
-  griddep_wait();
+  bool waited = false;                                                         // only the parts are of the kernel in front
   const int chunks = (a.H + 255) / 256, lane = threadIdx.x & 31;
   const long long total = (long long)a.M * chunks;
   constexpr int WARPS = F8_SUM_THREADS / 32;
@@ -220,6 +169,7 @@ __global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs
     const float wk = slot >= 0 ? __ldg(a.w + (size_t)m * a.K + lane) : 0.f;
     const uint4 sv = a.shared && in ? __ldg(reinterpret_cast<const uint4*>(a.shared + o)) : make_uint4(0u, 0u, 0u, 0u);
     const float gate = a.lg ? 1.f / (1.f + expf(-__ldg(a.lg + (size_t)m * a.ld + a.col))) : 1.f;
+    if (!waited) { griddep_wait(); waited = true; }
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
@@ -298,7 +248,7 @@ int f8_map(hb_ctx* ctx, CUtensorMap* m, const void* base, size_t row_bytes, size
 }
 
 struct F8Ws {
-  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; uint8_t* yq; float* ys; __nv_bfloat16* part; float* cut; uint8_t* wmaps;
+  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; uint8_t* yq; float* ys; __nv_bfloat16* part; float* cut; uint8_t* maps;
 };
 size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   size_t off = 0;
@@ -312,7 +262,7 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   t.yq = (uint8_t*)take(P * I); t.ys = (float*)take(P * f8_blocks(I) * 4);
   t.part = (__nv_bfloat16*)take(P * H * 2);
   t.cut = (float*)take(f8_part_bytes(bn));
-  t.wmaps = (uint8_t*)take(wm_bytes(2 * H) + wm_bytes(2 * I));               // (the maps count e2m1 columns, two to a byte)
+  t.maps = (uint8_t*)take((size_t)2 * F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap));   // of the gate/up pass and of the down pass
   if (w) *w = t;
   return off;
 }
@@ -418,37 +368,38 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   f8_carve(ws, M, K, E, H, I, &W);
   const int P = M * K, rows = f8_rows_for_pairs(P, E), box = rows == F8P_ROWS ? 128 : rows;
   int r;
+  // maps of a record's matrices (gate and up lie one behind the other), to be given their addresses on the device; of the rows of x and y
+  CUtensorMap tg, td, tx, ty;
+  const int wbox = rows == F8P_ROWS ? 64 : 128;
+  if ((r = f8_map(ctx, &tg, W.xq, H, H, 2 * I, wbox)) || (r = f8_map(ctx, &td, W.xq, I, I, H, wbox))) return r;
+  if ((r = f8_map(ctx, &tx, W.xq, H, H, P, box)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, box))) return r;
   F8PrepArgs pr{};
   F8RowsArgs& q = pr.rows;
   q.x = reinterpret_cast<const __nv_bfloat16*>(x); q.ldx = H; q.M = M; q.K = H; q.dest = W.pos_of; q.nd = K; q.q = W.xq; q.ldq = H; q.s = W.xs; q.lds = P;
-  if ((r = hbk_wm_stamp_args(ctx, tab, E, nullptr, 2 * H, 2 * I, W.wmaps, &pr.wm))) return r;
-  CUtensorMap tx, ty;
-  if ((r = f8_map(ctx, &tx, W.xq, H, H, P, box)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, box))) return r;
-  const long long units = (long long)M * f8_blocks(H), cap = (long long)ctx->sm_count * 32;
-  long long ctas = (units + 15) / 16;
-  if (P <= F8_PREP_PAIRS) {
-    pr.ids = ids; pr.P = P; pr.E = E; pr.bm = rows; pr.tab = tab; pr.pos_of = W.pos_of; pr.tiles = W.tiles; pr.n_tiles = W.n_tiles;
-    ++ctas;
+  const bool own_plan = P <= F8_PLAN_PAIRS && rows != F8P_ROWS;
+  if (own_plan) {
+    pr.plan = F8Plan{ids, P, E, rows, tab}; pr.pos_of = W.pos_of; pr.tiles = W.tiles; pr.n_tiles = W.n_tiles;
+    if ((r = hb_launch(ctx, "fp8_prep", true, fp8_prep_kernel, dim3(1 + (unsigned)((M * f8_blocks(H) + 15) / 16)), dim3(256), 0, st, pr))) return r;
   } else {
-    if (ctas > cap) ctas = cap;
     if ((r = hbk_pf_plan(ctx, hbk_plan{ids, P, E, tab, rows, W.hist, W.perm, W.pos_of, W.tiles, W.n_tiles, W.n_slots}, st))) return r;
+    if ((r = f8_rows(ctx, q, st))) return r;
   }
-  if ((r = hb_launch(ctx, "fp8_prep", true, fp8_prep_kernel, dim3(F8_PREP_STAMP + (unsigned)ctas), dim3(256), 0, st, pr))) return r;
   F8Args a{};
   a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.count = f8_counters(ctx); a.err = ctx->dev_err;
-  a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.wm = wm_args(W.wmaps, 2 * H);
+  a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.maps = W.maps;
   a.xs = W.xs; a.lds = P; a.yq = W.yq; a.ys = W.ys; a.ldys = P;
-  if ((r = f8_launch<F8_GU>(ctx, "fp8_gemm_gu", rows, a, tx, tx, st))) return r;
-  a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.wm = wm_args(W.wmaps + wm_bytes(2 * H), 2 * I);
+  if (own_plan) a.plan = pr.plan;
+  if ((r = f8_launch<F8_GU>(ctx, "fp8_gemm_gu", rows, a, tg, tx, st))) return r;
+  a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.maps = W.maps + (size_t)F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap);
   a.xs = W.ys; a.yb = W.part; a.ldy = H;
-  if ((r = f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, ty, ty, st))) return r;
+  if ((r = f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, td, ty, st))) return r;
   F8SumArgs su{W.part, W.pos_of, w, M, K, H, out, nullptr, nullptr, 0, 0, nullptr};
   if (cmb) {
     su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
     if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
   }
-  const long long sums = ((long long)M * ((H + 255) / 256) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32);
-  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(sums < cap / 2 ? sums : cap / 2)), dim3(F8_SUM_THREADS), 0, st, su);
+  const long long sums = ((long long)M * ((H + 255) / 256) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
+  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(sums < cap ? sums : cap)), dim3(F8_SUM_THREADS), 0, st, su);
 }
 
 }  // extern "C"

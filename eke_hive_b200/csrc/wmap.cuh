@@ -24,9 +24,8 @@ struct WmStamp {
   const uint8_t* const* tab; int n_tab; const uint8_t* extra;          // the call's records: a table and one more (or nullptr)
   uint8_t* dst[2]; int nv[2];                                          // where the maps go, how many
 };
-// The whole block takes part; with several blocks each stamps every parts-th map.  The maps are complete for kernels behind this one that acquire them
-// (tmap_acquire).
-__device__ __forceinline__ void wm_stamp(const WmStamp& s, int part = 0, int parts = 1) {
+// The whole block takes part.  The maps are complete for kernels behind this one that acquire them (tmap_acquire).
+__device__ __forceinline__ void wm_stamp(const WmStamp& s) {
   __shared__ unsigned long long lo;
   if (threadIdx.x == 0) lo = s.extra ? reinterpret_cast<unsigned long long>(s.extra) : ~0ull;
   __syncthreads();
@@ -37,8 +36,8 @@ __device__ __forceinline__ void wm_stamp(const WmStamp& s, int part = 0, int par
   if ((threadIdx.x & 31) == 0) atomicMin(&lo, mn);
   __syncthreads();
   const unsigned long long anchor = lo == ~0ull ? 1ull << 40 : lo & ~15ull;
-  if (threadIdx.x < 2 && part == 0) *reinterpret_cast<unsigned long long*>(threadIdx.x ? s.dst[1] : s.dst[0]) = anchor;
-  for (int i = threadIdx.x * parts + part; i < s.nv[0] + s.nv[1]; i += blockDim.x * parts) {
+  if (threadIdx.x < 2) *reinterpret_cast<unsigned long long*>(threadIdx.x ? s.dst[1] : s.dst[0]) = anchor;
+  for (int i = threadIdx.x; i < s.nv[0] + s.nv[1]; i += blockDim.x) {
     const bool dn = i >= s.nv[0];
     const int v = dn ? i - s.nv[0] : i;
     const uint4* src = reinterpret_cast<const uint4*>(dn ? &s.tpl[1] : &s.tpl[0]);
@@ -68,7 +67,7 @@ struct WmReader {
     b.map = nullptr; b.row = 0; b.far = w;
     if (row + (1ull << 24) < (1ull << 31)) {
       b.map = reinterpret_cast<const CUtensorMap*>(a.base + kWmHead) + (rem >> 4); b.row = (int)row;
-      const uint32_t bit = (rem & ((1u << a.gshift) - 1u)) || (rem >> a.gshift) > 31u ? 0u : 1u << (rem >> a.gshift);
+      const uint32_t bit = rem & ((1u << a.gshift) - 1u) ? 0u : 1u << (rem >> a.gshift);
       if (!(seen & bit)) { tmap_acquire(b.map); seen |= bit; }
     }
     return true;
