@@ -57,6 +57,26 @@ __device__ __forceinline__ F8At f8_plan_at(const F8Plan& a, const int* e_s, int 
 // pair of a run, and its number is that of the starts at smaller slots.  Returns the number of tiles; the caller synchronises before the list is read.
 // slots: where pair p's slot goes (or nullptr).
 __device__ __forceinline__ int f8_plan_tiles(const F8Plan& a, uint8_t* tmp, TileRef* tiles, int threads, int* slots = nullptr) {
+  if (a.P <= 32) {                                     // a token or a few: one warp, a pair a lane (a kernel's code comes from afar the first time: the less, the sooner)
+    uint32_t starts = 0u;
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x;
+      int e = lane < a.P ? __ldg(a.ids + lane) : -1;
+      if (e < 0 || e >= a.E || __ldg(reinterpret_cast<const unsigned long long*>(a.tab) + e) == 0ull) e = 0x7fffffff;
+      int less = 0;
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) less += __shfl_sync(0xffffffffu, e, i) < e;
+      const uint32_t same = __match_any_sync(0xffffffffu, e), front = same & ((1u << lane) - 1u);
+      const int rank = __popc(front), run = __popc(same), slot = less + rank, nt = (run + a.bm - 1) / a.bm, tper = (run + nt - 1) / nt;
+      const bool on = e != 0x7fffffff, start = on && rank % tper == 0;
+      starts = __reduce_or_sync(0xffffffffu, start ? 1u << slot : 0u);
+      if (start) tiles[__popc(starts & ((1u << slot) - 1u))] = TileRef{slot, min(tper, run - rank), e};
+      if (slots && lane < a.P) slots[lane] = on ? slot : -1;
+      if (lane == 0) *reinterpret_cast<int*>(tmp) = __popc(starts);
+    }
+    __syncthreads();
+    return *reinterpret_cast<const int*>(tmp);
+  }
   int* e_s = reinterpret_cast<int*>(tmp);
   uint32_t* flag = reinterpret_cast<uint32_t*>(e_s + F8_PLAN_PAIRS);
   f8_plan_load(a, e_s, threads);
@@ -195,24 +215,27 @@ __device__ __forceinline__ uint4 f8_pack8(const float* v) {                     
   return make_uint4(p[0], p[1], p[2], p[3]);
 }
 // A warp's staged 32 rows × 64 bytes to memory, eight rows an instruction (a lane has a row: its own stores would touch 32 rows each).  to: the first
-// row's place; bytes: how much of a row there is room for; es: bytes of an element.
-__device__ __forceinline__ void f8_flush(const uint8_t* stg, uint8_t* to, size_t ld, int rows, int bytes, int es, int lane) {
+// row's place; bytes: how much of a row there is room for.
+__device__ __forceinline__ void f8_flush(const uint8_t* stg, uint8_t* to, size_t ld, int rows, int bytes, int lane) {
   __syncwarp();
   const int c = (lane & 3) * 16;
-  const bool wide = ((reinterpret_cast<uintptr_t>(to) | ld) & 15) == 0;
+  const uint32_t al = (uint32_t)(reinterpret_cast<uintptr_t>(to) | ld) & 15u;   // what all rows' places are aligned to: 0: 16 bytes
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 8 * i + (lane >> 2);
     const uint4 v = *reinterpret_cast<const uint4*>(stg + r * F8_STG_PITCH + c);
     if (r >= rows) continue;
     uint8_t* p = to + (size_t)r * ld + c;
-    if (wide && c + 16 <= bytes) *reinterpret_cast<uint4*>(p) = v;
-    else if (c < bytes) {
+    if (al == 0 && c + 16 <= bytes) *reinterpret_cast<uint4*>(p) = v;
+    else if ((al & 7u) == 0 && c + 16 <= bytes) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(p + 8) = make_uint2(v.z, v.w);
+    } else {
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (es == 4) { if (c + 4 * j < bytes) *reinterpret_cast<uint32_t*>(p + 4 * j) = w[j]; }
-        else {
+        if ((al & 3u) == 0 && c + 4 * j + 4 <= bytes) *reinterpret_cast<uint32_t*>(p + 4 * j) = w[j];
+        else {                                                                 // (a row of fp32 has room for whole words)
           if (c + 4 * j < bytes) *reinterpret_cast<uint16_t*>(p + 4 * j) = (uint16_t)(w[j] & 0xffffu);
           if (c + 4 * j + 2 < bytes) *reinterpret_cast<uint16_t*>(p + 4 * j + 2) = (uint16_t)(w[j] >> 16);
         }
