@@ -17,21 +17,39 @@ __host__ __device__ constexpr int f8_blocks(int n) { return (n + F8_B - 1) / F8_
 // Blocks of very small or very large values are brought to the middle of the range by a power of two first: nothing over- or underflows
 // that could be more than a zero code.
 struct F8Block {
-  float f, d, r; bool live;                            // v·f is the value scaled, d = amax·f, r = 1 / d
+  float f448, f, d, r; bool live;                      // f: the power of two; d = amax·f, r = 1 / d
   __device__ __forceinline__ float init(uint32_t bits) {   // returns the scale
     const float amax = __uint_as_float(bits);
     live = bits > 0u && bits < 0x7f800000u;
     f = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.f;
+    f448 = f * 448.f;
     d = __fmul_rn(amax, f); r = live ? __frcp_rn(d) : 0.f;
-    return bits < 0x7f800000u ? __fdiv_rn(amax, 448.f) : __int_as_float(0x7fc00000);
+    if (bits >= 0x7f800000u) return __int_as_float(0x7fc00000);
+    const float q = __fmul_rn(amax, 1.f / 448.f);
+    return amax > 0x1p-90f ? __fmaf_rn(__fmaf_rn(-q, 448.f, amax), 1.f / 448.f, q) : __fdiv_rn(amax, 448.f);
   }
-  __device__ __forceinline__ float quotient(float v) const {
-    const float t = __fmul_rn(__fmul_rn(v, f), 448.f), q = __fmul_rn(t, r);
-    return copysignf(__fmaf_rn(__fmaf_rn(-q, d, t), r, q), t);
+  __device__ __forceinline__ float quotient(float v) const {   // (a zero comes out as +0)
+    const float t = __fmul_rn(v, f448), q = __fmul_rn(t, r);
+    return __fmaf_rn(__fmaf_rn(-q, d, t), r, q);
   }
   __device__ __forceinline__ uint32_t pair(float a, float b) const {   // codes of two values, the first in the low byte
     uint16_t o;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(quotient(b)), "f"(quotient(a)));
+    return live ? (uint32_t)o : 0u;
+  }
+};
+// The same for values that are themselves rounded fp32 results (y of a routed expert): v · (448 / amax), one rounding more and no tie to be seen as one.
+struct F8BlockFast {
+  float f, k; bool live;
+  __device__ __forceinline__ float init(uint32_t bits) {
+    F8Block b;
+    const float s = b.init(bits);
+    f = b.f; live = b.live; k = live ? __fdiv_rn(448.f, b.d) : 0.f;
+    return s;
+  }
+  __device__ __forceinline__ uint32_t pair(float a, float b) const {
+    uint16_t o;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(__fmul_rn(__fmul_rn(b, f), k)), "f"(__fmul_rn(__fmul_rn(a, f), k)));
     return live ? (uint32_t)o : 0u;
   }
 };

@@ -206,7 +206,7 @@ __device__ __forceinline__ void f8_fma2(float& a0, float& a1, uint32_t d0, uint3
 }
 __device__ __forceinline__ float f8_swiglu(float g, float u, float limit) {
   if (limit > 0.f) { g = fminf(g, limit); u = fminf(fmaxf(u, -limit), limit); }
-  return g / (1.f + expf(-g)) * u;
+  return __fdividef(g, 1.f + expf(-g)) * u;                                    // (two steps; y is rounded to three bits next)
 }
 __device__ __forceinline__ uint4 f8_pack8(const float* v) {                     // eight values as bf16
   uint32_t p[4];
@@ -257,11 +257,6 @@ template <int W>
 __device__ __forceinline__ void f8_add(float* acc, const uint32_t (&d)[W], float s) {
 #pragma unroll
   for (int c = 0; c < W; c += 2) f8_fma2(acc[c], acc[c + 1], d[c], d[c + 1], s, s);
-}
-__device__ __forceinline__ bool named_bar_and(int id, int threads, bool v) {   // barrier of `threads` threads; true where all bring true
-  uint32_t o;
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(o) : "r"(id), "r"(threads), "r"((uint32_t)v) : "memory");
-  return o != 0;
 }
 // The columns asked for before have arrived; the registers are named so that nothing that reads them is moved in front of it.
 template <int W>
@@ -452,7 +447,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + h * C::CW;
     uint32_t it = 0;
     bool ok = true;
-    while (ok && sch.next(item, kb0, kb1)) {
+    while (sch.next(item, kb0, kb1)) {                                          // after a wait that gave up: on to the end without waits and results, but through every barrier
       const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
       const TileRef tl = tile_of(ti);
       const int cols = min(max(tl.rows - h * C::CW, 0), C::CW);                // this warp's columns that hold rows of x
@@ -473,7 +468,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         f8_ld<C::LD>(t + (n / half) * BN + (n % half) * C::LD, ra);
         f8_ld<C::LD>(t + ((n + 1) / half) * BN + ((n + 1) % half) * C::LD, rb);
       };
-      if ((ok = arrived(it)) && active) read2(trow + (it & 1u) * (2 * BN), 0);
+      if ((ok = ok && arrived(it)) && active) read2(trow + (it & 1u) * (2 * BN), 0);
       for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
         const uint32_t buf = it & 1u, tb = trow + buf * (2 * BN);
         const float* sb = scl + (it & 3u) * (2 * BN) + h * C::CW;
@@ -505,7 +500,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         }
       }
       // ---- an item that other CTAs have parts of: leave the sums, the last one to arrive goes on with everybody's
-      if (!(ok = named_bar_and(1, 256, ok))) break;
       if (kb1 - kb0 < KB) {
         const uint32_t s0 = (uint32_t)item * (uint32_t)KB, c_first = sch.owner(s0), c_last = sch.owner(s0 + KB - 1);
         // a part: [column][tile][lane]; a CTA's first run is its part 0
@@ -515,7 +509,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         for (int c = 0; c < C::CW; ++c)
           if (active && c < cols) { __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]); }
         named_bar_sync(1, 256);
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && !ok) *last = 0u;
+        else if (threadIdx.x == 0) {
           __threadfence();                                                     // everybody's sums are out before this CTA is counted
           const bool all = atomicAdd(a.count + item, 1u) == c_last - c_first;
           if (all) a.count[item] = 0u;                                         // zero again for the next launch
@@ -567,8 +562,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         named_bar_sync(2 + h, 128);
 #pragma unroll
         for (int c = 0; c < C::CW; ++c) {
-          if (c < cols) {
-            F8Block blk;
+          if (c < cols && ok) {
+            F8BlockFast blk;
             const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
             const int slot = tl.slot0 + h * C::CW + c;
             a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)blk.pair(acc[0][c], 0.f);
@@ -580,7 +575,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int n = nt * 256 + u * 128 + row;
-          if (n < a.N) {
+          if (n < a.N && ok) {
 #pragma unroll
             for (int c = 0; c < C::CW; ++c)
               if (c < cols) {

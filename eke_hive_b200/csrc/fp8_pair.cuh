@@ -1,8 +1,9 @@
-// The product of fp8_gemm.cuh for many rows: two CTAs of a cluster work on one tile of 256 rows of x × 256 weight rows (tcgen05 cta_group::2).
+// The product of fp8_gemm.cuh for many rows: two CTAs of a cluster work on one tile of 256 rows of x × 256 weight rows (tcgen05 cta_group::2), or one CTA on a
+// tile of 128 rows.
 //
 // Rows of x are the A operand, 128 of them in each CTA's shared and tensor memory; the weight rows are the B operand, of which each CTA loads half
 // and both read all: 32 KB of operands per CTA and step for 128 × 256 × 128 multiply-adds.  (One CTA alone needs 48 KB for them, and the SMs pull no more than
-// some 10 TB/s out of L2: 1.7 PFLOP/s.)  A lane of tensor memory is a row of x: the scale of a step is one number a thread, the row's
+// some 10 TB/s out of L2: 1.7 PFLOP/s.  That form is for calls whose runs of rows would leave much of a pair's tile empty.)  A lane of tensor memory is a row of x: the scale of a step is one number a thread, the row's
 // times the weight block's.
 //
 // The 256 weight rows are two halves of 128, each with an accumulator of its own, double buffered (all of tensor memory), and its own warps: warps 0-3 read
@@ -17,11 +18,16 @@
 
 namespace hb {
 
-constexpr int F8P_ROWS = 256;                          // rows of x a tile may have
-constexpr int F8P_STAGE = 2 * 128 * 128, F8P_ST = 6;   // a stage of one CTA: 128 rows of x, 128 weight rows (64 of each half), 128 values each
-constexpr int F8P_STG = 8 * F8_STG_BYTES;
-constexpr int F8P_SMEM = 1024 + F8P_ST * F8P_STAGE + F8P_STG + 2 * 128 * 4 + 512;
-static_assert(F8P_ST < F8_MAPS && F8P_SMEM <= 227 * 1024, "map slots, shared memory");
+constexpr int F8S_ROWS = 128, F8P_ROWS = 256;          // rows of x a tile may have: one CTA, a pair
+template <bool PAIR>
+struct F8PCfg {
+  static constexpr int CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS;
+  static constexpr int XB = 128 * 128, HB = 128 * 128 / CTAS;   // a stage of one CTA: 128 rows of x, its rows of each half (64 or 128), 128 values each
+  static constexpr int STAGE = XB + 2 * HB, ST = PAIR ? 6 : 4;
+  static constexpr int STG = 8 * F8_STG_BYTES;
+  static constexpr int SMEM = 1024 + ST * STAGE + STG + 2 * 128 * 4 + 512;
+  static_assert(ST < F8_MAPS && SMEM <= 227 * 1024, "map slots, shared memory");
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
@@ -61,40 +67,55 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
                ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
 
-template <int MODE>
-__global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+template <bool PAIR>
+__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR) tc_mma2_f8(d, ad, bd, idesc, accumulate);
+  else tc_mma_f8(d, ad, bd, idesc, accumulate);
+}
+template <bool PAIR>
+__device__ __forceinline__ void f8_commit(uint64_t* bar) {
+  if constexpr (PAIR) tc_commit2(bar);
+  else tc_commit(bar);
+}
+
+template <int MODE, bool PAIR>
+__global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+  using C = F8PCfg<PAIR>;
   extern __shared__ uint8_t f8p_raw[];
   const uint32_t raw = smem_u32(f8p_raw), base = (raw + 1023u) & ~1023u;       // the same offset in both CTAs
   uint8_t* sm = f8p_raw + (base - raw);
-  uint32_t* amx = reinterpret_cast<uint32_t*>(sm + F8P_ST * F8P_STAGE + F8P_STG);   // magnitudes of y [2 halves][128 rows]
+  uint32_t* amx = reinterpret_cast<uint32_t*>(sm + C::ST * C::STAGE + C::STG);   // magnitudes of y [2 halves][128 rows]
   uint64_t* full = reinterpret_cast<uint64_t*>(amx + 256);                     // [ST] CTA 0: both CTAs' operands of the stage have landed
-  uint64_t* empty = full + F8P_ST;                                             // [ST] each CTA: the MMAs that read the stage are done
-  uint64_t* acc_full = empty + F8P_ST;                                         // [2 halves][2 buffers] each CTA: its sums are there
+  uint64_t* empty = full + C::ST;                                             // [ST] each CTA: the MMAs that read the stage are done
+  uint64_t* acc_full = empty + C::ST;                                         // [2 halves][2 buffers] each CTA: its sums are there
   uint64_t* acc_empty = acc_full + 4;                                          // [2][2] CTA 0: both CTAs have read them
   uint64_t* mma_done = acc_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile uint32_t* last = tmem_slot + 1;
   const int warp = warp_uniform(), lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < F8P_ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
-    for (int s = 0; s < 4; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+    for (int s = 0; s < C::ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
+    for (int s = 0; s < 4; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * C::CTAS); }
     mbar_init(mma_done, 2);
     mbar_fence_init();
   }
-  if (warp == F8_W_MMA) tmem_alloc2(tmem_slot, 512);
+  if (warp == F8_W_MMA) {
+    if constexpr (PAIR) tmem_alloc2(tmem_slot, 512);
+    else { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if constexpr (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // before griddep_wait: as in fp8_gemm.cuh (the tiles come from the kernel in front of the one in front)
-  const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + F8P_ROWS - 1) / F8P_ROWS : *a.n_tiles;
+  const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / 2, blockIdx.x / 2, true);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / C::CTAS, blockIdx.x / C::CTAS, true);
   auto tile_of = [&](int ti) -> TileRef {
     if (MODE != F8_PLAIN) return a.tiles[ti];
-    return TileRef{ti * F8P_ROWS, min(F8P_ROWS, a.M - ti * F8P_ROWS), 0};
+    return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
   };
   int item, kb0, kb1;
 
@@ -106,41 +127,50 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         uint32_t s = 0, ph = 1;
         bool ok = true, waited = false;
         F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
-        const uint32_t full0 = mapa_u32(smem_u32(full), 0);
+        const uint32_t full0 = PAIR ? mapa_u32(smem_u32(full), 0) : 0u;
         while (ok && sch.next(item, kb0, kb1)) {
           const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
           const TileRef tl = tile_of(ti);
           const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab[tl.expert] + a.off_w);
-          // this CTA's 64 rows of each half; rows past the last read as zero codes
-          const int r0 = MODE == F8_GU ? nt * 128 + (int)rank * a.row2 : nt * 256 + (int)rank * 64, r1 = r0 + (MODE == F8_GU ? 64 : 128);
+          // rows of each half, in boxes of 64: of a pair each CTA loads one, else both are this CTA's.  Rows past the last read as zero codes
+          const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, box = MODE == F8_GU ? a.row2 : 64, half = MODE == F8_GU ? 64 : 128;
           auto weights = [&](uint32_t st, int kb) {
-            const uint32_t wb = base + st * F8P_STAGE + 128 * 128, bar = full0 + st * 8;
-            if (rank == 0) mbar_expect_tx(&full[st], 2 * F8P_STAGE);
-            tma_load_2d_pair(wb, mw, kb * 128, r0, bar);
-            tma_load_2d_pair(wb + 64 * 128, mw, kb * 128, r1, bar);
+            const uint32_t wb = base + st * C::STAGE + C::XB, bar = full0 + st * 8;
+            if (rank == 0) mbar_expect_tx(&full[st], C::CTAS * C::STAGE);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if constexpr (PAIR) tma_load_2d_pair(wb + h * C::HB, mw, kb * 128, r0 + h * half + (int)rank * box, bar);
+              else {
+                tma_load_2d(wb + h * C::HB, mw, kb * 128, r0 + h * half, &full[st]);
+                tma_load_2d(wb + h * C::HB + C::HB / 2, mw, kb * 128, r0 + h * half + box, &full[st]);
+              }
+            }
           };
-          auto rows = [&](uint32_t st, int kb) { tma_load_2d_pair(base + st * F8P_STAGE, &tmX, kb * 128, tl.slot0 + (int)rank * 128, full0 + st * 8); };
+          auto rows = [&](uint32_t st, int kb) {
+            if constexpr (PAIR) tma_load_2d_pair(base + st * C::STAGE, &tmX, kb * 128, tl.slot0 + (int)rank * 128, full0 + st * 8);
+            else tma_load_2d(base + st * C::STAGE, &tmX, kb * 128, tl.slot0, &full[st]);
+          };
           int kb = kb0;
           if (!waited) {
-            const int n = MODE == F8_PLAIN ? 0 : min(kb1 - kb0, F8P_ST);
+            const int n = MODE == F8_PLAIN ? 0 : min(kb1 - kb0, C::ST);
             for (int i = 0; i < n; ++i) weights(i, kb0 + i);
             griddep_wait();
             waited = true;
             for (int i = 0; i < n; ++i) rows(i, kb0 + i);
             kb += n;
-            s = n == F8P_ST ? 0 : n; ph = n == F8P_ST ? 0 : 1;
+            s = n == C::ST ? 0 : n; ph = n == C::ST ? 0 : 1;
           }
           for (; kb < kb1; ++kb) {
             if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
             weights(s, kb);
             rows(s, kb);
-            if (++s == F8P_ST) { s = 0; ph ^= 1u; }
+            if (++s == C::ST) { s = 0; ph ^= 1u; }
           }
         }
-        // CTA 0 announces free stages to both CTAs: the last announcements arrive before either ends
-        for (int n = 0; ok && n < F8P_ST; ++n) {
+        // free stages are announced to both CTAs of a pair: the last announcements arrive before either ends
+        for (int n = 0; ok && n < C::ST; ++n) {
           ok = mbar_wait(&empty[s], ph, a.err, 0x100u);
-          if (++s == F8P_ST) { s = 0; ph ^= 1u; }
+          if (++s == C::ST) { s = 0; ph ^= 1u; }
         }
       }
     } else if ((warp == F8_W_MMA || warp == F8_W_MMA + 1) && rank == 0) {
@@ -150,25 +180,25 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         const uint32_t h = warp - F8_W_MMA;
         uint32_t s = 0, ph = 0, it = 0;
         bool ok = true;
-        // kind::f8f6f4: D fp32 (bit 4), A and B e4m3, both K-major, N / 8 = 16 at bit 17, M / 16 = 16 at bit 24
-        constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((256u >> 4) << 24);
-        const uint64_t ad0 = tc_desc_sw128(base), bd0 = tc_desc_sw128(base + 128 * 128 + h * (64 * 128));
+        // kind::f8f6f4: D fp32 (bit 4), A and B e4m3, both K-major, N / 8 = 16 at bit 17, M / 16 at bit 24
+        constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((uint32_t)(C::ROWS >> 4) << 24);
+        const uint64_t ad0 = tc_desc_sw128(base), bd0 = tc_desc_sw128(base + C::XB + h * C::HB);
         while (ok && sch.next(item, kb0, kb1)) {
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t buf = it & 1u;
             if (!(ok = mbar_wait(&full[s], ph, a.err, 0x400u))) break;
             if (!(ok = mbar_wait(&acc_empty[h * 2 + buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x200u))) break;
             tc_fence_after();
-            const uint64_t ad = ad0 + s * (uint32_t)(F8P_STAGE >> 4), bd = bd0 + s * (uint32_t)(F8P_STAGE >> 4);
+            const uint64_t ad = ad0 + s * (uint32_t)(C::STAGE >> 4), bd = bd0 + s * (uint32_t)(C::STAGE >> 4);
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)                                   // 32 values further along the swizzled rows
-              tc_mma2_f8(tmem + buf * 256 + h * 128, ad + 2 * j, bd + 2 * j, idesc, j);
-            tc_commit2(&acc_full[h * 2 + buf]);
-            tc_commit2(&empty[s]);
-            if (++s == F8P_ST) { s = 0; ph ^= 1u; }
+              f8_mma<PAIR>(tmem + buf * 256 + h * 128, ad + 2 * j, bd + 2 * j, idesc, j);
+            f8_commit<PAIR>(&acc_full[h * 2 + buf]);
+            f8_commit<PAIR>(&empty[s]);
+            if (++s == C::ST) { s = 0; ph ^= 1u; }
           }
         }
-        tc_commit2(mma_done);                                                  // nothing is in flight when tensor memory is freed
+        f8_commit<PAIR>(mma_done);                                                  // nothing is in flight when tensor memory is freed
       }
     }
   } else {
@@ -178,10 +208,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
     // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has rows [32 q, 32 q + 32) of half h, a row a lane
     const int h = warp >> 2, q = warp & 3, row = 32 * q + lane;
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + h * 128;
-    const uint32_t empty0 = mapa_u32(smem_u32(&acc_empty[h * 2]), 0);
+    const uint32_t empty0 = PAIR ? mapa_u32(smem_u32(&acc_empty[h * 2]), 0) : 0u;
     uint32_t it = 0;
     bool ok = true;
-    while (ok && sch.next(item, kb0, kb1)) {
+    while (sch.next(item, kb0, kb1)) {                                          // after a wait that gave up: on to the end without waits and results, but through every barrier
       const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
       const TileRef tl = tile_of(ti);
       const int rows = min(max(tl.rows - 128 * (int)rank, 0), 128);            // of this CTA
@@ -216,7 +246,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         tc_fence_after();
         return (bool)__all_sync(0xffffffffu, o);
       };
-      if ((ok = arrived(it)) && active) { tc_ld32(trow + (it & 1u) * 256, ra); tc_ld32(trow + (it & 1u) * 256 + 32, rb); }
+      if ((ok = ok && arrived(it)) && active) { tc_ld32(trow + (it & 1u) * 256, ra); tc_ld32(trow + (it & 1u) * 256 + 32, rb); }
       for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
         const uint32_t buf = it & 1u, tb = trow + buf * 256;
         const float f0 = x[0] * s0[0], f1 = MODE == F8_GU ? x[0] * s1[0] : f0;
@@ -233,7 +263,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(empty0 + buf * 8);                  // the buffer's sums are in registers
+        if (lane == 0) {                                                       // the buffer's sums are in registers
+          if constexpr (PAIR) mbar_arrive_cluster(empty0 + buf * 8);
+          else mbar_arrive(&acc_empty[h * 2 + buf]);
+        }
         if (active) f8_add<32>(acc + 64, ra, f1);
         const bool more = kb + 1 < kb1 && (ok = arrived(it + 1)) && active;
         const uint32_t nb = trow + (buf ^ 1u) * 256;
@@ -242,20 +275,20 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         if (more) tc_ld32(nb + 32, rb);
       }
       // ---- an item that other pairs have parts of: leave the sums, the last one to arrive goes on with everybody's
-      if (!(ok = named_bar_and(1, 256, ok))) break;
       if (kb1 - kb0 < KB) {
         const uint32_t st0 = (uint32_t)item * (uint32_t)KB, c_first = sch.owner(st0), c_last = sch.owner(st0 + KB - 1);
         // a part: [column][half][row]; a pair's first run is its part 0
-        auto part_of = [&](uint32_t c, uint32_t st) { return a.part + ((size_t)(2 * c + rank) * 2 + (c == c_first && st != st0 ? 1 : 0)) * (256 * 128) + h * 128 + row; };
+        auto part_of = [&](uint32_t c, uint32_t st) { return a.part + ((size_t)(C::CTAS * c + rank) * 2 + (c == c_first && st != st0 ? 1 : 0)) * (256 * 128) + h * 128 + row; };
         float* mine = part_of(sch.me, sch.start(sch.me));
         if (active) {
 #pragma unroll
           for (int c = 0; c < 128; ++c) __stcg(mine + c * 256, acc[c]);
         }
         named_bar_sync(1, 256);
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && !ok) *last = 0u;
+        else if (threadIdx.x == 0) {
           __threadfence();                                                     // everybody's sums are out before this CTA is counted
-          unsigned int* count = a.count + 2 * item + rank;
+          unsigned int* count = a.count + C::CTAS * item + rank;
           const bool all = atomicAdd(count, 1u) == c_last - c_first;
           if (all) *count = 0u;                                                // zero again for the next launch
           __threadfence();
@@ -271,7 +304,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         const float* rest = part_of(c_first, st0);                             // the later pairs' parts are their first ones
         if (active) {
           for (uint32_t cc = c_first; cc <= c_last; ++cc) {
-            const float* p = cc == c_first ? first : rest + (size_t)(cc - c_first) * (4 * 256 * 128);
+            const float* p = cc == c_first ? first : rest + (size_t)(cc - c_first) * (C::CTAS * 2 * 256 * 128);
 #pragma unroll
             for (int g = 0; g < 128; g += 64) {
               float t[64];
@@ -292,9 +325,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
         }
         amx[h * 128 + row] = mx;
         named_bar_sync(1, 256);
-        F8Block blk;
+        F8BlockFast blk;
         const float sc = blk.init(max(amx[row], amx[128 + row]));
-        if (valid) {
+        if (valid && ok) {
           uint8_t* to = a.yq + (slot0 + row) * a.N + nt * 128 + h * 64;
 #pragma unroll
           for (int c = 0; c < 64; c += 16) {
@@ -306,8 +339,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
           if (h == 0) a.ys[(size_t)nt * a.ldys + slot0 + row] = sc;
         }
         named_bar_sync(1, 256);                                                // the magnitudes have been read
-      } else if (active) {
-        uint8_t* stg = sm + F8P_ST * F8P_STAGE + (size_t)warp * F8_STG_BYTES;
+      } else if (active && ok) {
+        uint8_t* stg = sm + C::ST * C::STAGE + (size_t)warp * F8_STG_BYTES;
         const int nrow = min(32, rows - 32 * q), n0 = nt * 256 + h * 128;
         const size_t row0 = slot0 + 32 * q;
         if (MODE == F8_DOWN || a.yb) {
@@ -332,8 +365,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_pair_kernel(const __grid_co
   if (warp == F8_W_TMA) mbar_wait(mma_done, 0, a.err, 0x800u);                 // in both CTAs: the last MMA has retired, and so has the announcement of it
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
-  if (warp == F8_W_MMA) { tc_fence_after(); tmem_dealloc2(tmem, 512); }
+  if constexpr (PAIR) cluster_sync_all();
+  if (warp == F8_W_MMA) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc2(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
 }
 
 }  // namespace hb

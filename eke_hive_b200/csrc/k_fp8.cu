@@ -11,62 +11,70 @@ struct F8RowsArgs {
   const int* dest; int nd;                             // [M, nd], negative: none; nd == 0: no destinations
   uint8_t* q; int ldq; float* s; int lds;
 };
-// Block b of row m; slot: of lane l16 < nd's pair, or -1.
+// Block b of row m by LN lanes, 128 / LN values each; slot: of lane l < nd's pair, or -1.
+template <int LN>
 __device__ __forceinline__ void f8_quant_unit(const F8RowsArgs& a, int m, int b, int slot) {
-  const int l16 = threadIdx.x & 15, k = b * F8_B + l16 * 8, sh = threadIdx.x & 16;
-  const uint32_t half = 0xffffu << sh;
-  float v[8];
+  constexpr int V = F8_B / LN;
+  const int l = threadIdx.x & (LN - 1), k = b * F8_B + l * V, sh = threadIdx.x & (32 - LN);
+  const uint32_t group = (uint32_t)((1ull << LN) - 1ull) << sh;
+  float v[V];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  if (k < a.K) {                                                               // K is a multiple of 16: eight values are inside or outside together
+  for (int j = 0; j < V; ++j) v[j] = 0.f;
+  if (k < a.K) {                                                               // K is a multiple of 16: a lane's values are inside or outside together
     const __nv_bfloat16* p = a.x + (size_t)m * a.ldx + k;
     if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(ww[j] << 16); v[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
+      for (int i = 0; i < V / 8; ++i) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[8 * i + 2 * j] = __uint_as_float(ww[j] << 16); v[8 * i + 2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u); }
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __bfloat162float(p[j]);
+      for (int j = 0; j < V; ++j) v[j] = __bfloat162float(p[j]);
     }
   }
   uint32_t mx = 0u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) mx = max(mx, f8_mag(v[j]));
+  for (int j = 0; j < V; ++j) mx = max(mx, f8_mag(v[j]));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(half, mx, o));
+  for (int o = LN / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(group, mx, o));
   F8Block blk;
   const float sc = blk.init(mx);
-  const uint2 c = make_uint2(blk.pair(v[0], v[1]) | blk.pair(v[2], v[3]) << 16, blk.pair(v[4], v[5]) | blk.pair(v[6], v[7]) << 16);
+  uint32_t c[V / 4];
+#pragma unroll
+  for (int j = 0; j < V / 4; ++j) c[j] = blk.pair(v[4 * j], v[4 * j + 1]) | blk.pair(v[4 * j + 2], v[4 * j + 3]) << 16;
+  auto put = [&](int to) {
+    if (k >= a.K) return;
+    uint8_t* d = a.q + (size_t)to * a.ldq + k;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(d) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<uint4*>(d) = make_uint4(c[0], c[1], c[2], c[3]);
+  };
   if (a.nd == 0) {
-    if (k < a.K) *reinterpret_cast<uint2*>(a.q + (size_t)m * a.ldq + k) = c;
-    if (l16 == 0) a.s[(size_t)b * a.lds + m] = sc;
+    put(m);
+    if (l == 0) a.s[(size_t)b * a.lds + m] = sc;
     return;
   }
   if (slot >= 0) a.s[(size_t)b * a.lds + slot] = sc;
-  for (uint32_t on = __ballot_sync(half, slot >= 0) >> sh & 0xffffu; on; on &= on - 1u) {
-    const int to = __shfl_sync(half, slot, (__ffs(on) - 1) + sh);
-    if (k < a.K) *reinterpret_cast<uint2*>(a.q + (size_t)to * a.ldq + k) = c;
-  }
+  for (uint32_t on = (__ballot_sync(group, slot >= 0) >> sh) & (uint32_t)((1ull << LN) - 1ull); on; on &= on - 1u) put(__shfl_sync(group, slot, (__ffs(on) - 1) + sh));
 }
-// CTA `cta` of `ctas`: every ctas-th run of 16 blocks
-__device__ __forceinline__ void f8_quant_rows(const F8RowsArgs& a, int cta, int ctas) {
-  const int nb = f8_blocks(a.K), l16 = threadIdx.x & 15;
-  const uint32_t half = 0xffffu << (threadIdx.x & 16);
-  const long long total = (long long)a.M * nb;
-  for (long long i = (long long)cta * 16 + (threadIdx.x >> 4); i < total; i += (long long)ctas * 16) {
-    const int m = (int)(i / nb), b = (int)(i - (long long)m * nb);
-    if (a.nd == 0) { f8_quant_unit(a, m, b, -1); continue; }
-    for (int d = 0; d < a.nd; d += 16) {                                       // (more than 16 destinations: once more)
-      const int slot = d + l16 < a.nd ? __ldg(a.dest + (size_t)m * a.nd + d + l16) : -1;
-      if (__any_sync(half, slot >= 0)) f8_quant_unit(a, m, b, slot);           // a row nobody here wants is not read
-    }
-  }
-}
+// Eight lanes a block: what a lane does once for a block (the reciprocal, the scale) is some 40 instructions beside five a value, and their number is what
+// bounds the kernel (4096 rows of 5120: 28 us with sixteen lanes a block and nine instructions a value).
 __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const F8RowsArgs a) {
   griddep_wait();
   griddep_launch();
-  f8_quant_rows(a, blockIdx.x, gridDim.x);
+  const int nb = f8_blocks(a.K), l = threadIdx.x & 7;
+  const uint32_t group = 0xffu << (threadIdx.x & 24);
+  const long long total = (long long)a.M * nb;
+  for (long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); i < total; i += (long long)gridDim.x * 32) {
+    const int m = (int)(i / nb), b = (int)(i - (long long)m * nb);
+    if (a.nd == 0) { f8_quant_unit<8>(a, m, b, -1); continue; }
+    for (int d = 0; d < a.nd; d += 8) {                                        // (more than eight destinations: once more)
+      const int slot = d + l < a.nd ? __ldg(a.dest + (size_t)m * a.nd + d + l) : -1;
+      if (__any_sync(group, slot >= 0)) f8_quant_unit<8>(a, m, b, slot);       // a row nobody here wants is not read
+    }
+  }
 }
 
 // The front of a routed layer's call with a short list of pairs, in one launch: CTA 0 writes the plan down (the slots for the sum at the end, the tiles for the down
@@ -97,7 +105,7 @@ __global__ void __launch_bounds__(256) fp8_prep_kernel(const F8PrepArgs a) {
     const int m = u / nb;
     for (int d = 0; d < nd; d += 16) {
       const int slot = d + l16 < nd ? slots[(m - m0) * nd + d + l16] : -1;
-      if (__any_sync(0xffffu << (t & 16), slot >= 0)) f8_quant_unit(a.rows, m, u - m * nb, slot);
+      if (__any_sync(0xffffu << (t & 16), slot >= 0)) f8_quant_unit<16>(a.rows, m, u - m * nb, slot);
     }
   }
 }
@@ -211,14 +219,15 @@ using namespace hb;
 namespace {
 using F8Kernel = void (*)(const F8Args, const CUtensorMap, const CUtensorMap);
 struct F8Pick { F8Kernel fn; int smem; };
-// rows: of a tile, at most (16, 32, 64: one CTA's tile; 256: a pair's)
+// rows: of a tile, at most (256: a pair's)
 template <int MODE>
 F8Pick f8_kernel(int rows) {
   switch (rows) {
     case 16: return {fp8_gemm_kernel<16, MODE>, F8Cfg<16>::SMEM};
     case 32: return {fp8_gemm_kernel<32, MODE>, F8Cfg<32>::SMEM};
-    case 64: return {fp8_gemm_kernel<64, MODE>, F8Cfg<64>::SMEM};
-    default: return {fp8_pair_kernel<MODE>, F8P_SMEM};
+    case 64: return {fp8_gemm_kernel<64, F8_PLAIN>, F8Cfg<64>::SMEM};
+    case F8S_ROWS: return {fp8_many_kernel<MODE, false>, F8PCfg<false>::SMEM};
+    default: return {fp8_many_kernel<F8_PLAIN, true>, F8PCfg<true>::SMEM};
   }
 }
 template <int MODE>
@@ -230,10 +239,15 @@ int f8_launch(hb_ctx* ctx, const char* name, int rows, const F8Args& a, const CU
   return hb_launch_cluster(ctx, name, true, rows == F8P_ROWS ? 2 : 1, k.fn, dim3(n), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
 }
 size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows > 64 ? 128 : rows) * 4; }
-// rows of a tile for a product of M rows
-int f8_rows_for(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : F8P_ROWS; }
-// pairs of a tile by what an expert gets on average: runs that are longer are cut into tiles, which read the expert's weights again
-int f8_rows_for_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 16ll * E ? 32 : P <= 48ll * E ? 64 : F8P_ROWS; }
+// Rows of a tile for a product of M rows and n_nt items a tile.  Up to 32 rows a weight row a lane (17408 x 5120, 32 rows: 24 us; a row of x a lane: 28); up to 64
+// the same where an item is cut three times and more (5120 x 17408, 64 rows: 33 us against 46, whose parts are four times the size), else and up to 128 a
+// row of x a lane (37888 x 4096, 64 rows: 31 against 34); more: a pair's tile (18944 x 4096, 512 rows: 45 against 51).
+int f8_rows_for(const hb_ctx* ctx, int M, int n_nt) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 && 3 * n_nt <= ctx->sm_count ? 64 : M <= 128 ? F8S_ROWS : F8P_ROWS; }
+// Pairs of a tile by what an expert gets on average: longer runs are cut into tiles, which read the expert's weights again, and a tile that is not full
+// wastes its MMAs.  Gate/up + down of 512 experts of 2048 / 512: 20 pairs an expert 310 us with 32, 359 with 128 (39 pairs: 476, 375; 10 pairs: 294, and 293
+// with 16).  A pair of CTAs gains nothing here: 32 experts of 7168 / 2048, 256 pairs an expert, 533 us with 128, 661 with 256, half of whose second tiles are
+// empty; 8 experts of 4096 / 1536, 2048 pairs: 399, 439.
+int f8_rows_for_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 24ll * E ? 32 : F8S_ROWS; }
 // map of a byte matrix [n_rows][row_bytes], rows ld bytes apart, in boxes of 128 bytes × box_rows under the 128-byte swizzle; bytes and rows past the
 // end read as zero codes
 int f8_map(hb_ctx* ctx, CUtensorMap* m, const void* base, size_t row_bytes, size_t ld, size_t n_rows, int box_rows) {
@@ -268,14 +282,14 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
 }
 unsigned int* f8_counters(hb_ctx* ctx) { return reinterpret_cast<unsigned int*>(ctx->dev_err) + kErrCounters; }
 int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
-  const long long units = (long long)a.M * f8_blocks(a.K), ctas = (units + 15) / 16, cap = (long long)ctx->sm_count * 32;
+  const long long units = (long long)a.M * f8_blocks(a.K), ctas = (units + 31) / 32, cap = (long long)ctx->sm_count * 32;
   return hb_launch(ctx, "fp8_quant_rows", true, fp8_quant_rows_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(256), 0, st, a);
 }
 }  // namespace
 
 int hbk_fp8_setup(hb_ctx* ctx) {
-  for (int bn : {16, 32, 64, F8P_ROWS})
-    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {
+  for (int bn : {16, 32, 64, F8S_ROWS, F8P_ROWS})
+    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {   // (64 and 256: the dense product alone)
       cudaFuncAttributes at;
       HB_CUDA(ctx, cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(k.fn)));
       // a warp that asks for more registers than the block was launched with would wait for good
@@ -311,7 +325,7 @@ int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t*
   return hb_launch(ctx, "fp8_quantize", false, fp8_quantize_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float*>(w), N, K, q, s);
 }
 
-size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(f8_rows_for(M)) : 0; }
+size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M <= 16 ? 16 : M <= 32 ? 32 : F8P_ROWS) : 0; }
 
 int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb, float* yf, int ldy, void* ws, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
@@ -324,16 +338,16 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "fp8_gemm: ws NULL or not 256-byte aligned");
-  const int rows = f8_rows_for(M), nt = (M + rows - 1) / rows;
+  const int rows = f8_rows_for(ctx, M, (W->N + 255) / 256), nt = (M + rows - 1) / rows;
   F8Args a{};
-  a.M = M; a.per = ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
+  a.M = M; a.per = rows == F8P_ROWS ? rows : ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
   HB_REQUIRE(ctx, (long long)nt * a.n_nt < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d", M, W->N);
   a.ws = reinterpret_cast<const float*>(W->s); a.xs = xs; a.lds = lds;
   a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.count = f8_counters(ctx); a.err = ctx->dev_err;
   CUtensorMap tw, tx;
-  const bool pair = rows == F8P_ROWS;
+  const bool many = rows >= F8S_ROWS;
   int r;
-  if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, pair ? 64 : 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, pair ? 128 : rows))) return r;
+  if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, many ? 64 : 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, many ? 128 : rows))) return r;
   return f8_launch<F8_PLAIN>(ctx, "fp8_gemm", rows, a, tw, tx, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -366,17 +380,17 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   const uint8_t* const* tab = rec_tab + (size_t)li * E;
   F8Ws W;
   f8_carve(ws, M, K, E, H, I, &W);
-  const int P = M * K, rows = f8_rows_for_pairs(P, E), box = rows == F8P_ROWS ? 128 : rows;
+  const int P = M * K, rows = f8_rows_for_pairs(P, E), box = rows < 128 ? rows : 128;
   int r;
   // maps of a record's matrices (gate and up lie one behind the other), to be given their addresses on the device; of the rows of x and y
   CUtensorMap tg, td, tx, ty;
-  const int wbox = rows == F8P_ROWS ? 64 : 128;
+  const int wbox = rows >= F8S_ROWS ? 64 : 128;
   if ((r = f8_map(ctx, &tg, W.xq, H, H, 2 * I, wbox)) || (r = f8_map(ctx, &td, W.xq, I, I, H, wbox))) return r;
   if ((r = f8_map(ctx, &tx, W.xq, H, H, P, box)) || (r = f8_map(ctx, &ty, W.yq, I, I, P, box))) return r;
   F8PrepArgs pr{};
   F8RowsArgs& q = pr.rows;
   q.x = reinterpret_cast<const __nv_bfloat16*>(x); q.ldx = H; q.M = M; q.K = H; q.dest = W.pos_of; q.nd = K; q.q = W.xq; q.ldq = H; q.s = W.xs; q.lds = P;
-  const bool own_plan = P <= F8_PLAN_PAIRS && rows != F8P_ROWS;
+  const bool own_plan = P <= F8_PLAN_PAIRS && rows < F8S_ROWS;
   if (own_plan) {
     pr.plan = F8Plan{ids, P, E, rows, tab}; pr.pos_of = W.pos_of; pr.tiles = W.tiles; pr.n_tiles = W.n_tiles;
     if ((r = hb_launch(ctx, "fp8_prep", true, fp8_prep_kernel, dim3(1 + (unsigned)((M * f8_blocks(H) + 15) / 16)), dim3(256), 0, st, pr))) return r;
