@@ -20,9 +20,15 @@ __all__ = ["Context", "context", "ExpertRecLayout", "nvfp4_dequant", "nvfp4_gemv
            "moe_decode_supported", "GMat", "dense_gemv", "dense_gemv_gu", "dense_gemv_ws_bytes", "lb_dequant", "dispatch_plan", "moe_layer", "moe_layer_ws_bytes", "PeerExchange", "moe_decode_ep_local", "moe_prefill_supported", "moe_prefill_ws_bytes", "fn_moe_prefill", "nvfp4_gemm_a4", "fp4_peak_probe", "fp8_quant_rows", "fp8_quantize", "fp8_gemm_ws_bytes", "fp8_gemm", "Fp8RecLayout", "fp8_record", "moe_fp8_ws_bytes", "moe_fp8", "FMT_NVFP4", "FMT_LB3_G64", "FMT_LB2_G64", "FMT_FP8_B128", "expert_dequant", "csf_decode", "record_pack", "record_pack_ws_bytes", "record_jobs", "record_pack_batch", "CSF_OK", "CSF_EXC_INDEX", "CSF_EXC_DELTA", "CSF_EXC_VALUE", "CSF_CODE", "gather_rows", "swiglu_rows", "scatter_add_rows", "add_f32", "make_pairs", "rec_table", "HbError"]
 
 
+_lib_handle = None
+
+
 def _L():
-    from . import lib
-    return lib
+    global _lib_handle
+    if _lib_handle is None:
+        from . import lib
+        _lib_handle = lib
+    return _lib_handle
 
 
 def _p(t):
@@ -39,12 +45,35 @@ def _stream(device: int | None = None):
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
 
 
+try:
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_cuda     # what compiled graphs allocate with: a third of torch.empty's time
+except ImportError:
+    def _empty_cuda(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+def _empty(rows: int, cols: int, dtype):
+    return _empty_cuda((rows, cols), (cols, 1), dtype)                         # on the current device
+
+
+def _bytes(n: int):
+    return _empty_cuda((n,), (1,), torch.uint8)
+
+
 def _here(t: torch.Tensor, ctx: "Context | None"):
     """(context, stream handle) of a call on tensor t: t, the context and the current device have to be the same device."""
     d = torch.cuda.current_device()
-    if t.device.index != d or (ctx is not None and ctx.device != d):
+    if t.get_device() != d or (ctx is not None and ctx.device != d):
         raise HbError(-1, f"tensor on {t.device}, context on cuda:{d if ctx is None else ctx.device}, current device cuda:{d}: they have to be the same")
-    return ctx or context(d), torch._C._cuda_getCurrentRawStream(d)
+    return ctx or _CTX.get(d) or context(d), torch._C._cuda_getCurrentRawStream(d)
+
+
+def _row_ptr(t: torch.Tensor):
+    """(address, elements from row to row) of a matrix whose rows are contiguous."""
+    r, c = t.stride()
+    if c != 1 and t.shape[1] > 1:
+        raise HbError(-1, "rows must be contiguous")
+    return t.data_ptr(), max(r, t.shape[1]) if t.shape[0] <= 1 else r
 
 
 class Context:
@@ -212,10 +241,11 @@ def router_grouped_topk(logits: torch.Tensor, k: int, n_group: int = 1, topk_gro
     score + bias, weights from the score alone.  logits fp32 [M, ld]; returns ids int32 [M, k], w fp32 [M, k]."""
     ctx, st = _here(logits, ctx)
     M, cols = logits.shape
-    ids = logits.new_empty((M, k), dtype=torch.int32) if ids is None else ids
-    w = logits.new_empty((M, k)) if w is None else w
-    ctx.check(_L().hb_route_grouped_topk(ctx.handle, _p(logits), _rows(logits), M, cols if E is None else E, k, n_group, topk_group, group_top, _SCORE[score],
-                                         _p(bias), renorm, scale, _p(ids), _p(w), st))
+    ids = _empty(M, k, torch.int32) if ids is None else ids
+    w = _empty(M, k, torch.float32) if w is None else w
+    lp, ld = _row_ptr(logits)
+    ctx.check(_L().hb_route_grouped_topk(ctx.handle, lp, ld, M, cols if E is None else E, k, n_group, topk_group, group_top, _SCORE[score],
+                                         None if bias is None else bias.data_ptr(), renorm, scale, ids.data_ptr(), w.data_ptr(), st))
     return ids, w
 
 
@@ -403,19 +433,14 @@ def lb_dequant(W: GMat, out=None, ctx: Context | None = None):
 
 
 # ---------------------------------------------------------------------------------------------------- 8-bit floats, a scale per block of 128
-def _rows(t):
-    assert t.stride(-1) == 1, "rows must be contiguous"
-    return t.stride(0)
-
-
 def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     """hb_fp8_quant_rows: x bf16 [M, K] → (codes u8 [M, K], scales fp32 [ceil(K/128), M])."""
     ctx, st = _here(x, ctx)
     assert x.dtype == torch.bfloat16
     M, K = x.shape
-    q = x.new_empty((M, K), dtype=torch.uint8) if q is None else q
-    s = x.new_empty((-(-K // 128), M), dtype=torch.float32) if s is None else s
-    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, _p(x), _rows(x), M, K, _p(q), _rows(q), _p(s), _rows(s), st))
+    q = _empty(M, K, torch.uint8) if q is None else q
+    s = _empty(-(-K // 128), M, torch.float32) if s is None else s
+    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, *_row_ptr(x), M, K, *_row_ptr(q), *_row_ptr(s), st))
     return q, s
 
 
@@ -425,9 +450,10 @@ def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     bf16 = w.dtype == torch.bfloat16
     assert (bf16 or w.dtype == torch.float32) and w.is_contiguous()
     N, K = w.shape
-    q = w.new_empty((N, K), dtype=torch.uint8) if q is None else q
-    s = w.new_empty((-(-N // 128), -(-K // 128)), dtype=torch.float32) if s is None else s
-    ctx.check(_L().hb_fp8_quantize(ctx.handle, _p(w), bf16, N, K, _p(q), _p(s), st))
+    q = _empty(N, K, torch.uint8) if q is None else q
+    s = _empty(-(-N // 128), -(-K // 128), torch.float32) if s is None else s
+    assert q.is_contiguous() and s.is_contiguous()
+    ctx.check(_L().hb_fp8_quantize(ctx.handle, w.data_ptr(), bf16, N, K, q.data_ptr(), s.data_ptr(), st))
     return q, s
 
 
@@ -438,11 +464,13 @@ def fp8_gemm_ws_bytes(M: int, N: int, K: int) -> int:
 def fp8_gemm(W: GMat, xq, xs, out_dtype=torch.bfloat16, y=None, ws=None, ctx: Context | None = None):
     """hb_fp8_gemm: y [M, N] (bf16 or fp32) = rows quantised by fp8_quant_rows times the block-scaled matrix W (FMT_FP8_B128)."""
     ctx, st = _here(xq, ctx)
+    L = _L()
     M = xq.shape[0]
-    y = xs.new_empty((M, W.N), dtype=out_dtype) if y is None else y
-    ws = xq.new_empty(_L().hb_fp8_gemm_ws_bytes(M, W.N, W.K), dtype=torch.uint8) if ws is None else ws
-    yb, yf = (_p(y), None) if y.dtype == torch.bfloat16 else (None, _p(y))
-    ctx.check(_L().hb_fp8_gemm(ctx.handle, C.byref(W.c), _p(xq), _rows(xq), _p(xs), _rows(xs), M, yb, yf, _rows(y), _p(ws), st))
+    y = _empty(M, W.N, out_dtype) if y is None else y
+    ws = _bytes(L.hb_fp8_gemm_ws_bytes(M, W.N, W.K)) if ws is None else ws
+    yp, ldy = _row_ptr(y)
+    yb, yf = (yp, None) if y.dtype == torch.bfloat16 else (None, yp)
+    ctx.check(L.hb_fp8_gemm(ctx.handle, C.byref(W.c), *_row_ptr(xq), *_row_ptr(xs), M, yb, yf, ldy, ws.data_ptr(), st))
     return y
 
 
@@ -480,14 +508,18 @@ def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg
     """hb_moe_fp8: routed experts of FP8 records for any number of rows; ids int32 / w fp32 [M, K], x bf16 [M, H].  bf16 out adds the gated shared
     rows where given; out_dtype (or out.dtype) float32 gives the routed sum alone."""
     ctx, st = _here(x, ctx)
+    L = _L()
     M, K = ids.shape
-    assert x.is_contiguous() and ids.is_contiguous() and w.is_contiguous()
-    out = x.new_empty((M, H), dtype=out_dtype) if out is None else out
-    ws = x.new_empty(_L().hb_moe_fp8_ws_bytes(M, K, E, H, I), dtype=torch.uint8) if ws is None else ws
-    assert out.is_contiguous() and (shared is None or shared.is_contiguous())
-    assert out.dtype == torch.bfloat16 or (shared is None and lg is None), "shared rows are added to a bf16 output"
-    cmb = C.byref(PfCombine(_p(shared), _p(lg), 0 if lg is None else lg.stride(0), col, _p(out))) if out.dtype == torch.bfloat16 else None
-    ctx.check(_L().hb_moe_fp8(ctx.handle, _p(ids), _p(w), M, K, _p(rec_tab), li, E, _p(x), H, I, limit, None if cmb else _p(out), cmb, _p(ws), st))
+    out = _empty(M, H, out_dtype) if out is None else out
+    ws = _bytes(L.hb_moe_fp8_ws_bytes(M, K, E, H, I)) if ws is None else ws
+    assert x.is_contiguous() and ids.is_contiguous() and w.is_contiguous() and out.is_contiguous() and (shared is None or shared.is_contiguous())
+    op, cmb = out.data_ptr(), None
+    if out.dtype == torch.bfloat16:
+        cmb = C.byref(PfCombine(None if shared is None else shared.data_ptr(), _p(lg), 0 if lg is None else lg.stride(0), col, op))
+    else:
+        assert shared is None and lg is None, "shared rows are added to a bf16 output"
+    ctx.check(L.hb_moe_fp8(ctx.handle, ids.data_ptr(), w.data_ptr(), M, K, rec_tab.data_ptr(), li, E, x.data_ptr(), H, I, limit, None if cmb else op, cmb,
+                           ws.data_ptr(), st))
     return out
 
 
