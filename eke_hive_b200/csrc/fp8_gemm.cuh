@@ -9,8 +9,8 @@
 // a weight row, a column a row of x, so a call with few rows wastes no tensor-core columns, and what a thread ends up with is one output column
 // n for many rows m — in the gate/up pass gate and up of the same value.
 //
-// Work: items (tile of rows × 256 weight rows) of ceil(K / 128) steps.  Whole items go round the CTAs; what is left over, less than two rounds, is cut into
-// equal runs of steps, one a CTA, without regard to where an item ends.  A CTA that holds part of an item leaves its sums in the workspace; the last
+// Work: items (tile of rows × 256 weight rows) of ceil(K / 128) steps.  The list is cut into equal runs of steps, one a CTA, without regard to where an item
+// ends (in fp8_pair.cuh only what whole rounds of items over the CTAs leave over).  A CTA that holds part of an item leaves its sums in the workspace; the last
 // one to arrive (a counter an item) adds all parts in the order of the CTAs — the same order in every run — and finishes the item.  So a product
 // with one row of x keeps all SMs streaming weights to the end.  Nobody waits for anybody.
 //
@@ -19,6 +19,7 @@
 // of the columns, 4-7 the second) and end the items.  Two accumulator buffers: one fills while the other is read.  Every wait is bounded.
 #pragma once
 #include "fp8_common.cuh"
+#include "hb_kernels.h"
 #include "tc_common.cuh"
 
 namespace hb {
@@ -26,13 +27,12 @@ namespace hb {
 enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
 
 constexpr int F8_MAX_CTAS = 160;                       // grid at most; the workspace holds two partial items of each
-constexpr int F8_COUNTERS = 2 * F8_MAX_CTAS;           // items that are cut, at most
+constexpr int F8_COUNTERS = F8_MAX_CTAS;               // items that are cut, at most: a CTA's last one
 constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
 // Plan of a short list of pairs (at most F8_PLAN_PAIRS), worked out by every CTA that needs it for itself: a pair's slot is the number of pairs with a smaller
-// expert plus the number of earlier ones with its own, counted over the whole list in shared memory — no histogram, no meeting of CTAs, no launch of its own.
+// expert plus the number of earlier ones with its own: the same for every CTA, whatever the order its threads run in, without a launch of its own.
 constexpr int F8_PLAN_PAIRS = 1024;
 struct F8Plan { const int32_t* ids; int P, E, bm; const uint8_t* const* tab; };   // bm: pairs of a tile, at most
-struct F8At { int slot, rank, run, expert; };          // slot -1: the pair contributes nothing
 // ids with a record, the others NONE, to shared memory (room for P rounded up to four); the caller synchronises behind it
 __device__ __forceinline__ void f8_plan_load(const F8Plan& a, int* e_s, int threads) {
   for (int p = threadIdx.x; p < (a.P + 3) / 4 * 4; p += threads) {
@@ -40,22 +40,22 @@ __device__ __forceinline__ void f8_plan_load(const F8Plan& a, int* e_s, int thre
     e_s[p] = e >= 0 && e < a.E && __ldg(reinterpret_cast<const unsigned long long*>(a.tab) + e) != 0ull ? e : 0x7fffffff;
   }
 }
-__device__ __forceinline__ F8At f8_plan_at(const F8Plan& a, const int* e_s, int p) {
+// The slot of pair p, -1 if it contributes nothing.
+__device__ __forceinline__ int f8_plan_at(const F8Plan& a, const int* e_s, int p) {
   const int e = e_s[p];
-  int less = 0, before = 0, run = 0;
+  int n = 0;
 #pragma unroll 4
   for (int i = 0; i < (a.P + 3) / 4; ++i) {
     const int4 v = reinterpret_cast<const int4*>(e_s)[i];
-    less += (v.x < e) + (v.y < e) + (v.z < e) + (v.w < e);
-    const int c = (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
-    run += c;
-    before += 4 * i + 4 <= p ? c : (v.x == e && 4 * i < p) + (v.y == e && 4 * i + 1 < p) + (v.z == e && 4 * i + 2 < p);
+    n += (v.x < e) + (v.y < e) + (v.z < e) + (v.w < e);
+    if (4 * i + 4 <= p) n += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+    else n += (v.x == e && 4 * i < p) + (v.y == e && 4 * i + 1 < p) + (v.z == e && 4 * i + 2 < p);
   }
-  return e == 0x7fffffff ? F8At{-1, 0, 0, 0} : F8At{less + before, before, run, e};
+  return e == 0x7fffffff ? -1 : n;
 }
-// The tile list; tmp: 16-byte aligned room for 5 KB that may be written over.  A run of pairs is cut into tiles of equal size; a tile starts at every tper-th
-// pair of a run, and its number is that of the starts at smaller slots.  Returns the number of tiles; the caller synchronises before the list is read.
-// slots: where pair p's slot goes (or nullptr).
+// The tile list; tmp: 16-byte aligned room of F8_PLAN_TMP bytes that may be written over.  A run of pairs is cut into tiles of equal size.  Returns the number of
+// tiles; the caller synchronises before the list is read.  slots: where pair p's slot goes (or nullptr).
+constexpr int F8_PLAN_TMP = F8_PLAN_PAIRS * 8 + HB_MAX_EXPERTS * 4 + 256;
 __device__ __forceinline__ int f8_plan_tiles(const F8Plan& a, uint8_t* tmp, TileRef* tiles, int threads, int* slots = nullptr) {
   if (a.P <= 32) {                                     // a token or a few: one warp, a pair a lane (a kernel's code comes from afar the first time: the less, the sooner)
     uint32_t starts = 0u;
@@ -77,37 +77,49 @@ __device__ __forceinline__ int f8_plan_tiles(const F8Plan& a, uint8_t* tmp, Tile
     __syncthreads();
     return *reinterpret_cast<const int*>(tmp);
   }
-  int* e_s = reinterpret_cast<int*>(tmp);
-  uint32_t* flag = reinterpret_cast<uint32_t*>(e_s + F8_PLAN_PAIRS);
+  // Ranks by one warp that goes through the list 32 pairs at a time, counting as it goes; then the experts' starts by a scan over the counts.  (Counting for every
+  // pair over the whole list, as f8_plan_at does for a few, took 30 us of 640 pairs in every CTA.)
+  int *e_s = reinterpret_cast<int*>(tmp), *rank_s = e_s + F8_PLAN_PAIRS, *cnt = rank_s + F8_PLAN_PAIRS, *tot = cnt + HB_MAX_EXPERTS;
+  const int t = threadIdx.x, lane = t & 31, wp = t >> 5, nw = threads >> 5;
   f8_plan_load(a, e_s, threads);
-  for (int i = threadIdx.x; i < F8_PLAN_PAIRS / 32; i += threads) flag[i] = 0u;
+  for (int e = t; e < a.E; e += threads) cnt[e] = 0;
   __syncthreads();
-  auto first = [&](const F8At& at, int& rows) {
-    const int nt = (at.run + a.bm - 1) / a.bm, tper = (at.run + nt - 1) / nt;
-    rows = min(tper, at.run - at.rank);
-    return at.rank % tper == 0;
-  };
-  F8At mine{-1, 0, 0, 0};                              // of the thread's first pair: lists this short are the rule
-  for (int p = threadIdx.x; p < a.P; p += threads) {
-    const F8At at = f8_plan_at(a, e_s, p);
-    if (p == (int)threadIdx.x) mine = at;
-    if (slots) slots[p] = at.slot;
-    int rows;
-    if (at.slot >= 0 && first(at, rows)) atomicOr(&flag[at.slot >> 5], 1u << (at.slot & 31));
+  if (wp == 0) {
+    for (int p0 = 0; p0 < a.P; p0 += 32) {
+      const int e = p0 + lane < a.P ? e_s[p0 + lane] : 0x7fffffff;
+      const uint32_t same = __match_any_sync(0xffffffffu, e), front = same & ((1u << lane) - 1u);
+      const int base = e != 0x7fffffff ? cnt[e] : 0;
+      __syncwarp();
+      if (p0 + lane < a.P) rank_s[p0 + lane] = base + __popc(front);
+      if (e != 0x7fffffff && front == 0u) cnt[e] = base + __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < a.P; p += threads) {
-    const F8At at = p == (int)threadIdx.x ? mine : f8_plan_at(a, e_s, p);
-    int rows;
-    if (at.slot < 0 || !first(at, rows)) continue;
-    int n = __popc(flag[at.slot >> 5] & ((1u << (at.slot & 31)) - 1u));
-    for (int w = 0; w < at.slot >> 5; ++w) n += __popc(flag[w]);
-    tiles[n] = TileRef{at.slot, rows, at.expert};
+  // thread t: experts [t·per, (t + 1)·per)
+  const int per = (a.E + threads - 1) / threads, e0 = min(t * per, a.E), e1 = min(e0 + per, a.E);
+  int c = 0, n = 0;
+  for (int e = e0; e < e1; ++e) { c += cnt[e]; n += (cnt[e] + a.bm - 1) / a.bm; }
+  int ic = c, in = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int uc = __shfl_up_sync(0xffffffffu, ic, o), un = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) { ic += uc; in += un; }
   }
-  int n = 0;
-  for (int w = 0; w < (a.P + 31) / 32; ++w) n += __popc(flag[w]);
-  __syncthreads();                                     // tmp has been read
-  return n;
+  if (lane == 31) { tot[wp] = ic; tot[16 + wp] = in; }
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < nw; ++w) { if (w < wp) { ic += tot[w]; in += tot[16 + w]; } total += tot[16 + w]; }
+  int run0 = ic - c, tile = in - n;
+  for (int e = e0; e < e1; ++e) {
+    const int run = cnt[e], nt = (run + a.bm - 1) / a.bm, tper = nt > 0 ? (run + nt - 1) / nt : 0;
+    for (int i = 0; i < nt; ++i) tiles[tile++] = TileRef{run0 + i * tper, min(tper, run - i * tper), e};
+    cnt[e] = run0;                                     // from here on the run's first slot
+    run0 += run;
+  }
+  __syncthreads();
+  if (slots) for (int p = t; p < a.P; p += threads) slots[p] = e_s[p] != 0x7fffffff ? cnt[e_s[p]] + rank_s[p] : -1;
+  return total;
 }
 
 constexpr int F8_STG_PITCH = 80, F8_STG_BYTES = 32 * F8_STG_PITCH;   // a warp's staging: 32 rows of 64 bytes (pitch: 16-byte accesses without bank conflicts)
@@ -139,7 +151,7 @@ struct F8Args {
   float limit;
   __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN
   uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
-  float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256], arrivals (zero before and after)
+  float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256]; arrivals, by the CTA of an item's first step (zero before and after)
   uint32_t* err;
 };
 
@@ -162,13 +174,15 @@ struct F8Maps {
 };
 
 // The steps of a CTA, the same for all its warps: segments (item, first step, end).
-struct F8Sched {                                       // (32 bits: at most 320 cut items of at most 2^16 steps, times 160 CTAs)
+struct F8Sched {                                       // (32 bits: at most 320 items of at most 2^16 steps, or 2^24 steps, times 160 CTAs)
   uint32_t KB, G, me, dp, sk, U, Gs, u, u1, i;
-  // even: with fewer items than CTAs cut every one into the same number of runs and leave CTAs without work
-  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool even) {
+  // runs: no rounds, the whole list in equal runs (as long as its steps can be counted so): a CTA stays with an expert.  Else, even: with fewer items than CTAs
+  // cut every one into the same number of runs and leave CTAs without work
+  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool runs, bool even) {
     KB = KB_; G = G_; me = me_;
     const uint32_t waves = items / G, rem = items - waves * G;
-    dp = rem == 0u ? waves : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
+    const bool all = runs && (unsigned long long)items * KB < (1ull << 24);
+    dp = all ? 0u : rem == 0u ? waves : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
     sk = items - dp * G;
     U = sk * KB;
     Gs = min(even && waves == 0u && items > 0u ? G / items * items : G, max(U, 1u));   // CTAs that get a run of steps: none is empty
@@ -316,7 +330,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   const int KB = f8_blocks(a.K);
   if (!own_plan) n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, false);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, true, false);
   auto tile_of = [&](int ti) -> TileRef {
     if (own_plan) return tile_s[ti];
     if (MODE != F8_PLAIN) return a.tiles[ti];
@@ -512,8 +526,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         if (threadIdx.x == 0 && !ok) *last = 0u;
         else if (threadIdx.x == 0) {
           __threadfence();                                                     // everybody's sums are out before this CTA is counted
-          const bool all = atomicAdd(a.count + item, 1u) == c_last - c_first;
-          if (all) a.count[item] = 0u;                                         // zero again for the next launch
+          const bool all = atomicAdd(a.count + c_first, 1u) == c_last - c_first;
+          if (all) a.count[c_first] = 0u;                                         // zero again for the next launch
           __threadfence();
           *last = all;
         }

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
   // before griddep_wait: as in fp8_gemm.cuh (the tiles come from the kernel in front of the one in front)
   const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / C::CTAS, blockIdx.x / C::CTAS, true);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / C::CTAS, blockIdx.x / C::CTAS, false, true);
   auto tile_of = [&](int ti) -> TileRef {
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         if (threadIdx.x == 0 && !ok) *last = 0u;
         else if (threadIdx.x == 0) {
           __threadfence();                                                     // everybody's sums are out before this CTA is counted
-          unsigned int* count = a.count + C::CTAS * item + rank;
+          unsigned int* count = a.count + C::CTAS * c_first + rank;
           const bool all = atomicAdd(count, 1u) == c_last - c_first;
           if (all) *count = 0u;                                                // zero again for the next launch
           __threadfence();

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const F8RowsArgs a)
 // one-row call's 75 us.)
 struct F8PrepArgs { F8RowsArgs rows; F8Plan plan; int* pos_of; TileRef* tiles; int* n_tiles; };
 __global__ void __launch_bounds__(256) fp8_prep_kernel(const F8PrepArgs a) {
-  __shared__ __align__(16) uint8_t tmp[F8_PLAN_PAIRS * 4 + F8_PLAN_PAIRS / 8];
+  __shared__ __align__(16) uint8_t tmp[F8_PLAN_TMP];
   __shared__ int slots[512];
   const int t = threadIdx.x;
   griddep_wait();
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) fp8_prep_kernel(const F8PrepArgs a) {
   __syncthreads();
   const int nb = f8_blocks(a.rows.K), u0 = (blockIdx.x - 1) * 16, total = a.rows.M * nb, nd = a.rows.nd;
   const int m0 = u0 / nb, m1 = min(u0 + 15, total - 1) / nb;
-  for (int i = t; i < (m1 - m0 + 1) * nd; i += 256) slots[i] = f8_plan_at(a.plan, e_s, m0 * nd + i).slot;
+  for (int i = t; i < (m1 - m0 + 1) * nd; i += 256) slots[i] = f8_plan_at(a.plan, e_s, m0 * nd + i);
   __syncthreads();
   const int u = u0 + (t >> 4), l16 = t & 15;
   if (u < total) {
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
 }
 
 // ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)], k in order (+ gate·shared[m]) ----------------------------------
-// A warp takes 256 columns of a row, a lane eight of them (16 bytes of every pair's part).  Lane k looks up pair k; only pairs that have a slot are gone
+// A warp takes 512 columns of a row, a lane twice eight of them (16 bytes of every pair's part).  Lane k looks up pair k; only pairs that have a slot are gone
 // through, four parts fetched at a time.
 constexpr int F8_SUM_THREADS = 128;
 struct F8SumArgs {
@@ -166,49 +166,54 @@ struct F8SumArgs {
 };
 __global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs a) {
   bool waited = false;                                                         // only the parts are of the kernel in front
-  const int chunks = (a.H + 255) / 256, lane = threadIdx.x & 31;
+  const int chunks = (a.H + 511) / 512, lane = threadIdx.x & 31;
   const long long total = (long long)a.M * chunks;
   constexpr int WARPS = F8_SUM_THREADS / 32;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   for (long long i = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); i < total; i += (long long)gridDim.x * WARPS) {
-    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 256 + lane * 8;
-    const bool in = n < a.H;                                                   // H is a multiple of 128
+    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 512 + lane * 8;
+    const bool in[2] = {n < a.H, n + 256 < a.H};                               // H is a multiple of 128
     const size_t o = (size_t)m * a.H + n;
     const int slot = lane < a.K ? __ldg(a.pos_of + (size_t)m * a.K + lane) : -1;
-    const float wk = slot >= 0 ? __ldg(a.w + (size_t)m * a.K + lane) : 0.f;
-    const uint4 sv = a.shared && in ? __ldg(reinterpret_cast<const uint4*>(a.shared + o)) : make_uint4(0u, 0u, 0u, 0u);
+    const float wk = lane < a.K ? __ldg(a.w + (size_t)m * a.K + lane) : 0.f;
+    uint4 sv[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sv[h] = a.shared && in[h] ? __ldg(reinterpret_cast<const uint4*>(a.shared + o + 256 * h)) : zero;
     const float gate = a.lg ? 1.f / (1.f + expf(-__ldg(a.lg + (size_t)m * a.ld + a.col))) : 1.f;
     if (!waited) { griddep_wait(); waited = true; }
-    float acc[8];
+    float acc[2][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    auto add = [&](const uint4& v, float f) {
+    for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
+    auto add = [&](float (&to)[8], const uint4& v, float f) {
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { acc[2 * j] = fmaf(f, __uint_as_float(u[j] << 16), acc[2 * j]); acc[2 * j + 1] = fmaf(f, __uint_as_float(u[j] & 0xffff0000u), acc[2 * j + 1]); }
+      for (int j = 0; j < 4; ++j) { to[2 * j] = fmaf(f, __uint_as_float(u[j] << 16), to[2 * j]); to[2 * j + 1] = fmaf(f, __uint_as_float(u[j] & 0xffff0000u), to[2 * j + 1]); }
     };
     for (uint32_t on = __ballot_sync(0xffffffffu, slot >= 0); on;) {
-      uint4 v[4]; float f[4];
+      uint4 v[4][2]; float f[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int k = on ? __ffs(on) - 1 : 0;
-        const int sl = __shfl_sync(0xffffffffu, slot, k);
-        f[j] = __shfl_sync(0xffffffffu, wk, k);
-        v[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (!on) f[j] = 0.f;
-        else if (in) v[j] = __ldcs(reinterpret_cast<const uint4*>(a.part + (size_t)sl * a.H + n));
+        const __nv_bfloat16* p = a.part + (size_t)__shfl_sync(0xffffffffu, slot, k) * a.H + n;
+        f[j] = on ? __shfl_sync(0xffffffffu, wk, k) : 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[j][h] = on && in[h] ? __ldcs(reinterpret_cast<const uint4*>(p + 256 * h)) : zero;
         on &= on - 1u;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add(v[j], f[j]);
+      for (int j = 0; j < 4; ++j) { add(acc[0], v[j][0], f[j]); add(acc[1], v[j][1], f[j]); }
     }
-    if (!in) continue;
-    if (!a.cout) {
-      *reinterpret_cast<float4*>(a.out + o) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      *reinterpret_cast<float4*>(a.out + o + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!in[h]) continue;
+      if (!a.cout) {
+        *reinterpret_cast<float4*>(a.out + o + 256 * h) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+        *reinterpret_cast<float4*>(a.out + o + 256 * h + 4) = make_float4(acc[h][4], acc[h][5], acc[h][6], acc[h][7]);
+      } else {
+        if (a.shared) add(acc[h], sv[h], gate);
+        *reinterpret_cast<uint4*>(a.cout + o + 256 * h) = f8_pack8(acc[h]);
+      }
     }
-    if (a.shared) add(sv, gate);
-    *reinterpret_cast<uint4*>(a.cout + o) = f8_pack8(acc);
   }
 }
 
@@ -412,7 +417,7 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
     su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
     if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
   }
-  const long long sums = ((long long)M * ((H + 255) / 256) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
+  const long long sums = ((long long)M * ((H + 511) / 512) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
   return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(sums < cap ? sums : cap)), dim3(F8_SUM_THREADS), 0, st, su);
 }
 
