@@ -21,6 +21,12 @@ struct RouteGroupedArgs {
   const float* logits; int ld, M, E, k, n_group, topk_group, group_top, sigmoid, renorm; const float* bias; float scale; int32_t* ids; float* w;
 };
 
+// A bias in the range of finite values, NaN the lowest: no sum of two is NaN, whose order would be nobody's.
+__device__ __forceinline__ float rg_bias(const RouteGroupedArgs& a, int e) {
+  constexpr float top = 3.402823466e38f;
+  return a.bias ? fminf(fmaxf(__ldg(a.bias + e), -top), top) : 0.f;
+}
+
 // a before b: the larger value, the smaller index among equals
 __device__ __forceinline__ bool rg_before(double a, int ia, double b, int ib) { return a > b || (a == b && ia < ib); }
 
@@ -39,7 +45,7 @@ __device__ __noinline__ void route_grouped_row64(const RouteGroupedArgs& a, cons
     return mx == -INFINITY ? 0.0 : exp(logit(e) - mx) / sum;                     // a row without a finite logit: all scores 0
   };
   for (int e = lane; e < a.E; e += 32) {
-    const double v = score(e) + (a.bias ? (double)a.bias[e] : 0.0);
+    const double v = score(e) + (double)rg_bias(a, e);
     c[e] = v == v ? v : -INFINITY;
   }
   __syncwarp();
@@ -110,7 +116,7 @@ __device__ __noinline__ uint32_t route_grouped_keep64(const RouteGroupedArgs& a,
     double s;
     if (a.sigmoid) { const float v = __ldg(lr + e); s = v == v ? 1.0 / (1.0 + exp(-(double)v)) : 0.0; }
     else s = a.bias ? c[e] * scale : c[e];
-    c[e] = a.bias ? s + (double)__ldg(a.bias + e) : s;
+    c[e] = a.bias ? s + (double)rg_bias(a, e) : s;
   }
   __syncwarp();
   const int size = a.E / a.n_group;
@@ -167,7 +173,7 @@ __device__ __forceinline__ bool route_grouped_row32(const RouteGroupedArgs& a, c
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int e = lane + 32 * j;
-    const float v = e < a.E ? s[j] + (a.bias ? __ldg(a.bias + e) : 0.f) : 0.f;
+    const float v = e < a.E ? s[j] + rg_bias(a, e) : 0.f;
     if (e < a.E) c[lane + 36 * j] = v;                                           // (four words aside every 32: a group's lanes below meet no bank conflicts)
     key[j] = e < a.E ? rg_key(v) : 0u;
   }
@@ -276,7 +282,7 @@ __device__ __forceinline__ bool route_grouped_row32(const RouteGroupedArgs& a, c
   auto inputs = [&](float& l, float& b) {                                        // of the lane's pick
     l = mykey ? __ldg(lr + id) : -INFINITY;
     if (!(l == l)) l = -INFINITY;
-    b = mykey && a.bias ? __ldg(a.bias + id) : 0.f;
+    b = mykey ? rg_bias(a, id) : 0.f;
   };
   float l, b;
   inputs(l, b);
@@ -369,12 +375,13 @@ extern "C" int hb_route_grouped_topk(hb_ctx* ctx, const float* logits, int ld, i
              n_group, E, topk_group, k);
   HB_REQUIRE(ctx, (group_top == 1 || group_top == 2) && (score == HB_SCORE_SOFTMAX || score == HB_SCORE_SIGMOID), HB_ERR_INVALID,
              "route_grouped_topk: group_top=%d (1 or 2) score=%d", group_top, score);
+  HB_REQUIRE(ctx, hb_aligned(logits, 4) && hb_aligned(bias, 4) && hb_aligned(ids, 4) && hb_aligned(w, 4), HB_ERR_INVALID, "route_grouped_topk: pointers must be aligned to their elements");
   RouteGroupedArgs a{logits, ld, M, E, k, n_group, topk_group, group_top, score == HB_SCORE_SIGMOID, renorm, bias, scale, ids, w};
   auto pick = [&](auto sig) {
     constexpr bool S = decltype(sig)::value;
     return E <= 128 ? route_grouped_kernel<4, S> : E <= 256 ? route_grouped_kernel<8, S> : E <= 512 ? route_grouped_kernel<16, S> : route_grouped_kernel<32, S>;
   };
   auto fn = a.sigmoid ? pick(std::true_type{}) : pick(std::false_type{});
-  return hb_launch(ctx, "route_grouped", !(ctx->flags & HB_FLAG_NO_PDL), fn, dim3((M + RG_WARPS - 1) / RG_WARPS), dim3(RG_WARPS * 32),
+  return hb_launch(ctx, "route_grouped", !(ctx->flags & HB_FLAG_NO_PDL), fn, dim3((M - 1) / RG_WARPS + 1), dim3(RG_WARPS * 32),
                    (size_t)RG_WARPS * (E > 32 ? E : 32) * 8, reinterpret_cast<cudaStream_t>(stream), a);
 }

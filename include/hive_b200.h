@@ -155,7 +155,8 @@ HB_API int hb_route_sigmoid_topk(hb_ctx* ctx, const float* logits, const float* 
                                  float* w, void* stream);
 /* (No counterpart in the reference.)  Routing limited to groups of experts, the general router of this library's two score functions.  Per
  * row of logits l (fp32 [M,ld], columns 0..E-1):
- *   s = sigmoid(l) or softmax(l) over the E experts;  c = s + bias (fp32 [E], NULL = none): the bias balances the load, it picks but does not weigh;
+ *   s = sigmoid(l) or softmax(l) over the E experts;  c = s + bias (fp32 [E], NULL = none; infinities count as the largest finite values, NaN as the
+ *   lowest): the bias balances the load, it picks but does not weigh;
  *   the E experts are n_group runs of E / n_group; a group's value is the sum of its group_top (1 or 2) largest c; the topk_group groups of
  *   the largest values stay;  the k experts of the largest c among theirs are picked, best first;
  *   w = s of the pick, divided by (the picks' sum + 1e-20) when renorm, times scale.

@@ -88,6 +88,24 @@ def test_masks_and_extremes(E, score):
                 assert all(len(set(r)) == 6 for r in i.tolist())
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("Ex,k,ng,tg", [(64, 6, 8, 2), (64, 6, 1, 1), (20, 8, 10, 4), (256, 8, 8, 4)])
+def test_bias_that_is_not_finite(E, score, Ex, k, ng, tg):
+    """Infinities count as the largest finite values and NaN as the lowest: picks are experts, all different, whatever the bias holds."""
+    rng = np.random.default_rng(Ex)
+    lg = rng.normal(0, 1, (30, Ex)).astype(np.float32)
+    for n in (1, Ex // 2, Ex):
+        bias = rng.normal(0, 0.1, Ex).astype(np.float32)
+        bias[rng.permutation(Ex)[:n]] = rng.choice([np.nan, np.inf, -np.inf, np.finfo(np.float32).max], n)
+        for gt in (1, 2):
+            import torch
+            ids, w = E.router_grouped_topk(torch.from_numpy(lg).cuda(), k, ng, tg, group_top=gt, score=score, bias=torch.from_numpy(bias).cuda())
+            top = np.finfo(np.float32).max
+            i0, w0 = R.route(lg, np.clip(np.where(np.isnan(bias), -top, bias), -top, top), k, ng, tg, gt, score, True, 1.0)
+            assert np.array_equal(ids.cpu().numpy(), i0)
+            assert (np.abs(w.cpu().numpy() - w0) <= R.route_bound(lg, score) * np.abs(w0) + 2.0 ** -149).all()
+
+
 def test_row_stride_and_rows_behind_the_last(E):
     import torch
     rng = np.random.default_rng(8)
