@@ -159,9 +159,15 @@ struct F8Args {
 // is one map for all experts but for its address.  A CTA's slots go round; one is written again when F8_MAPS items, of at least one stage each, have gone by, more
 // than there are stages: what was loaded through it has been multiplied.
 constexpr int F8_MAPS = 8;
+// A record has to lie at a 16-byte boundary.  One that does not is read from the boundary in front of it, where no load faults, and reported (0x400000).
+__device__ __forceinline__ const uint8_t* f8_rec(const uint8_t* const* tab, int expert) {
+  return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(tab[expert]) & ~(uintptr_t)15);
+}
 struct F8Maps {
   uint8_t* slots; uint32_t n;
-  __device__ __forceinline__ const void* make(const CUtensorMap& tpl, const void* addr) {
+  __device__ __forceinline__ const void* make(const CUtensorMap& tpl, const uint8_t* const* tab, int expert, uint64_t off, uint32_t* err) {
+    const uint8_t* addr = f8_rec(tab, expert) + off;
+    if (reinterpret_cast<uintptr_t>(tab[expert]) & 15u) atomicOr(err, 0x400000u);
     uint8_t* to = slots + (size_t)(n++ % F8_MAPS) * sizeof(CUtensorMap);
     const uint4* from = reinterpret_cast<const uint4*>(&tpl);
 #pragma unroll
@@ -219,7 +225,7 @@ __device__ __forceinline__ void f8_fma2(float& a0, float& a1, uint32_t d0, uint3
       : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
 }
 __device__ __forceinline__ float f8_swiglu(float g, float u, float limit) {
-  if (limit > 0.f) { g = fminf(g, limit); u = fminf(fmaxf(u, -limit), limit); }
+  if (limit > 0.f) { g = g > limit ? limit : g; u = u > limit ? limit : u < -limit ? -limit : u; }   // (NaN stays)
   return __fdividef(g, 1.f + expf(-g)) * u;                                    // (two steps; y is rounded to three bits next)
 }
 __device__ __forceinline__ uint4 f8_pack8(const float* v) {                     // eight values as bf16
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       while (ok && sch.next(item, kb0, kb1)) {
         const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
         const TileRef tl = tile_of(ti);
-        const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab[tl.expert] + a.off_w);
+        const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab, tl.expert, a.off_w, a.err);
         const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, r1 = MODE == F8_GU ? r0 + a.row2 : r0 + 128;   // rows past the last read as zero codes
         auto weights = [&](uint32_t st, int kb) {
           mbar_expect_tx(&full[st], C::STAGE);
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       const float *w0, *w1;
       if (MODE == F8_PLAIN) { w0 = a.ws + (size_t)(2 * nt) * KB; w1 = nt * 256 + 128 < a.N ? w0 + KB : w0; }
       else {
-        const uint8_t* rec = a.tab[tl.expert];
+        const uint8_t* rec = f8_rec(a.tab, tl.expert);
         const int b0 = MODE == F8_GU ? nt : 2 * nt, b1 = MODE == F8_GU ? nt : nt * 256 + 128 < a.N ? b0 + 1 : b0;
         w0 = reinterpret_cast<const float*>(rec + a.off_s0) + (size_t)b0 * KB;
         w1 = reinterpret_cast<const float*>(rec + a.off_s1) + (size_t)b1 * KB;

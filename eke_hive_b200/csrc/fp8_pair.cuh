@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         while (ok && sch.next(item, kb0, kb1)) {
           const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
           const TileRef tl = tile_of(ti);
-          const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab[tl.expert] + a.off_w);
+          const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab, tl.expert, a.off_w, a.err);
           // rows of each half, in boxes of 64: of a pair each CTA loads one, else both are this CTA's.  Rows past the last read as zero codes
           const int r0 = MODE == F8_GU ? nt * 128 : nt * 256, box = MODE == F8_GU ? a.row2 : 64, half = MODE == F8_GU ? 64 : 128;
           auto weights = [&](uint32_t st, int kb) {
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
       const float *w0, *w1;
       if (MODE == F8_PLAIN) w0 = w1 = a.ws + (size_t)min(2 * nt + h, (a.N - 1) / 128) * KB;
       else {
-        const uint8_t* rec = a.tab[tl.expert];
+        const uint8_t* rec = f8_rec(a.tab, tl.expert);
         const int b = MODE == F8_GU ? nt : min(2 * nt + h, (a.N - 1) / 128);
         w0 = reinterpret_cast<const float*>(rec + a.off_s0) + (size_t)b * KB;
         w1 = MODE == F8_GU ? reinterpret_cast<const float*>(rec + a.off_s1) + (size_t)b * KB : w0;

@@ -252,6 +252,24 @@ def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
 
 
+@pytest.mark.parametrize("M,Ex,K", [(5, 6, 3), (60, 6, 3), (150, 4, 3)])
+@pytest.mark.parametrize("limit", [0.0, 1.0])
+def test_moe_rows_that_are_not_finite(E, M, Ex, K, limit):
+    """NaN and infinities of a row come out as NaN in that row alone, clamped or not."""
+    import torch
+    H, I = 256, 256
+    recs = [record(E, H, I, 10 * e) for e in range(Ex)]
+    tab = E.rec_table([r[0] for r in recs])
+    x = torch.randn(M, H, device="cuda", generator=gen(M)).to(torch.bfloat16)
+    ids, w = routing(M, K, Ex, M)
+    ref = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, limit=limit, out_dtype=torch.float32)
+    x[1, 200] = float("nan"); x[3, 0] = float("inf"); x[M - 1, 130] = -float("inf")
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, limit=limit, out_dtype=torch.float32)
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[[1, 3, M - 1]] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], ref[~bad])
+
+
 def test_moe_hot_expert_missing_records_and_invalid_ids(E):
     import torch
 
@@ -281,6 +299,30 @@ def test_moe_rows_behind_the_last_and_layers(E):
         out = torch.full((M + 4, H), -7.0, device="cuda")
         E.moe_fp8(ids, w, tab, li, Ex, x, H, I, out=out[:M])
         assert ((out[:M].double() - o0).abs() <= tol).all() and (out[M:] == -7).all()
+
+
+@pytest.mark.parametrize("M", [3, 40, 150])
+def test_moe_misaligned_record_is_reported(E, M):
+    """A record off its 16-byte boundary sets the device error word; the context works on."""
+    import torch
+    H, I, Ex, K = 256, 256, 4, 2
+    buf = [torch.zeros(E.Fp8RecLayout(H, I).total + 64, dtype=torch.uint8, device="cuda") for _ in range(Ex)]
+    recs = [record(E, H, I, 100 + e) for e in range(Ex)]
+    x = torch.randn(M, H, device="cuda", generator=gen(1)).to(torch.bfloat16)
+    ids, w = routing(M, K, Ex, 2)
+    ids[0, 0] = 1
+    ctx = E.Context()
+    good = E.rec_table([r[0] for r in recs])
+    ref = E.moe_fp8(ids, w, good, 0, Ex, x, H, I, ctx=ctx)
+    ctx.check_device()
+    for off in (1, 4, 8):
+        bad = good.clone()
+        bad[1] = buf[1].data_ptr() + 16 + off
+        E.moe_fp8(ids, w, bad, 0, Ex, x, H, I, ctx=ctx)
+        with pytest.raises(E.HbError, match="0x400000"):
+            ctx.check_device()
+        assert torch.equal(E.moe_fp8(ids, w, good, 0, Ex, x, H, I, ctx=ctx), ref)
+        ctx.check_device()
 
 
 def test_moe_refusals(E):
