@@ -310,7 +310,7 @@ int hb_fp8_quant_rows(hb_ctx* ctx, const void* x, int ldx, int M, int K, uint8_t
   if (!ctx) return HB_ERR_INVALID;
   if (M == 0) return HB_OK;
   HB_REQUIRE(ctx, x && q && s, HB_ERR_INVALID, "fp8_quant_rows: NULL argument");
-  HB_REQUIRE(ctx, M > 0 && K > 0 && K % 16 == 0, HB_ERR_UNSUPPORTED, "fp8_quant_rows: M=%d K=%d (K %% 16)", M, K);
+  HB_REQUIRE(ctx, M > 0 && K > 0 && K % 16 == 0 && K <= 1 << 30, HB_ERR_UNSUPPORTED, "fp8_quant_rows: M=%d K=%d (K %% 16, K <= 2^30)", M, K);
   HB_REQUIRE(ctx, ldx >= K && ldq >= K && ldq % 16 == 0 && lds >= M, HB_ERR_INVALID, "fp8_quant_rows: ldx=%d ldq=%d (>= K=%d, ldq %% 16) lds=%d (>= M=%d)", ldx, ldq, K, lds, M);
   HB_REQUIRE(ctx, hb_aligned(x, 2) && hb_aligned(q, 16) && hb_aligned(s, 4), HB_ERR_INVALID, "fp8_quant_rows: q must be 16-byte aligned, x and s to their elements");
   F8RowsArgs a{};
@@ -321,8 +321,8 @@ int hb_fp8_quant_rows(hb_ctx* ctx, const void* x, int ldx, int M, int K, uint8_t
 int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t* q, float* s, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
   HB_REQUIRE(ctx, w && q && s, HB_ERR_INVALID, "fp8_quantize: NULL argument");
-  HB_REQUIRE(ctx, N > 0 && K > 0 && K % 16 == 0, HB_ERR_UNSUPPORTED, "fp8_quantize: N=%d K=%d (K %% 16)", N, K);
-  HB_REQUIRE(ctx, hb_aligned(w, 16) && hb_aligned(q, 16) && hb_aligned(s, 4), HB_ERR_INVALID, "fp8_quantize: w and q must be 16-byte aligned");
+  HB_REQUIRE(ctx, N > 0 && N <= 1 << 30 && K > 0 && K % 16 == 0 && K <= 1 << 30, HB_ERR_UNSUPPORTED, "fp8_quantize: N=%d K=%d (K %% 16, both <= 2^30)", N, K);
+  HB_REQUIRE(ctx, hb_aligned(w, 16) && hb_aligned(q, 16) && hb_aligned(s, 4), HB_ERR_INVALID, "fp8_quantize: w and q must be 16-byte aligned, s to its elements");
   const long long blocks = (long long)f8_blocks(N) * f8_blocks(K);
   HB_REQUIRE(ctx, blocks < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_quantize: N=%d K=%d", N, K);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -338,7 +338,7 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, W && W->w && W->s && xq && xs && (!yb != !yf), HB_ERR_INVALID, "fp8_gemm: NULL argument, or not exactly one output");
   HB_REQUIRE(ctx, W->fmt == HB_FMT_FP8_B128 && W->N > 0 && W->K > 0 && W->K % 16 == 0 && M > 0, HB_ERR_UNSUPPORTED, "fp8_gemm: FP8_B128 matrix with K %% 16 == 0 wanted (fmt %d N=%d K=%d M=%d)",
              W->fmt, W->N, W->K, M);
-  HB_REQUIRE(ctx, W->K <= 1 << 23, HB_ERR_UNSUPPORTED, "fp8_gemm: K=%d (<= 2^23)", W->K);
+  HB_REQUIRE(ctx, W->K <= 1 << 23 && W->N <= 1 << 30 && M <= 1 << 30, HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d (<= 2^30) K=%d (<= 2^23)", M, W->N, W->K);
   HB_REQUIRE(ctx, ldq >= W->K && ldq % 16 == 0 && lds >= M && ldy >= W->N, HB_ERR_INVALID, "fp8_gemm: ldq=%d (>= K=%d, %% 16) lds=%d (>= M=%d) ldy=%d (>= N=%d)", ldq, W->K, lds, M, ldy, W->N);
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
@@ -357,7 +357,7 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
 }
 
 int hb_fp8_rec_layout_make(int H, int I, hb_fp8_rec_layout* L) {
-  if (!L || H <= 0 || I <= 0 || (H % 128) || (I % 128)) return HB_ERR_INVALID;
+  if (!L || H <= 0 || I <= 0 || (H % 128) || (I % 128) || H > 1 << 20 || I > 1 << 20) return HB_ERR_INVALID;
   const uint64_t w = (uint64_t)H * I, s = (uint64_t)(H / 128) * (I / 128) * 4;
   L->w1 = 0; L->w3 = w; L->w2 = 2 * w; L->s1 = 3 * w; L->s3 = L->s1 + s; L->s2 = L->s3 + s;
   L->total = (L->s2 + s + 4095) / 4096 * 4096;
@@ -377,9 +377,11 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   HB_REQUIRE(ctx, ids && w && rec_tab && x && (cmb ? cmb->out != nullptr : out != nullptr), HB_ERR_INVALID, "moe_fp8: NULL argument");
   hb_fp8_rec_layout L;
   HB_REQUIRE(ctx, hb_fp8_rec_layout_make(H, I, &L) == HB_OK && M > 0 && K >= 1 && K <= 32 && E >= 1 && E <= HB_MAX_EXPERTS && li >= 0 && (long long)M * K < (1ll << 30), HB_ERR_UNSUPPORTED,
-             "moe_fp8: H=%d I=%d (multiples of 128) M=%d K=%d (1..32, M·K < 2^30) E=%d (1..%d) li=%d", H, I, M, K, E, HB_MAX_EXPERTS, li);
+             "moe_fp8: H=%d I=%d (multiples of 128 up to 2^20) M=%d K=%d (1..32, M·K < 2^30) E=%d (1..%d) li=%d", H, I, M, K, E, HB_MAX_EXPERTS, li);
   HB_REQUIRE(ctx, hb_aligned(x, 16) && hb_aligned(out, 16) && (!cmb || (hb_aligned(cmb->shared, 16) && hb_aligned(cmb->out, 16))), HB_ERR_INVALID,
              "moe_fp8: x, out, shared rows and combined output must be 16-byte aligned");
+  HB_REQUIRE(ctx, hb_aligned(ids, 4) && hb_aligned(w, 4) && hb_aligned(rec_tab, 8) && (!cmb || (hb_aligned(cmb->lg, 4) && (!cmb->shared || !cmb->lg || (cmb->col >= 0 && cmb->col < cmb->ld)))), HB_ERR_INVALID,
+             "moe_fp8: ids, w, rec_tab and lg must be aligned to their elements, col within lg's rows");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "moe_fp8: ws NULL or not 256-byte aligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const uint8_t* const* tab = rec_tab + (size_t)li * E;

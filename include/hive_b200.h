@@ -311,7 +311,7 @@ HB_API int hb_fp4_peak_probe(hb_ctx* ctx, int rounds, float* tflops);
 /* ---- 8-bit floats with a scale per block of 128 (e4m3 codes, fp32 scales) ----
  * The format of the reference's FP8 expert and shared-expert matrices (engine/include/hive/glm/glm_moe_fp8.h:24-43): a weight [N,K] is e4m3 codes
  * with one fp32 scale per 128 × 128 block.  Activations are quantised on the way into a product: e4m3 codes with one fp32 scale per
- * row and 128 values of K.  K is a multiple of 16 throughout; the last block of a row may be short.
+ * row and 128 values of K.  K is a multiple of 16 throughout, at most 2^30 (2^23 for the product); the last block of a row may be short.
  *
  * Quantisation of a block (both kinds): amax = its largest magnitude, s = amax / 448, code = e4m3(v · 448 / amax) to the nearest code, ties to the
  * even one; the product and the quotient are fp32 (for bf16 input the code is then the one nearest to the exact quotient).  A block of zeros has s = 0
@@ -325,12 +325,12 @@ HB_API int hb_fp8_quant_rows(hb_ctx* ctx, const void* x_bf16, int ldx, int M, in
 HB_API int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t* q, float* s, void* stream);
 /* y[m,n] = Σ_b xs[b,m]·W.s[n/128,b]·Σ_{k in block b} xq[m,k]·W.w[n,k], written as bf16 (yb) or fp32 (yf): exactly one non-NULL, row stride ldy
  * elements.  W of format HB_FMT_FP8_B128; xq / xs as hb_fp8_quant_rows writes them.  M ≥ 0 (0 does nothing) from one token to prompt chunks,
- * any N.  Products are exact, sums fp32.  xq and W.w 16-byte aligned.  ws ≥ hb_fp8_gemm_ws_bytes(M, N, K), 256-byte aligned. */
+ * any N (both at most 2^30).  Products are exact, sums fp32.  xq and W.w 16-byte aligned.  ws ≥ hb_fp8_gemm_ws_bytes(M, N, K), 256-byte aligned. */
 HB_API size_t hb_fp8_gemm_ws_bytes(int M, int N, int K);
 HB_API int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb_bf16, float* yf, int ldy, void* ws,
                        void* stream);
 /* An expert of such weights as one record: codes of gate w1 [I,H], up w3 [I,H], down w2 [H,I], then their scales s1, s3 [I/128,H/128],
- * s2 [H/128,I/128], to a multiple of 4096 bytes.  H and I multiples of 128. */
+ * s2 [H/128,I/128], to a multiple of 4096 bytes.  H and I multiples of 128, at most 2^20. */
 typedef struct hb_fp8_rec_layout {
   uint64_t w1, w3, w2, s1, s3, s2, total;
 } hb_fp8_rec_layout;

@@ -38,6 +38,14 @@ def test_refusals_without_a_device(lib):
     assert L.hb_route_grouped_topk(None, None, 1, 1, 1, 1, 1, 1, 1, 0, None, 0, 1.0, None, None, None) < 0
 
 
+def test_shapes_beyond_the_range(lib):
+    L = lib.load()
+    r = lib.Fp8RecLayout()
+    assert L.hb_fp8_rec_layout_make(1 << 20, 128, C.byref(r)) == 0 and r.w3 == 128 << 20
+    for H, I in (((1 << 20) + 128, 128), (128, (1 << 20) + 128), (2 ** 31 - 128, 128)):
+        assert L.hb_fp8_rec_layout_make(H, I, C.byref(r)) < 0 and L.hb_moe_fp8_ws_bytes(1, 1, 1, H, I) == 0
+
+
 def test_workspaces_grow_with_the_call(lib):
     L = lib.load()
     last = 0

@@ -247,6 +247,86 @@ def test_moe(E, M, H, I, Ex, K):
     moe_check(E, M, H, I, Ex, K, M + H)
 
 
+# (pairs, pairs an expert): a list of 32 and one more; the longest that the kernels order for themselves and one more; experts just at 8 and 24 pairs on
+# average and above; more experts than rows; the most experts and picks a call may have
+@pytest.mark.parametrize("M,Ex,K", [(8, 4, 4), (11, 4, 3), (256, 160, 4), (205, 150, 5), (16, 4, 2), (17, 4, 2), (48, 4, 2), (49, 4, 2), (600, 80, 3), (3, 1024, 32), (40, 1024, 32)])
+def test_moe_lists_of_pairs(E, M, Ex, K):
+    """Every way the pairs are put in order and cut into tiles, over few different records."""
+    import torch
+    H, I, R0 = 256, 128, 6
+    recs = [record(E, H, I, 10 * e + M) for e in range(R0)]
+    tab = torch.tensor([0 if e % 13 == 5 else recs[e % R0][0].data_ptr() for e in range(Ex)], dtype=torch.int64, device="cuda")
+    ids, w = routing(M, K, Ex, M)
+    ids[M // 2, 0] = Ex; ids[0, K - 1] = -5
+    x = (torch.randn(M, H, device="cuda", generator=gen(M)) * 2).to(torch.bfloat16)
+    # of the same record: the reference's expert
+    at = torch.where((ids >= 0) & (ids < Ex) & (ids % 13 != 5), ids % R0, -1)
+    o0, tol = torch.zeros(M, H, dtype=torch.float64, device="cuda"), torch.zeros(M, H, dtype=torch.float64, device="cuda")
+    for k in range(K):                                                                  # pair by pair: a row may have a record more than once
+        o, t, _ = R.moe(at[:, k:k + 1], w[:, k:k + 1], [r[1] for r in recs], x)
+        o0 += o; tol += t
+    tol += 2.0 ** -23 * K * K * o0.abs() + 2.0 ** -23 * K * tol                         # the sum over the picks: an addition each, of sums no larger than all together
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=torch.float32)
+    big = torch.zeros_like(o0)
+    for k in range(K):
+        o, _, _ = R.moe(at[:, k:k + 1], w[:, k:k + 1], [r[1] for r in recs], x)
+        big += o.abs()
+    assert ((out.double() - o0).abs() <= tol + 2.0 ** -23 * K * big + 1e-30).all()
+    assert torch.equal(out, E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=torch.float32))
+
+
+def test_few_ctas_and_many(E):
+    """Contexts that may use fewer CTAs cut the items elsewhere: the results stay within fp32 summation order, cut items or not."""
+    import torch
+    for M, N, K in ((1, 1000, 2048), (20, 640, 1024), (50, 500, 2048), (100, 700, 1536), (300, 1100, 1024)):
+        q, s = matrix(N, K, N)
+        W = E.GMat(E.FMT_FP8_B128, N, K, q, s)
+        xq, xs = E.fp8_quant_rows(rows(M, K, M))
+        y0, a = R.gemm(R.codes_to_f64(xq), xs.double(), q.double(), s.double())
+        tol = R.sum_bound(K) * a
+        tol = tol + R.HALF[torch.float32] * (y0.abs() + tol)
+        for n in (1, 2, 3, 7, 64, 147):
+            ctx = E.Context(max_ctas=n)
+            y = E.fp8_gemm(W, xq, xs, out_dtype=torch.float32, ctx=ctx)
+            assert ((y.double() - y0).abs() <= tol).all(), (M, n)
+            ctx.check_device()
+    H, I, Ex, Kk, M = 512, 256, 5, 3, 70
+    recs = [record(E, H, I, 10 * e) for e in range(Ex)]
+    tab = E.rec_table([r[0] for r in recs])
+    x = torch.randn(M, H, device="cuda", generator=gen(7)).to(torch.bfloat16)
+    for m in (1, 12, M):
+        ids, w = routing(m, Kk, Ex, m)
+        o0, tol, _ = R.moe(ids, w, [r[1] for r in recs], x[:m])
+        for n in (1, 5, 40):
+            ctx = E.Context(max_ctas=n)
+            out = E.moe_fp8(ids, w, tab, 0, Ex, x[:m], H, I, out_dtype=torch.float32, ctx=ctx)
+            assert ((out.double() - o0).abs() <= tol).all(), (m, n)
+            ctx.check_device()
+
+
+def test_gemm_matrix_beyond_32_bits(E):
+    """Rows of a weight, and rows of x, more than 2^32 bytes from their first."""
+    import torch
+    M, N, K = 3, 300000, 16384
+    q = torch.zeros(N, K, dtype=torch.uint8, device="cuda")
+    s = torch.ones(R.up(N), R.up(K), device="cuda")
+    part, _ = matrix(256, K, 1)
+    q[-256:] = part.view(torch.uint8)
+    xq, xs = E.fp8_quant_rows(rows(M, K, M))
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q, s), xq, xs, out_dtype=torch.float32)
+    y0, a = R.gemm(R.codes_to_f64(xq), xs.double(), part.double(), s[:2].double())
+    assert (y[:, :-256] == 0).all()
+    assert ((y[:, -256:].double() - y0).abs() <= R.sum_bound(K) * a + R.HALF[torch.float32] * (y0.abs() + R.sum_bound(K) * a)).all()
+    del y
+    # the same memory as rows of x: the last 300 of them, and all in one call
+    part2, s2 = matrix(130, K, 2)
+    xs = torch.ones(R.up(K), N, device="cuda")
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, 130, K, part2, s2), q, xs, out_dtype=torch.float32)
+    y0, a = R.gemm(part.double(), torch.ones(R.up(K), 256, dtype=torch.float64, device="cuda"), part2.double(), s2.double())
+    assert (y[:-256] == 0).all()
+    assert ((y[-256:].double() - y0).abs() <= R.sum_bound(K) * a + R.HALF[torch.float32] * (y0.abs() + R.sum_bound(K) * a)).all()
+
+
 def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
@@ -342,6 +422,32 @@ def test_moe_refusals(E):
     with pytest.raises(E.HbError):
         E.Fp8RecLayout(200, 128)
     assert E.moe_fp8(ids[:0], w[:0], tab, 0, 4, x[:0], 256, 256).shape == (0, 256)
+
+
+def test_arguments_of_the_wrong_type_or_shape(E):
+    import torch
+    q, s = matrix(64, 256, 1)
+    W = E.GMat(E.FMT_FP8_B128, 64, 256, q, s)
+    xq, xs = E.fp8_quant_rows(rows(4, 256, 2))
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    calls = [lambda: E.fp8_gemm(W, xq, xs, y=torch.empty(4, 64, dtype=torch.float16, device="cuda")), lambda: E.fp8_gemm(W, xq, xs, y=torch.empty(3, 64, **bf)),
+             lambda: E.fp8_gemm(W, xq, xs.double()), lambda: E.fp8_gemm(W, xq, xs[:1]), lambda: E.fp8_gemm(W, xq[:, :240], xs), lambda: E.fp8_gemm(W, xq.float(), xs),
+             lambda: E.fp8_quant_rows(rows(4, 256, 2), q=torch.empty(3, 256, dtype=torch.uint8, device="cuda")), lambda: E.fp8_quant_rows(rows(4, 256, 2), s=torch.empty(2, 3, device="cuda")),
+             lambda: E.fp8_quantize(rows(4, 256, 2), q=torch.empty(4, 512, dtype=torch.uint8, device="cuda")[:, ::2]),
+             lambda: E.router_grouped_topk(torch.zeros(2, 64, **bf), 2), lambda: E.router_grouped_topk(torch.zeros(2, 64, device="cuda"), 2, bias=torch.zeros(63, device="cuda")),
+             lambda: E.router_grouped_topk(torch.zeros(2, 64, device="cuda"), 2, ids=torch.zeros(1, 2, dtype=torch.int32, device="cuda")),
+             lambda: E.router_grouped_topk(torch.zeros(2, 64, device="cuda"), 2, ids=torch.zeros(2, 2, dtype=torch.int64, device="cuda"))]
+    x = torch.zeros(2, 256, **bf)
+    ids, w = routing(2, 2, 4, 1)
+    tab = torch.zeros(4, dtype=torch.int64, device="cuda")
+    moe = lambda **k: E.moe_fp8(**{**dict(ids=ids, w=w, rec_tab=tab, li=0, E=4, x=x, H=256, I=256), **k})
+    moe()
+    calls += [lambda k=k: moe(**k) for k in (dict(ids=ids.long()), dict(w=w.double()), dict(w=w[:1]), dict(x=x.float()), dict(x=x[:, :128]), dict(x=x[:1]), dict(rec_tab=tab[:3]), dict(li=1),
+                                             dict(out=torch.empty(1, 256, **bf)), dict(out=torch.empty(2, 256, dtype=torch.float16, device="cuda")), dict(shared=x[:1]), dict(shared=x.float()),
+                                             dict(shared=x, lg=torch.zeros(2, 3, device="cuda"), col=3), dict(shared=x, lg=torch.zeros(2, 3, device="cuda"), col=-1), dict(shared=x, lg=x))]
+    for c in calls:
+        with pytest.raises(E.HbError):
+            c()
 
 
 # ---------------------------------------------------------------------------------------------------- together
