@@ -10,7 +10,7 @@
 // n for many rows m — in the gate/up pass gate and up of the same value.
 //
 // Work: items (tile of rows × 256 weight rows) of ceil(K / 128) steps.  The list is cut into equal runs of steps, one a CTA, without regard to where an item
-// ends (in fp8_pair.cuh only what whole rounds of items over the CTAs leave over).  A CTA that holds part of an item leaves its sums in the workspace; the last
+// ends.  A CTA that holds part of an item leaves its sums in the workspace; the last
 // one to arrive (a counter an item) adds all parts in the order of the CTAs — the same order in every run — and finishes the item.  So a product
 // with one row of x keeps all SMs streaming weights to the end.  Nobody waits for anybody.
 //
@@ -18,6 +18,8 @@
 // MMAs, warp 10 multiplies the step's scales, warps 0-7 read the sums back (a warp reaches the 32 lanes of its number mod 4; warps 0-3 take the first half
 // of the columns, 4-7 the second) and end the items.  Two accumulator buffers: one fills while the other is read.  Every wait is bounded.
 #pragma once
+#include <type_traits>
+
 #include "fp8_common.cuh"
 #include "hb_kernels.h"
 #include "tc_common.cuh"
@@ -129,13 +131,10 @@ constexpr int F8_A_BYTES = 128 * 128;                  // a tile of weights: 128
 
 template <int BN_>
 struct F8Cfg {
-  static constexpr int BN = BN_, CW = BN / 2;          // rows of x a tile may have; columns of tensor memory an epilogue warp reads of each weight tile
+  static constexpr int BN = BN_, CW = BN / 2;          // rows of x a tile may have; columns of tensor memory an epilogue warp reads of each weight tile, at a time
   static constexpr int B_BYTES = BN * 128, STAGE = 2 * F8_A_BYTES + B_BYTES;
   static constexpr int ST = 200 * 1024 / STAGE;        // ring of operand stages
   static constexpr int TMEM = BN <= 16 ? 64 : 4 * BN;  // two buffers of two tiles
-  static constexpr int LD = CW < 32 ? CW : 32;         // columns read at a time
-  static constexpr int NCH = 2 * CW / LD;              // reads a step takes: even
-  static constexpr bool SPLIT = BN >= 64;              // the sums need more registers than a twelfth of the file: the other warps give some of theirs
   static constexpr int SMEM = 1024 + ST * STAGE + 4 * 2 * BN * 4 + 8 * CW * 4 + 512 + F8_PLAN_PAIRS * (int)sizeof(TileRef);   // (the tile list: GU)
   static_assert(F8_COUNTERS <= kErrCounterWords, "counters of the context");
   static_assert(ST < 8 && SMEM <= 227 * 1024 && TMEM <= 512 && STAGE % 1024 == 0, "shared memory, tensor memory, swizzle atoms");
@@ -145,6 +144,7 @@ struct F8Args {
   const TileRef* tiles; const int* n_tiles;            // GU / DOWN: tiles of slots; PLAIN: ceil(M / per) tiles of `per` rows
   F8Plan plan;                                         // GU with plan.P > 0: the tiles are worked out here
   int M, per, N, K, n_nt;                              // n_nt: items a tile has (GU: N / 128 with N = I, else ceil(N / 256))
+  int split;                                           // fp8_pair.cuh, tiles of single CTAs: CTAs of a cluster, 1, 2 or 4
   const float* ws; const uint8_t* const* tab; uint64_t off_w, off_s0, off_s1; int row2;   // PLAIN: scales; else records, offsets of the codes and of the two tiles' scales, rows from the first tile's matrix to the second's (GU)
   uint8_t* maps;                                       // GU / DOWN: room for F8_MAPS tensor maps a CTA
   const float* xs; int lds;                            // scales of the rows
@@ -181,17 +181,18 @@ struct F8Maps {
 
 // The steps of a CTA, the same for all its warps: segments (item, first step, end).
 struct F8Sched {                                       // (32 bits: at most 320 items of at most 2^16 steps, or 2^24 steps, times 160 CTAs)
-  uint32_t KB, G, me, dp, sk, U, Gs, u, u1, i;
-  // runs: no rounds, the whole list in equal runs (as long as its steps can be counted so): a CTA stays with an expert.  Else, even: with fewer items than CTAs
-  // cut every one into the same number of runs and leave CTAs without work
-  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool runs, bool even) {
+  uint32_t KB, G, me, dp, sk, U, Gs, end, u, u1, i;
+  // runs: no rounds, the whole list in equal runs (as long as its steps can be counted so): a CTA stays with an expert.  Else rounds, and of what they leave over
+  // items are cut where that saves more than `slack` steps
+  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool runs, uint32_t slack) {
     KB = KB_; G = G_; me = me_;
     const uint32_t waves = items / G, rem = items - waves * G;
     const bool all = runs && (unsigned long long)items * KB < (1ull << 24);
-    dp = all ? 0u : rem == 0u ? waves : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
-    sk = items - dp * G;
-    U = sk * KB;
-    Gs = min(even && waves == 0u && items > 0u ? G / items * items : G, max(U, 1u));   // CTAs that get a run of steps: none is empty
+    const bool cut = rem != 0u && (unsigned long long)(G - rem) * KB > (unsigned long long)slack * G;
+    dp = all ? 0u : !cut ? waves + (rem != 0u) : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
+    sk = all || cut ? items - dp * G : 0u;
+    U = sk * KB; end = items;
+    Gs = min(G, max(U, 1u));                                                   // CTAs that get a run of steps: none is empty
     u = start(me); u1 = start(me + 1u);
     i = 0u;
   }
@@ -205,7 +206,7 @@ struct F8Sched {                                       // (32 bits: at most 320 
     }
     if (i >= dp) return false;
     item = (int)(sk + i * G + me); kb0 = 0; kb1 = (int)KB; ++i;
-    return true;
+    return (uint32_t)item < end;
   }
   __device__ __forceinline__ uint32_t owner(uint32_t step) const { return ((step + 1u) * Gs - 1u) / U; }
 };
@@ -290,8 +291,7 @@ __device__ __forceinline__ void f8_landed(uint32_t (&r)[W], uint32_t (&p)[W]) {
 }
 template <int W>
 __device__ __forceinline__ void f8_ld(uint32_t taddr, uint32_t (&r)[W]) {
-  if constexpr (W == 32) tc_ld32(taddr, r);
-  else if constexpr (W == 16) tc_ld16(taddr, r);
+  if constexpr (W == 16) tc_ld16(taddr, r);
   else tc_ld8(taddr, r);
 }
 
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   const int KB = f8_blocks(a.K);
   if (!own_plan) n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
   F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, true, false);
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x, blockIdx.x, true, 0u);
   auto tile_of = [&](int ti) -> TileRef {
     if (own_plan) return tile_s[ti];
     if (MODE != F8_PLAIN) return a.tiles[ti];
@@ -345,7 +345,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   int item, kb0, kb1;
 
   if (warp >= 8) {
-  if constexpr (C::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_REGS_REST));
   if (warp == F8_W_TMA) {
     // ------------------------------------------------------------------------------------------------ operand tiles, one thread
     if (elect_one()) {
@@ -458,7 +457,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     }
   }
   } else {
-    if constexpr (C::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
     griddep_wait();
     griddep_launch();
     // ------------------------------------------------------------------------------------------------ sums: warp (h, q) has lanes [32 q, 32 q + 32) and of each weight
@@ -475,49 +473,29 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       float acc[2][C::CW];
 #pragma unroll
       for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
-      // Read i of a buffer: columns (i mod NCH / 2)·LD of tile i / (NCH / 2).  A wait for reads waits for all that are under way, so two go out together,
-      // each as soon as the registers it writes have been added up (one at a time, each behind the other's additions: 730 clocks a step of 256 columns)
-      uint32_t ra[C::LD], rb[C::LD];
+      // A wait for reads waits for all that are under way, so two go out together (one weight tile each), each as soon as the registers it writes have been
+      // added up (one at a time, each behind the other's additions: 730 clocks a step of 256 columns)
+      uint32_t ra[C::CW], rb[C::CW];
       auto arrived = [&](uint32_t n) {
         const bool o = mbar_wait(&acc_full[n & 1u], (n >> 1) & 1u, a.err, 0x1000u);
         tc_fence_after();
         return (bool)__all_sync(0xffffffffu, o);
       };
-      auto read2 = [&](uint32_t t, int n) {
-        constexpr int half = C::NCH / 2;
-        f8_ld<C::LD>(t + (n / half) * BN + (n % half) * C::LD, ra);
-        f8_ld<C::LD>(t + ((n + 1) / half) * BN + ((n + 1) % half) * C::LD, rb);
-      };
-      if ((ok = ok && arrived(it)) && active) read2(trow + (it & 1u) * (2 * BN), 0);
+      if ((ok = ok && arrived(it)) && active) { f8_ld<C::CW>(trow + (it & 1u) * (2 * BN), ra); f8_ld<C::CW>(trow + (it & 1u) * (2 * BN) + BN, rb); }
       for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
-        const uint32_t buf = it & 1u, tb = trow + buf * (2 * BN);
+        const uint32_t buf = it & 1u, nb = trow + (buf ^ 1u) * (2 * BN);
         const float* sb = scl + (it & 3u) * (2 * BN) + h * C::CW;
-        constexpr int half = C::NCH / 2;
-        auto add = [&](float* to, const uint32_t (&d)[C::LD], int u, int c0) {
-          f8_add<C::LD>(to, d, sb + u * BN + c0);
-        };
         if (active) {
-#pragma unroll
-          for (int i = 0; i < C::NCH; i += 2) {
-            f8_landed<C::LD>(ra, rb);
-            const bool end = i + 2 == C::NCH;
-            if (end) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&acc_empty[buf]);                     // the buffer's sums are in registers
-            }
-            add(&acc[i / half][(i % half) * C::LD], ra, i / half, (i % half) * C::LD);
-            const bool more = !end || (kb + 1 < kb1 && (ok = arrived(it + 1)));
-            const uint32_t nb = end ? trow + (buf ^ 1u) * (2 * BN) : tb;
-            const int n = end ? 0 : i + 2;
-            if (more) f8_ld<C::LD>(nb + (n / half) * BN + (n % half) * C::LD, ra);
-            add(&acc[(i + 1) / half][((i + 1) % half) * C::LD], rb, (i + 1) / half, ((i + 1) % half) * C::LD);
-            if (more) f8_ld<C::LD>(nb + ((n + 1) / half) * BN + ((n + 1) % half) * C::LD, rb);
-          }
-        } else {
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          if (kb + 1 < kb1) ok = arrived(it + 1);
+          f8_landed<C::CW>(ra, rb);
+          tc_fence_before();
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);                           // the buffer's sums are in registers
+        if (active) f8_add<C::CW>(acc[0], ra, sb);
+        const bool more = kb + 1 < kb1 && (ok = arrived(it + 1)) && active;
+        if (more) f8_ld<C::CW>(nb, ra);
+        if (active) f8_add<C::CW>(acc[1], rb, sb + BN);
+        if (more) f8_ld<C::CW>(nb + BN, rb);
       }
       // ---- an item that other CTAs have parts of: leave the sums, the last one to arrive goes on with everybody's
       if (kb1 - kb0 < KB) {
@@ -544,28 +522,24 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
         // parts and columns fetched together; a value's parts are added in order
-        constexpr int NP = C::CW <= 8 ? 8 : 2, GC = C::CW < 32 ? C::CW : 16;
+        constexpr int NP = C::CW <= 8 ? 8 : 2;
         const float* first = part_of(c_first, sch.start(c_first));
         const float* rest = part_of(c_first, s0);                              // the later CTAs' parts are their first ones: 2 · 256 · BN apart
-        for (uint32_t cc = c_first; cc <= c_last; cc += NP) {
+        for (uint32_t cc = c_first; cc <= c_last && active; cc += NP) {
+          float t[NP][2][C::CW];
 #pragma unroll
-          for (int g = 0; g < C::CW; g += GC) {
-            if (!active || g >= cols) break;
-            float t[NP][2][GC];
+          for (int i = 0; i < NP; ++i) {
+            const float* p = cc + i == c_first ? first : rest + (size_t)(cc + i - c_first) * (2 * 256 * BN);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              const float* p = cc + i == c_first ? first : rest + (size_t)(cc + i - c_first) * (2 * 256 * BN);
-#pragma unroll
-              for (int c = 0; c < GC; ++c) {
-                const bool on = g + c < cols && cc + i <= c_last;
-                t[i][0][c] = on ? __ldcg(p + (g + c) * 256) : 0.f; t[i][1][c] = on ? __ldcg(p + (g + c) * 256 + 128) : 0.f;
-              }
+            for (int c = 0; c < C::CW; ++c) {
+              const bool on = c < cols && cc + i <= c_last;
+              t[i][0][c] = on ? __ldcg(p + c * 256) : 0.f; t[i][1][c] = on ? __ldcg(p + c * 256 + 128) : 0.f;
             }
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-#pragma unroll
-              for (int c = 0; c < GC; ++c) { acc[0][g + c] += t[i][0][c]; acc[1][g + c] += t[i][1][c]; }
           }
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int c = 0; c < C::CW; ++c) { acc[0][c] += t[i][0][c]; acc[1][c] += t[i][1][c]; }
         }
       }
       // ---- the item's results

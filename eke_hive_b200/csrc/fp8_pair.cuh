@@ -1,24 +1,50 @@
 // The product of fp8_gemm.cuh for many rows: two CTAs of a cluster work on one tile of 256 rows of x × 256 weight rows (tcgen05 cta_group::2), or one CTA on a
 // tile of 128 rows.
 //
-// Rows of x are the A operand, 128 of them in each CTA's shared and tensor memory; the weight rows are the B operand, of which each CTA loads half
+// Rows of x are the A operand, 128 of them in each CTA's shared and tensor memory; the weight rows are the B operand, of which each CTA of a pair loads half
 // and both read all: 32 KB of operands per CTA and step for 128 × 256 × 128 multiply-adds.  (One CTA alone needs 48 KB for them, and the SMs pull no more than
-// some 10 TB/s out of L2: 1.7 PFLOP/s.  That form is for calls whose runs of rows would leave much of a pair's tile empty.)  A lane of tensor memory is a row of x: the scale of a step is one number a thread, the row's
-// times the weight block's.
+// some 10 TB/s out of L2: 4096 rows of 17408 x 5120 take 444 us with single CTAs, 396 with pairs.  That form is for runs of rows that would leave much of a
+// pair's tile empty, and where there are few items.)  A lane of tensor memory is a row of x: the scale of a step is one number a thread, the row's times the
+// weight block's.
 //
 // The 256 weight rows are two halves of 128, each with an accumulator of its own, double buffered (all of tensor memory), and its own warps: warps 0-3 read
-// back half 0, warps 4-7 half 1, and while one half's MMAs run the other half is read.  Gate/up: a half is 64 gate rows (loaded by CTA 0) and the 64 up
-// rows that belong to them (CTA 1), so a thread has both for its row of x.
+// back half 0, warps 4-7 half 1, and while one half's MMAs run the other half is read.  Gate/up (single CTAs): a half is 64 gate rows and the 64 up rows that
+// belong to them, so a thread has both for its row of x.
 //
-// Warp 8 (one thread) loads, warps 9 and 10 (one thread each, in CTA 0) issue the MMAs of both CTAs, a half each, and announce finished buffers and free
-// stages to both.  Work is cut
-// and put together as in fp8_gemm.cuh, a pair of CTAs in the place of a CTA; each CTA looks after the parts of its own 128 rows.
+// Warp 8 (one thread) loads, warps 9 and 10 (one thread each, of a pair those of CTA 0) issue the MMAs, a half each, and announce finished buffers and free
+// stages.  What bounds it: the read-back and scaling of every block's sums, 256 clocks of fused multiply-adds a step of 512 clocks of MMAs, behind waits and
+// scales of their own: some 1000 clocks a step in all; large products run at the power limit's clock.
+//
+// Work is items as in fp8_gemm.cuh, in rounds of one item a CTA (or pair).  Of single CTAs, items that the last full round leaves over are split along K among
+// the CTAs of a cluster, two or four, that add their sums up through each other's shared memory: 4 to 5 us.  Of pairs, they are cut and put together through the
+// workspace as in fp8_gemm.cuh, each CTA with the parts of its own 128 rows, where 20 us of that are less than what it saves.
 #pragma once
 #include "fp8_gemm.cuh"
 
 namespace hb {
 
 constexpr int F8S_ROWS = 128, F8P_ROWS = 256;          // rows of x a tile may have: one CTA, a pair
+constexpr uint32_t F8S_WHOLE = 16;                     // steps up to which an item of single CTAs stays whole: putting its sums together takes some 8 (two CTAs) or 12 (four)
+constexpr uint32_t F8P_SLACK = 40;                     // steps that cutting has to save: leaving and adding up parts takes a pair some 20 us
+// Steps of a CTA of the one-CTA form: rounds of whole items, then the items left over, each split among the CTAs of a cluster where there are enough clusters.
+struct F8Rounds {
+  uint32_t KB, G, me, dp, rem, split, i;
+  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool, uint32_t cluster) {
+    KB = KB_; G = G_; me = me_;
+    dp = items / G; rem = items - dp * G;
+    split = rem * cluster <= G && KB > F8S_WHOLE ? cluster : 1u;
+    i = 0u;
+  }
+  __device__ __forceinline__ bool splits() const { return split > 1u && me / split < rem; }   // the same for all CTAs of a cluster
+  __device__ __forceinline__ bool next(int& item, int& kb0, int& kb1) {
+    if (i > dp) return false;
+    if (i++ < dp) { item = (int)((i - 1u) * G + me); kb0 = 0; kb1 = (int)KB; return true; }
+    const uint32_t t = me / split, r = me - t * split;
+    if (t >= rem) return false;
+    item = (int)(dp * G + t); kb0 = (int)(KB * r / split); kb1 = (int)(KB * (r + 1u) / split);
+    return true;
+  }
+};
 template <bool PAIR>
 struct F8PCfg {
   static constexpr int CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS;
@@ -26,6 +52,8 @@ struct F8PCfg {
   static constexpr int STAGE = XB + 2 * HB, ST = PAIR ? 6 : 4;
   static constexpr int STG = 8 * F8_STG_BYTES;
   static constexpr int SMEM = 1024 + ST * STAGE + STG + 2 * 128 * 4 + 512;
+  using Sched = std::conditional_t<PAIR, F8Sched, F8Rounds>;
+  static_assert(PAIR || ST * STAGE >= 2 * 128 * 128 * 4, "a split item's sums take the place of the operands");
   static_assert(ST < F8_MAPS && SMEM <= 227 * 1024, "map slots, shared memory");
 };
 
@@ -38,6 +66,11 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 // Arrival on a barrier of the pair.  No memory is handed over by it: what it orders are reads of tensor memory that have come back (tcgen05.wait::ld) and the
 // MMAs that write there next; a release for the cluster, and acquires to match in every wait, cost 1000 clocks a step.
@@ -93,7 +126,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile uint32_t* last = tmem_slot + 1;
   const int warp = warp_uniform(), lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;                            // of the pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
     for (int s = 0; s < 4; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * C::CTAS); }
@@ -111,8 +144,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
   const uint32_t tmem = *tmem_slot;
   // before griddep_wait: as in fp8_gemm.cuh (the tiles come from the kernel in front of the one in front)
   const int KB = f8_blocks(a.K), n_tiles = MODE == F8_PLAIN ? (a.M + a.per - 1) / a.per : *a.n_tiles;
-  F8Sched sch;
-  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / C::CTAS, blockIdx.x / C::CTAS, false, true);
+  typename C::Sched sch;
+  sch.init((uint32_t)n_tiles * a.n_nt, KB, gridDim.x / C::CTAS, blockIdx.x / C::CTAS, false, PAIR ? F8P_SLACK : (uint32_t)a.split);
   auto tile_of = [&](int ti) -> TileRef {
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
@@ -216,7 +249,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
       const TileRef tl = tile_of(ti);
       const int rows = min(max(tl.rows - 128 * (int)rank, 0), 128);            // of this CTA
       const size_t slot0 = (size_t)tl.slot0 + 128 * rank;
-      const bool active = 32 * q < rows, valid = row < rows;
+      bool active = 32 * q < rows, valid = row < rows;
       // scales: of the row, of the weight blocks (gate/up: columns 0-63 gate, 64-127 up; else one block)
       const float *w0, *w1;
       if (MODE == F8_PLAIN) w0 = w1 = a.ws + (size_t)min(2 * nt + h, (a.N - 1) / 128) * KB;
@@ -274,8 +307,51 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         if (active) f8_add<32>(acc + 96, rb, f1);
         if (more) tc_ld32(nb + 32, rb);
       }
-      // ---- an item that other pairs have parts of: leave the sums, the last one to arrive goes on with everybody's
-      if (kb1 - kb0 < KB) {
+      if constexpr (!PAIR) {
+        // ---- an item split among the cluster's CTAs (this one's last): the sums take the operands' place in shared memory, CTA r goes on with everybody's
+        // of its part of the rows, added up in the order of the CTAs
+        if (kb1 - kb0 < KB) {
+          mbar_wait(mma_done, 0, a.err, 0x800u);                               // no MMA reads the operands any more
+          float4* mine = reinterpret_cast<float4*>(sm) + h * 128 + row;        // [four columns][half][row]
+          if (active) {
+#pragma unroll
+            for (int c = 0; c < 128; c += 4) mine[c * 64] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          }
+          __syncwarp();
+          cluster_sync_all();
+          // all eight warps add up, four columns of a row at a time, and put the sum in the place of this CTA's own
+          const int rs = 128 / (int)sch.split, r0 = (int)cluster_rank() * rs, lr = 31 - __clz(rs);
+          if (r0 < rows) {
+#pragma unroll 1
+            for (int u0 = threadIdx.x; u0 < 64 * rs; u0 += 4 * 256) {          // [four columns][half][row], four under way at a time
+              uint32_t at[4]; float4 v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int u = u0 + 256 * i;
+                at[i] = (uint32_t)(((u >> lr) << 7) + r0 + (u & (rs - 1))) * 16u; v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              }
+#pragma unroll 1
+              for (uint32_t cc = 0; cc < sch.split; ++cc) {
+                const uint32_t from = mapa_u32(base, cc);
+                float4 t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] = ld_cluster(from + at[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { v[i].x += t[i].x; v[i].y += t[i].y; v[i].z += t[i].z; v[i].w += t[i].w; }
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(sm + at[i]) = v[i];
+            }
+          }
+          named_bar_sync(1, 256);
+          active = active && 32 * q / rs == (int)cluster_rank(); valid = valid && active;
+          if (active) {
+#pragma unroll
+            for (int c = 0; c < 128; c += 4) { const float4 v = mine[c * 64]; acc[c] = v.x; acc[c + 1] = v.y; acc[c + 2] = v.z; acc[c + 3] = v.w; }
+          }
+        }
+      } else if (kb1 - kb0 < KB) {
+        // ---- an item that other pairs have parts of: leave the sums, the last one to arrive goes on with everybody's
         const uint32_t st0 = (uint32_t)item * (uint32_t)KB, c_first = sch.owner(st0), c_last = sch.owner(st0 + KB - 1);
         // a part: [column][half][row]; a pair's first run is its part 0
         auto part_of = [&](uint32_t c, uint32_t st) { return a.part + ((size_t)(C::CTAS * c + rank) * 2 + (c == c_first && st != st0 ? 1 : 0)) * (256 * 128) + h * 128 + row; };
@@ -362,10 +438,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
     }
   }
   __syncwarp();
+  bool splits = false;
+  if constexpr (!PAIR) splits = sch.splits();
+  if (splits && warp >= 8) cluster_sync_all();                                 // the sums are in shared memory
   if (warp == F8_W_TMA) mbar_wait(mma_done, 0, a.err, 0x800u);                 // in both CTAs: the last MMA has retired, and so has the announcement of it
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();
+  if (PAIR || splits) cluster_sync_all();                                      // nobody reads this CTA's shared memory any more
   if (warp == F8_W_MMA) {
     tc_fence_after();
     if constexpr (PAIR) tmem_dealloc2(tmem, 512);

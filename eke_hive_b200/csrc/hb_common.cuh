@@ -35,6 +35,7 @@ struct hb_ctx {
   // streaming down kernels (one per split-K width): whether the planned number of CTAs per SM is really resident, i.e. whether the
   // CTAs may meet inside the kernel (k_moe_decode.cu)
   const void* down_fn[8] = {nullptr}; bool down_meet[8] = {false};
+  int fp8_clusters = 0;           // many-row FP8 product: clusters of four CTAs that are resident at once (k_fp8.cu)
   int dense_clusters[4] = {0};   // dense GEMV: clusters of 1, 2, 4, 8 CTAs that are resident at once (k_dense.cu)
   char err[512] = {0};
   // optional per-kernel timing (hb_profile_enable): a start/stop event pair around every launch, aggregated by hb_profile_read

@@ -230,24 +230,45 @@ F8Pick f8_kernel(int rows) {
   switch (rows) {
     case 16: return {fp8_gemm_kernel<16, MODE>, F8Cfg<16>::SMEM};
     case 32: return {fp8_gemm_kernel<32, MODE>, F8Cfg<32>::SMEM};
-    case 64: return {fp8_gemm_kernel<64, F8_PLAIN>, F8Cfg<64>::SMEM};
     case F8S_ROWS: return {fp8_many_kernel<MODE, false>, F8PCfg<false>::SMEM};
     default: return {fp8_many_kernel<F8_PLAIN, true>, F8PCfg<true>::SMEM};
   }
 }
+// CTAs of a launch: one an SM, in whole clusters of cl.  Not all SMs are in reach of clusters of four.
+int f8_grid(const hb_ctx* ctx, int rows, int cl) {
+  int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
+  if (n > F8_MAX_CTAS) n = F8_MAX_CTAS;
+  if (cl == 4 && rows == F8S_ROWS && n > 4 * ctx->fp8_clusters) n = 4 * ctx->fp8_clusters;
+  return n < cl ? cl : n / cl * cl;
+}
 template <int MODE>
 int f8_launch(hb_ctx* ctx, const char* name, int rows, const F8Args& a, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t st) {
   const F8Pick k = f8_kernel<MODE>(rows);
-  int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
-  if (n > F8_MAX_CTAS) n = F8_MAX_CTAS;
-  if (rows == F8P_ROWS) n = n < 2 ? 2 : n & ~1;
-  return hb_launch_cluster(ctx, name, true, rows == F8P_ROWS ? 2 : 1, k.fn, dim3(n), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
+  const int cl = rows == F8P_ROWS ? 2 : rows == F8S_ROWS ? a.split : 1;
+  return hb_launch_cluster(ctx, name, true, cl, k.fn, dim3(f8_grid(ctx, rows, cl)), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
 }
-size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows > 64 ? 128 : rows) * 4; }
-// Rows of a tile for a product of M rows and n_nt items a tile.  Up to 32 rows a weight row a lane (17408 x 5120, 32 rows: 24 us; a row of x a lane: 28); up to 64
-// the same where an item is cut three times and more (5120 x 17408, 64 rows: 33 us against 46, whose parts are four times the size), else and up to 128 a
-// row of x a lane (37888 x 4096, 64 rows: 31 against 34); more: a pair's tile (18944 x 4096, 512 rows: 45 against 51).
-int f8_rows_for(const hb_ctx* ctx, int M, int n_nt) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 && 3 * n_nt <= ctx->sm_count ? 64 : M <= 128 ? F8S_ROWS : F8P_ROWS; }
+// sums of cut items: two of each CTA.  (A row of x a lane: in pairs alone.)
+size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows == F8P_ROWS ? 128 : rows == F8S_ROWS ? 32 : rows) * 4; }
+// How a dense product is cut.  Up to 32 rows a weight row a lane (17408 x 5120, 32 rows: 24 us; a row of x a lane: 28).  More: a row of x a lane, tiles of 128 rows
+// of single CTAs or of 256 of pairs, by the steps the longest CTA takes.  Single: rounds of whole items, what is left over split among the two or four
+// CTAs of a cluster where there are that many, at the price of some 8 and 12 steps (128 rows of 4096 x 4096: 21 us whole, 17 in two, 15 in four; 2048 x 512: 6.4, 9.3, 10.3).
+// Pairs: a step takes less, as an SM pulls less out of L2, but what is left over is cut through the workspace.
+struct F8Cut { int rows, split; };
+F8Cut f8_cut(const hb_ctx* ctx, int M, int N, int K) {
+  if (M <= 32) return {M <= 16 ? 16 : 32, 1};
+  const long long KB = f8_blocks(K), n_nt = (N + 255) / 256;
+  F8Cut best{F8S_ROWS, 1};
+  long long least = 0;
+  for (int c : {1, 2, 4}) {
+    const long long G = f8_grid(ctx, F8S_ROWS, c), items = (M + F8S_ROWS - 1) / F8S_ROWS * n_nt, rem = items % G;
+    if (c > 1 && (rem * c > G || KB <= F8S_WHOLE)) continue;
+    const long long steps = items / G * KB + (rem == 0 ? 0 : c == 1 ? KB : (KB + c - 1) / c + (c == 2 ? 8 : 12));
+    if (c == 1 || steps < least) { least = steps; best.split = c; }
+  }
+  const long long G = f8_grid(ctx, F8P_ROWS, 2) / 2, items = (M + F8P_ROWS - 1) / F8P_ROWS * n_nt, rem = items % G, cut = (KB * rem + G - 1) / G + F8P_SLACK;
+  const long long steps = items / G * KB + (rem == 0 ? 0 : cut < KB ? cut : KB);
+  return 9 * steps < 10 * least ? F8Cut{F8P_ROWS, 2} : best;
+}
 // Pairs of a tile by what an expert gets on average: longer runs are cut into tiles, which read the expert's weights again, and a tile that is not full
 // wastes its MMAs.  Gate/up + down of 512 experts of 2048 / 512: 20 pairs an expert 310 us with 32, 359 with 128 (39 pairs: 476, 375; 10 pairs: 294, and 293
 // with 16).  A pair of CTAs gains nothing here: 32 experts of 7168 / 2048, 256 pairs an expert, 533 us with 128, 661 with 256, half of whose second tiles are
@@ -276,7 +297,7 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   const int bn = f8_rows_for_pairs((long long)P, E);
   F8Ws t;
   t.hist = (int*)take(hbk_pf_plan_hist_bytes(E)); t.n_slots = (int*)take(4); t.n_tiles = (int*)take(4);
-  t.tiles = (TileRef*)take((P / bn + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
+  t.tiles = (TileRef*)take((P / 16 + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
   t.xq = (uint8_t*)take(P * H); t.xs = (float*)take(P * f8_blocks(H) * 4);
   t.yq = (uint8_t*)take(P * I); t.ys = (float*)take(P * f8_blocks(I) * 4);
   t.part = (__nv_bfloat16*)take(P * H * 2);
@@ -293,14 +314,23 @@ int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
 }  // namespace
 
 int hbk_fp8_setup(hb_ctx* ctx) {
-  for (int bn : {16, 32, 64, F8S_ROWS, F8P_ROWS})
-    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {   // (64 and 256: the dense product alone)
+  for (int bn : {16, 32, F8S_ROWS, F8P_ROWS})
+    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {   // (256: the dense product alone)
       cudaFuncAttributes at;
       HB_CUDA(ctx, cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(k.fn)));
       // a warp that asks for more registers than the block was launched with would wait for good
-      HB_REQUIRE(ctx, bn < 64 || at.numRegs >= F8_REGS, HB_ERR_CUDA, "fp8_gemm: built with %d registers a thread, its warps share out %d", at.numRegs, F8_REGS);
+      HB_REQUIRE(ctx, bn < F8S_ROWS || at.numRegs >= F8_REGS, HB_ERR_CUDA, "fp8_gemm: built with %d registers a thread, its warps share out %d", at.numRegs, F8_REGS);
       HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
     }
+  // clusters of four CTAs of the one-CTA form that are resident at once: where an SM group's number of SMs is not a multiple of four, SMs are left over
+  const F8Pick k = f8_kernel<F8_PLAIN>(F8S_ROWS);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(4 * F8_MAX_CTAS); cfg.blockDim = dim3(F8_THREADS); cfg.dynamicSmemBytes = (size_t)k.smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 4; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  HB_CUDA(ctx, cudaOccupancyMaxActiveClusters(&ctx->fp8_clusters, reinterpret_cast<const void*>(k.fn), &cfg));
   return HB_OK;
 }
 
@@ -330,7 +360,7 @@ int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t*
   return hb_launch(ctx, "fp8_quantize", false, fp8_quantize_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float*>(w), N, K, q, s);
 }
 
-size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M <= 16 ? 16 : M <= 32 ? 32 : F8P_ROWS) : 0; }
+size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M <= 16 ? 16 : M <= F8S_ROWS ? 32 : F8P_ROWS) : 0; }
 
 int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb, float* yf, int ldy, void* ws, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
@@ -343,7 +373,8 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "fp8_gemm: ws NULL or not 256-byte aligned");
-  const int rows = f8_rows_for(ctx, M, (W->N + 255) / 256), nt = (M + rows - 1) / rows;
+  const F8Cut cut = f8_cut(ctx, M, W->N, W->K);
+  const int rows = cut.rows, nt = (M + rows - 1) / rows;
   F8Args a{};
   a.M = M; a.per = rows == F8P_ROWS ? rows : ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
   HB_REQUIRE(ctx, (long long)nt * a.n_nt < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d", M, W->N);
@@ -351,6 +382,7 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.count = f8_counters(ctx); a.err = ctx->dev_err;
   CUtensorMap tw, tx;
   const bool many = rows >= F8S_ROWS;
+  a.split = cut.split;
   int r;
   if ((r = f8_map(ctx, &tw, W->w, W->K, W->K, W->N, many ? 64 : 128)) || (r = f8_map(ctx, &tx, xq, W->K, ldq, M, many ? 128 : rows))) return r;
   return f8_launch<F8_PLAIN>(ctx, "fp8_gemm", rows, a, tw, tx, reinterpret_cast<cudaStream_t>(stream));
@@ -410,6 +442,7 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.maps = W.maps;
   a.xs = W.xs; a.lds = P; a.yq = W.yq; a.ys = W.ys; a.ldys = P;
   if (own_plan) a.plan = pr.plan;
+  a.split = 2;                                                                 // (all SMs are in reach of clusters of two)
   if ((r = f8_launch<F8_GU>(ctx, "fp8_gemm_gu", rows, a, tg, tx, st))) return r;
   a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.maps = W.maps + (size_t)F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap);
   a.xs = W.ys; a.yb = W.part; a.ldy = H;

@@ -133,6 +133,13 @@ def test_gemm(E, M, N, K, dt):
     assert not bad.any(), (bad.sum().item(), bad.nonzero()[:4].tolist(), ((y.double() - y0).abs() / (a + 1e-300)).max().item())
 
 
+# items split among two and four CTAs, behind whole rounds and without any, over a K that does not divide; pairs' items cut through the workspace
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,N,K", [(33, 300, 4096), (70, 1100, 2192), (128, 5000, 4112), (300, 2900, 2320), (150, 20000, 2304), (300, 15000, 2176), (512, 1281, 9216)])
+def test_gemm_split_items(E, M, N, K, dt):
+    test_gemm(E, M, N, K, dt)
+
+
 def test_gemm_strides_and_what_lies_around(E):
     import torch
     M, N, K = 37, 201, 336
