@@ -57,17 +57,10 @@ def _empty(rows: int, cols: int, dtype):
 
 
 def _out(t, rows_: int, cols: int, dtype, rows: bool = False):
-    """The given output, which has to have this type and room for these rows (contiguous, or with rows= contiguous rows), or a new one."""
-    if t is None:
-        return _empty(rows_, cols, dtype)
+    """The given output: it has to have this type and room for these rows (contiguous, or with rows= contiguous rows)."""
     if not (t.dtype == dtype and t.shape[0] >= rows_ and t.shape[1] == cols and (rows or t.is_contiguous())):
         raise HbError(-1, f"output {tuple(t.shape)} {t.dtype}: {(rows_, cols)} {dtype} wanted")
     return t
-
-
-def _need(*conditions):
-    if not all(conditions):
-        raise HbError(-1, "shape, type or layout of an argument")
 
 
 def _bytes(n: int):
@@ -255,11 +248,13 @@ def router_grouped_topk(logits: torch.Tensor, k: int, n_group: int = 1, topk_gro
     score + bias, weights from the score alone.  logits fp32 [M, ld]; returns ids int32 [M, k], w fp32 [M, k]."""
     ctx, st = _here(logits, ctx)
     M, cols = logits.shape
-    _need(logits.dtype == torch.float32, bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() >= (cols if E is None else E)), E is None or E <= cols)
-    ids = _out(ids, M, k, torch.int32)
-    w = _out(w, M, k, torch.float32)
+    E = cols if E is None else E
+    if logits.dtype is not torch.float32 or E > cols or (bias is not None and (bias.dtype is not torch.float32 or bias.numel() < E or not bias.is_contiguous())):
+        raise HbError(-1, "logits and bias have to be fp32, the bias contiguous, with a value for every expert")
+    ids = _empty(M, k, torch.int32) if ids is None else _out(ids, M, k, torch.int32)
+    w = _empty(M, k, torch.float32) if w is None else _out(w, M, k, torch.float32)
     lp, ld = _row_ptr(logits)
-    ctx.check(_L().hb_route_grouped_topk(ctx.handle, lp, ld, M, cols if E is None else E, k, n_group, topk_group, group_top, _SCORE[score],
+    ctx.check(_L().hb_route_grouped_topk(ctx.handle, lp, ld, M, E, k, n_group, topk_group, group_top, _SCORE[score],
                                          None if bias is None else bias.data_ptr(), renorm, scale, ids.data_ptr(), w.data_ptr(), st))
     return ids, w
 
@@ -453,8 +448,8 @@ def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     ctx, st = _here(x, ctx)
     assert x.dtype == torch.bfloat16
     M, K = x.shape
-    q = _out(q, M, K, torch.uint8, rows=True)
-    s = _out(s, -(-K // 128), M, torch.float32, rows=True)
+    q = _empty(M, K, torch.uint8) if q is None else _out(q, M, K, torch.uint8, rows=True)
+    s = _empty(-(-K // 128), M, torch.float32) if s is None else _out(s, -(-K // 128), M, torch.float32, rows=True)
     ctx.check(_L().hb_fp8_quant_rows(ctx.handle, *_row_ptr(x), M, K, *_row_ptr(q), *_row_ptr(s), st))
     return q, s
 
@@ -465,8 +460,8 @@ def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     bf16 = w.dtype == torch.bfloat16
     assert (bf16 or w.dtype == torch.float32) and w.is_contiguous()
     N, K = w.shape
-    q = _out(q, N, K, torch.uint8)
-    s = _out(s, -(-N // 128), -(-K // 128), torch.float32)
+    q = _empty(N, K, torch.uint8) if q is None else _out(q, N, K, torch.uint8)
+    s = _empty(-(-N // 128), -(-K // 128), torch.float32) if s is None else _out(s, -(-N // 128), -(-K // 128), torch.float32)
     ctx.check(_L().hb_fp8_quantize(ctx.handle, w.data_ptr(), bf16, N, K, q.data_ptr(), s.data_ptr(), st))
     return q, s
 
@@ -475,14 +470,19 @@ def fp8_gemm_ws_bytes(M: int, N: int, K: int) -> int:
     return int(_L().hb_fp8_gemm_ws_bytes(M, N, K))
 
 
+_FP8_OUT = (torch.bfloat16, torch.float32)
+
+
 def fp8_gemm(W: GMat, xq, xs, out_dtype=torch.bfloat16, y=None, ws=None, ctx: Context | None = None):
     """hb_fp8_gemm: y [M, N] (bf16 or fp32) = rows quantised by fp8_quant_rows times the block-scaled matrix W (FMT_FP8_B128)."""
     ctx, st = _here(xq, ctx)
     L = _L()
     M = xq.shape[0]
-    out_dtype = out_dtype if y is None else y.dtype
-    _need(out_dtype in (torch.bfloat16, torch.float32), xq.element_size() == 1, xs.dtype == torch.float32, xq.shape[1] >= W.K, xs.shape[0] >= -(-W.K // 128))
-    y = _out(y, M, W.N, out_dtype, rows=True)
+    if y is not None:
+        out_dtype = y.dtype
+    if out_dtype not in _FP8_OUT or xq.element_size() != 1 or xs.dtype is not torch.float32 or xq.shape[1] < W.K or xs.shape[0] * 128 < W.K:
+        raise HbError(-1, "codes [M, K] of one byte, scales fp32 [ceil(K/128), M], result bf16 or fp32")
+    y = _empty(M, W.N, out_dtype) if y is None else _out(y, M, W.N, out_dtype, rows=True)
     ws = _bytes(L.hb_fp8_gemm_ws_bytes(M, W.N, W.K)) if ws is None else ws
     yp, ldy = _row_ptr(y)
     yb, yf = (yp, None) if y.dtype == torch.bfloat16 else (None, yp)
@@ -526,11 +526,14 @@ def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg
     ctx, st = _here(x, ctx)
     L = _L()
     M, K = ids.shape
-    out_dtype = out_dtype if out is None else out.dtype
-    _need(out_dtype in (torch.bfloat16, torch.float32), ids.dtype == torch.int32, w.dtype == torch.float32, x.dtype == torch.bfloat16, rec_tab.dtype == torch.int64,
-          w.shape == ids.shape, x.shape == (M, H), rec_tab.numel() >= (li + 1) * E, x.is_contiguous(), ids.is_contiguous(), w.is_contiguous(),
-          shared is None or (shared.dtype == torch.bfloat16 and shared.shape == (M, H) and shared.is_contiguous()), lg is None or (lg.dtype == torch.float32 and lg.shape[0] == M))
-    out = _out(out, M, H, out_dtype)
+    if out is not None:
+        out_dtype = out.dtype
+    if (out_dtype not in _FP8_OUT or ids.dtype is not torch.int32 or w.dtype is not torch.float32 or x.dtype is not torch.bfloat16 or rec_tab.dtype is not torch.int64
+            or w.shape != ids.shape or x.shape != (M, H) or rec_tab.numel() < (li + 1) * E or not (x.is_contiguous() and ids.is_contiguous() and w.is_contiguous())
+            or (shared is not None and (shared.dtype is not torch.bfloat16 or shared.shape != (M, H) or not shared.is_contiguous()))
+            or (lg is not None and (lg.dtype is not torch.float32 or lg.shape[0] != M))):
+        raise HbError(-1, "ids int32 and w fp32 [M, K], x and shared bf16 [M, H], lg fp32 [M, ·], rec_tab int64 with li + 1 layers, all contiguous, result bf16 or fp32")
+    out = _empty(M, H, out_dtype) if out is None else _out(out, M, H, out_dtype)
     ws = _bytes(L.hb_moe_fp8_ws_bytes(M, K, E, H, I)) if ws is None else ws
     op, cmb = out.data_ptr(), None
     if out.dtype == torch.bfloat16:
