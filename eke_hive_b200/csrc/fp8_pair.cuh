@@ -24,6 +24,7 @@
 namespace hb {
 
 constexpr int F8S_ROWS = 128, F8P_ROWS = 256;          // rows of x a tile may have: one CTA, a pair
+constexpr int F8M_GROUP = 16;                          // tiles of rows that are gone through together
 constexpr uint32_t F8S_WHOLE = 16;                     // steps up to which an item of single CTAs stays whole: putting its sums together takes some 8 (two CTAs) or 12 (four)
 constexpr uint32_t F8P_SLACK = 40;                     // steps that cutting has to save: leaving and adding up parts takes a pair some 20 us
 // Steps of a CTA of the one-CTA form: rounds of whole items, then the items left over, each split among the CTAs of a cluster where there are enough clusters.
@@ -150,6 +151,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
     if (MODE != F8_PLAIN) return a.tiles[ti];
     return TileRef{ti * a.per, min(a.per, a.M - ti * a.per), 0};
   };
+  // Item → tile of rows, 256 weight rows.  Dense: the row tiles (in groups of 16) go by faster, so that the CTAs of a round share weights as well as rows of x and
+  // each comes from memory about once.  (Weights faster: 2048 rows of 17408 x 5120 read 577 MB, 203 us; this way 100 MB, all there is, 177.)
+  auto place = [&](int item, int& ti, int& nt) {
+    if (MODE != F8_PLAIN) { ti = item / a.n_nt; nt = item - ti * a.n_nt; return; }
+    const int g = item / (F8M_GROUP * a.n_nt), r = item - g * (F8M_GROUP * a.n_nt), gs = min(F8M_GROUP, n_tiles - g * F8M_GROUP);
+    nt = r / gs; ti = g * F8M_GROUP + r - nt * gs;
+  };
   int item, kb0, kb1;
 
   if (warp >= 8) {
@@ -162,7 +170,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
         const uint32_t full0 = PAIR ? mapa_u32(smem_u32(full), 0) : 0u;
         while (ok && sch.next(item, kb0, kb1)) {
-          const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
+          int ti, nt;
+          place(item, ti, nt);
           const TileRef tl = tile_of(ti);
           const void* mw = MODE == F8_PLAIN ? &tmW : maps.make(tmW, a.tab, tl.expert, a.off_w, a.err);
           // rows of each half, in boxes of 64: of a pair each CTA loads one, else both are this CTA's.  Rows past the last read as zero codes
@@ -245,7 +254,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
     uint32_t it = 0;
     bool ok = true;
     while (sch.next(item, kb0, kb1)) {                                          // after a wait that gave up: on to the end without waits and results, but through every barrier
-      const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
+      int ti, nt;
+      place(item, ti, nt);
       const TileRef tl = tile_of(ti);
       const int rows = min(max(tl.rows - 128 * (int)rank, 0), 128);            // of this CTA
       const size_t slot0 = (size_t)tl.slot0 + 128 * rank;
