@@ -252,7 +252,8 @@ size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows ==
 // How a dense product is cut.  Up to 32 rows a weight row a lane (17408 x 5120, 32 rows: 24 us; a row of x a lane: 28).  More: a row of x a lane, tiles of 128 rows
 // of single CTAs or of 256 of pairs, by the steps the longest CTA takes.  Single: rounds of whole items, what is left over split among the two or four
 // CTAs of a cluster where there are that many, at the price of some 8 and 12 steps (128 rows of 4096 x 4096: 21 us whole, 17 in two, 15 in four; 2048 x 512: 6.4, 9.3, 10.3).
-// Pairs: a step takes less, as an SM pulls less out of L2, but what is left over is cut through the workspace.
+// Pairs: a step takes a tenth less, as an SM pulls less out of L2 (512 rows of 18944 x 4096: 42 us, single CTAs 44; 5120 x 17408, where half the pairs' work is left over
+// and cut through the workspace: 62 and 74; 2048 rows of 5120 x 5120, split in two: 65 and 63).
 struct F8Cut { int rows, split; };
 F8Cut f8_cut(const hb_ctx* ctx, int M, int N, int K) {
   if (M <= 32) return {M <= 16 ? 16 : 32, 1};
@@ -271,8 +272,8 @@ F8Cut f8_cut(const hb_ctx* ctx, int M, int N, int K) {
 }
 // Pairs of a tile by what an expert gets on average: longer runs are cut into tiles, which read the expert's weights again, and a tile that is not full
 // wastes its MMAs.  Gate/up + down of 512 experts of 2048 / 512: 20 pairs an expert 310 us with 32, 359 with 128 (39 pairs: 476, 375; 10 pairs: 294, and 293
-// with 16).  A pair of CTAs gains nothing here: 32 experts of 7168 / 2048, 256 pairs an expert, 533 us with 128, 661 with 256, half of whose second tiles are
-// empty; 8 experts of 4096 / 1536, 2048 pairs: 399, 439.
+// with 16).  Pairs of CTAs gained nothing here (32 experts of 7168 / 2048, 256 pairs an expert: 533 us with 128, 661 with 256, half of whose second tiles were
+// empty; 8 experts of 4096 / 1536, 2048 pairs: 399, 439), so routed experts have no such form.
 int f8_rows_for_pairs(long long P, int E) { return P <= 8ll * E ? 16 : P <= 24ll * E ? 32 : F8S_ROWS; }
 // map of a byte matrix [n_rows][row_bytes], rows ld bytes apart, in boxes of 128 bytes × box_rows under the 128-byte swizzle; bytes and rows past the
 // end read as zero codes
