@@ -311,6 +311,39 @@ def test_few_ctas_and_many(E):
             ctx.check_device()
 
 
+def test_two_contexts_at_once(E):
+    """Calls on two streams, a context each: counters and workspaces are their own."""
+    import torch
+    N, K, H, I, Ex = 5120, 4096, 512, 256, 8
+    W = [E.GMat(E.FMT_FP8_B128, N, K, *matrix(N, K, i)) for i in range(2)]
+    recs = [record(E, H, I, 10 * e)[0] for e in range(Ex)]                              # (the table holds addresses: the records have to stay)
+    tab = E.rec_table(recs)
+    jobs = []
+    for i, M in enumerate((5, 9, 300, 520)):
+        x = rows(M, K, i)
+        xq, xs = E.fp8_quant_rows(x)
+        xe = torch.randn(M, H, device="cuda", generator=gen(i)).to(torch.bfloat16)
+        jobs.append((W[i % 2], xq, xs, *routing(M, 2, Ex, i), xe))
+
+    def run(j, ctx=None):
+        w, xq, xs, ids, wt, xe = j
+        return E.fp8_gemm(w, xq, xs, ctx=ctx), E.moe_fp8(ids, wt, tab, 0, Ex, xe, H, I, ctx=ctx)
+    ref = [run(j) for j in jobs]
+    streams, ctxs = [torch.cuda.Stream() for _ in range(2)], [E.Context() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for i in range(len(jobs)):
+            for s in range(2):
+                with torch.cuda.stream(streams[s]):
+                    got.append(((i + s) % len(jobs), run(jobs[(i + s) % len(jobs)], ctxs[s])))
+        torch.cuda.synchronize()
+        for i, g in got:
+            assert all(torch.equal(a, b) for a, b in zip(g, ref[i])), i
+    for c in ctxs:
+        c.check_device()
+
+
 def test_gemm_matrix_beyond_32_bits(E):
     """Rows of a weight, and rows of x, more than 2^32 bytes from their first."""
     import torch
