@@ -156,7 +156,7 @@ struct F8Args {
 };
 
 // Tensor maps of expert records, made by the thread that loads through them: a record's address is known on the device only, and the map of a matrix
-// is one map for all experts but for its address.  A CTA's slots go round; one is written again when F8_MAPS items, of at least one stage each, have gone by, more
+// is one map for all experts but for its address.  A CTA's slots go round; one is written again when F8_MAPS maps, of at least one stage each, have gone by, more
 // than there are stages: what was loaded through it has been multiplied.
 constexpr int F8_MAPS = 8;
 // A record has to lie at a 16-byte boundary.  One that does not is read from the boundary in front of it, where no load faults, and reported (0x400000).
@@ -164,11 +164,13 @@ __device__ __forceinline__ const uint8_t* f8_rec(const uint8_t* const* tab, int 
   return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(tab[expert]) & ~(uintptr_t)15);
 }
 struct F8Maps {
-  uint8_t* slots; uint32_t n;
+  uint8_t* slots; uint32_t n; int last; uint8_t* to;    // last: the expert that the newest map is of
   __device__ __forceinline__ const void* make(const CUtensorMap& tpl, const uint8_t* const* tab, int expert, uint64_t off, uint32_t* err) {
+    if (expert == last) return to;                       // a CTA stays with an expert for some items; making a map takes as long as a few steps
+    last = expert;
     const uint8_t* addr = f8_rec(tab, expert) + off;
     if (reinterpret_cast<uintptr_t>(tab[expert]) & 15u) atomicOr(err, 0x400000u);
-    uint8_t* to = slots + (size_t)(n++ % F8_MAPS) * sizeof(CUtensorMap);
+    to = slots + (size_t)(n++ % F8_MAPS) * sizeof(CUtensorMap);
     const uint4* from = reinterpret_cast<const uint4*>(&tpl);
 #pragma unroll
     for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(to)[j] = from[j];
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     if (elect_one()) {
       uint32_t s = 0, ph = 1;
       bool ok = true, waited = false;
-      F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
+      F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u, -1, nullptr};
       while (ok && sch.next(item, kb0, kb1)) {
         const int ti = item / a.n_nt, nt = item - ti * a.n_nt;
         const TileRef tl = tile_of(ti);

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
       if (elect_one()) {
         uint32_t s = 0, ph = 1;
         bool ok = true, waited = false;
-        F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u};
+        F8Maps maps{a.maps + (size_t)blockIdx.x * F8_MAPS * sizeof(CUtensorMap), 0u, -1, nullptr};
         const uint32_t full0 = PAIR ? mapa_u32(smem_u32(full), 0) : 0u;
         while (ok && sch.next(item, kb0, kb1)) {
           int ti, nt;
