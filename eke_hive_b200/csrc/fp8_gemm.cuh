@@ -297,8 +297,10 @@ __device__ __forceinline__ void f8_ld(uint32_t taddr, uint32_t (&r)[W]) {
   else tc_ld8(taddr, r);
 }
 
+// Registers: with 16 rows a tile 128 a thread are enough and leave room on the SM for a block of the small kernel behind this one, which then starts without waiting
+// for it to leave (16 rows over 512 experts: 106 us with 168, 103.5; one row of 5120 x 17408 behind its quantiser 26 and 25; with 32 rows a tile they spill, 24.4 and 27.6).
 template <int BN, int MODE>
-__global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
+__global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ F8Args a, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX) {
   using C = F8Cfg<BN>;
   extern __shared__ uint8_t f8_raw[];
   const uint32_t raw = smem_u32(f8_raw), base = (raw + 1023u) & ~1023u;
@@ -524,24 +526,28 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_gemm_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < C::CW; ++c) acc[0][c] = acc[1][c] = 0.f;
         // parts and columns fetched together; a value's parts are added in order
-        constexpr int NP = C::CW <= 8 ? 8 : 2;
+        constexpr int NP = C::CW <= 8 ? 8 : 2, GC = C::CW <= 8 ? 4 : C::CW;
         const float* first = part_of(c_first, sch.start(c_first));
         const float* rest = part_of(c_first, s0);                              // the later CTAs' parts are their first ones: 2 · 256 · BN apart
-        for (uint32_t cc = c_first; cc <= c_last && active; cc += NP) {
-          float t[NP][2][C::CW];
+        for (uint32_t cc = c_first; cc <= c_last; cc += NP) {
 #pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const float* p = cc + i == c_first ? first : rest + (size_t)(cc + i - c_first) * (2 * 256 * BN);
+          for (int g = 0; g < C::CW; g += GC) {
+            if (g >= cols) break;
+            float t[NP][2][GC];
 #pragma unroll
-            for (int c = 0; c < C::CW; ++c) {
-              const bool on = c < cols && cc + i <= c_last;
-              t[i][0][c] = on ? __ldcg(p + c * 256) : 0.f; t[i][1][c] = on ? __ldcg(p + c * 256 + 128) : 0.f;
+            for (int i = 0; i < NP; ++i) {
+              const float* p = cc + i == c_first ? first : rest + (size_t)(cc + i - c_first) * (2 * 256 * BN);
+#pragma unroll
+              for (int c = 0; c < GC; ++c) {
+                const bool on = g + c < cols && cc + i <= c_last;
+                t[i][0][c] = on ? __ldcg(p + (g + c) * 256) : 0.f; t[i][1][c] = on ? __ldcg(p + (g + c) * 256 + 128) : 0.f;
+              }
             }
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+              for (int c = 0; c < GC; ++c) { acc[0][g + c] += t[i][0][c]; acc[1][g + c] += t[i][1][c]; }
           }
-#pragma unroll
-          for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int c = 0; c < C::CW; ++c) { acc[0][c] += t[i][0][c]; acc[1][c] += t[i][1][c]; }
         }
       }
       // ---- the item's results
