@@ -2,8 +2,8 @@
 // tile of 128 rows.
 //
 // Rows of x are the A operand, 128 of them in each CTA's shared and tensor memory; the weight rows are the B operand, of which each CTA of a pair loads half
-// and both read all: 32 KB of operands per CTA and step for 128 × 256 × 128 multiply-adds.  (One CTA alone needs 48 KB for them, and the SMs pull no more than
-// some 10 TB/s out of L2: 4096 rows of 17408 x 5120 take 368 us with single CTAs, 338 with pairs.  That form is for runs of rows that would leave much of a
+// and both read all: 32 KB of operands per CTA and step for 128 × 256 × 128 multiply-adds.  (One CTA alone needs 48 KB for them, which is 11.6 TB/s out of L2 at
+// the rate it reaches: 4096 rows of 17408 x 5120 take 368 us with single CTAs, 338 with pairs.  That form is for runs of rows that would leave much of a
 // pair's tile empty, and where there are few items.)  A lane of tensor memory is a row of x: the scale of a step is one number a thread, the row's times the
 // weight block's.
 //
