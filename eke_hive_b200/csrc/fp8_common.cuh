@@ -2,12 +2,10 @@
 #pragma once
 #include <cuda_fp8.h>
 
+#include "fp8_cut.h"
 #include "hb_common.cuh"
 
 namespace hb {
-
-constexpr int F8_B = 128;                              // values a scale covers
-__host__ __device__ constexpr int f8_blocks(int n) { return (n + F8_B - 1) / F8_B; }
 
 // ---- quantisation -------------------------------------------------------------------------------------------------------------------
 // The largest magnitude of a block as the bits of a float: they order like the magnitudes, infinities and NaN last.  From it the scale that

@@ -28,7 +28,6 @@ namespace hb {
 
 enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
 
-constexpr int F8_MAX_CTAS = 160;                       // grid at most; the workspace holds two partial items of each
 constexpr int F8_COUNTERS = F8_MAX_CTAS;               // items that are cut, at most: a CTA's last one
 constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
 // Plan of a short list of pairs (at most F8_PLAN_PAIRS), worked out by every CTA that needs it for itself: a pair's slot is the number of pairs with a smaller
@@ -152,6 +151,7 @@ struct F8Args {
   __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN
   uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
   float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256]; arrivals, by the CTA of an item's first step (zero before and after)
+  uint32_t room;                                       // of part, in sums: range checks of the debug build
   uint32_t* err;
 };
 
@@ -179,38 +179,6 @@ struct F8Maps {
     tmap_acquire(to);
     return to;
   }
-};
-
-// The steps of a CTA, the same for all its warps: segments (item, first step, end).
-struct F8Sched {                                       // (32 bits: at most 320 items of at most 2^16 steps, or 2^24 steps, times 160 CTAs)
-  uint32_t KB, G, me, dp, sk, U, Gs, end, u, u1, i;
-  // runs: no rounds, the whole list in equal runs (as long as its steps can be counted so): a CTA stays with an expert.  Else rounds, and of what they leave over
-  // items are cut where that saves more than `slack` steps
-  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool runs, uint32_t slack) {
-    KB = KB_; G = G_; me = me_;
-    const uint32_t waves = items / G, rem = items - waves * G;
-    const bool all = runs && (unsigned long long)items * KB < (1ull << 24);
-    const bool cut = rem != 0u && (unsigned long long)(G - rem) * KB > (unsigned long long)slack * G;
-    dp = all ? 0u : !cut ? waves + (rem != 0u) : waves > 0u ? waves - 1u : 0u;   // rounds of whole items, after the cut ones
-    sk = all || cut ? items - dp * G : 0u;
-    U = sk * KB; end = items;
-    Gs = min(G, max(U, 1u));                                                   // CTAs that get a run of steps: none is empty
-    u = start(me); u1 = start(me + 1u);
-    i = 0u;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t c) const { return c >= Gs ? U : c * U / Gs; }
-  __device__ __forceinline__ bool next(int& item, int& kb0, int& kb1) {
-    if (u < u1) {
-      item = (int)(u / KB); kb0 = (int)(u - (uint32_t)item * KB);
-      kb1 = (int)min(KB, kb0 + (u1 - u));
-      u += (uint32_t)(kb1 - kb0);
-      return true;
-    }
-    if (i >= dp) return false;
-    item = (int)(sk + i * G + me); kb0 = 0; kb1 = (int)KB; ++i;
-    return (uint32_t)item < end;
-  }
-  __device__ __forceinline__ uint32_t owner(uint32_t step) const { return ((step + 1u) * Gs - 1u) / U; }
 };
 
 __device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int c0, int c1) {
@@ -509,7 +477,9 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
         float* mine = part_of(blockIdx.x, sch.start(blockIdx.x));
 #pragma unroll
         for (int c = 0; c < C::CW; ++c)
-          if (active && c < cols) { __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]); }
+          if (active && c < cols && HB_BOUND(a.err, (size_t)(mine - a.part) + c * 256 + 128 < a.room, 0x801u, mine - a.part)) {
+            __stcg(mine + c * 256, acc[0][c]); __stcg(mine + c * 256 + 128, acc[1][c]);
+          }
         named_bar_sync(1, 256);
         if (threadIdx.x == 0 && !ok) *last = 0u;
         else if (threadIdx.x == 0) {

@@ -23,29 +23,7 @@
 
 namespace hb {
 
-constexpr int F8S_ROWS = 128, F8P_ROWS = 256;          // rows of x a tile may have: one CTA, a pair
 constexpr int F8M_GROUP = 16;                          // tiles of rows that are gone through together
-constexpr uint32_t F8S_WHOLE = 16;                     // steps up to which an item of single CTAs stays whole: putting its sums together takes some 8 (two CTAs) or 12 (four)
-constexpr uint32_t F8P_SLACK = 40;                     // steps that cutting has to save: leaving and adding up parts takes a pair some 20 us
-// Steps of a CTA of the one-CTA form: rounds of whole items, then the items left over, each split among the CTAs of a cluster where there are enough clusters.
-struct F8Rounds {
-  uint32_t KB, G, me, dp, rem, split, i;
-  __device__ __forceinline__ void init(uint32_t items, uint32_t KB_, uint32_t G_, uint32_t me_, bool, uint32_t cluster) {
-    KB = KB_; G = G_; me = me_;
-    dp = items / G; rem = items - dp * G;
-    split = rem * cluster <= G && KB > F8S_WHOLE ? cluster : 1u;
-    i = 0u;
-  }
-  __device__ __forceinline__ bool splits() const { return split > 1u && me / split < rem; }   // the same for all CTAs of a cluster
-  __device__ __forceinline__ bool next(int& item, int& kb0, int& kb1) {
-    if (i > dp) return false;
-    if (i++ < dp) { item = (int)((i - 1u) * G + me); kb0 = 0; kb1 = (int)KB; return true; }
-    const uint32_t t = me / split, r = me - t * split;
-    if (t >= rem) return false;
-    item = (int)(dp * G + t); kb0 = (int)(KB * r / split); kb1 = (int)(KB * (r + 1u) / split);
-    return true;
-  }
-};
 template <bool PAIR>
 struct F8PCfg {
   static constexpr int CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS;
@@ -366,7 +344,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         // a part: [column][half][row]; a pair's first run is its part 0
         auto part_of = [&](uint32_t c, uint32_t st) { return a.part + ((size_t)(C::CTAS * c + rank) * 2 + (c == c_first && st != st0 ? 1 : 0)) * (256 * 128) + h * 128 + row; };
         float* mine = part_of(sch.me, sch.start(sch.me));
-        if (active) {
+        if (active && HB_BOUND(a.err, (size_t)(mine - a.part) + 127 * 256 < a.room, 0x802u, mine - a.part)) {
 #pragma unroll
           for (int c = 0; c < 128; ++c) __stcg(mine + c * 256, acc[c]);
         }

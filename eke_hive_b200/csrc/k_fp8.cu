@@ -237,41 +237,12 @@ F8Pick f8_kernel(int rows) {
     default: return {fp8_many_kernel<F8_PLAIN, true>, F8PCfg<true>::SMEM};
   }
 }
-// CTAs of a launch: one an SM, in whole clusters of cl.  Not all SMs are in reach of clusters of four.
-int f8_grid(const hb_ctx* ctx, int rows, int cl) {
-  int n = ctx->max_ctas > 0 && ctx->max_ctas < ctx->sm_count ? ctx->max_ctas : ctx->sm_count;
-  if (n > F8_MAX_CTAS) n = F8_MAX_CTAS;
-  if (cl == 4 && rows == F8S_ROWS && n > 4 * ctx->fp8_clusters) n = 4 * ctx->fp8_clusters;
-  return n < cl ? cl : n / cl * cl;
-}
+F8Gpu f8_gpu(const hb_ctx* ctx) { return {ctx->sm_count, ctx->max_ctas, ctx->fp8_clusters}; }
 template <int MODE>
 int f8_launch(hb_ctx* ctx, const char* name, int rows, const F8Args& a, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t st) {
   const F8Pick k = f8_kernel<MODE>(rows);
   const int cl = rows == F8P_ROWS ? 2 : rows == F8S_ROWS ? a.split : 1;
-  return hb_launch_cluster(ctx, name, true, cl, k.fn, dim3(f8_grid(ctx, rows, cl)), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
-}
-// sums of cut items: two of each CTA.  (A row of x a lane: in pairs alone.)
-size_t f8_part_bytes(int rows) { return (size_t)F8_MAX_CTAS * 2 * 256 * (rows == F8P_ROWS ? 128 : rows == F8S_ROWS ? 32 : rows) * 4; }
-// How a dense product is cut.  Up to 32 rows a weight row a lane (17408 x 5120, 32 rows: 24 us; a row of x a lane: 28).  More: a row of x a lane, tiles of 128 rows
-// of single CTAs or of 256 of pairs, by the steps the longest CTA takes.  Single: rounds of whole items, what is left over split among the two or four
-// CTAs of a cluster where there are that many, at the price of some 8 and 12 steps (128 rows of 4096 x 4096: 21 us whole, 17 in two, 15 in four; 2048 x 512: 6.4, 9.3, 10.3).
-// Pairs: a step takes a tenth less, as an SM pulls less out of L2 (512 rows of 18944 x 4096: 42 us, single CTAs 44; 5120 x 17408, where half the pairs' work is left over
-// and cut through the workspace: 62 and 74; 2048 rows of 5120 x 5120, split in two: 65 and 63).
-struct F8Cut { int rows, split; };
-F8Cut f8_cut(const hb_ctx* ctx, int M, int N, int K) {
-  if (M <= 32) return {M <= 16 ? 16 : 32, 1};
-  const long long KB = f8_blocks(K), n_nt = (N + 255) / 256;
-  F8Cut best{F8S_ROWS, 1};
-  long long least = 0;
-  for (int c : {1, 2, 4}) {
-    const long long G = f8_grid(ctx, F8S_ROWS, c), items = (M + F8S_ROWS - 1) / F8S_ROWS * n_nt, rem = items % G;
-    if (c > 1 && (rem * c > G || KB <= F8S_WHOLE)) continue;
-    const long long steps = items / G * KB + (rem == 0 ? 0 : c == 1 ? KB : (KB + c - 1) / c + (c == 2 ? 8 : 12));
-    if (c == 1 || steps < least) { least = steps; best.split = c; }
-  }
-  const long long G = f8_grid(ctx, F8P_ROWS, 2) / 2, items = (M + F8P_ROWS - 1) / F8P_ROWS * n_nt, rem = items % G, cut = (KB * rem + G - 1) / G + F8P_SLACK;
-  const long long steps = items / G * KB + (rem == 0 ? 0 : cut < KB ? cut : KB);
-  return 9 * steps < 10 * least ? F8Cut{F8P_ROWS, 2} : best;
+  return hb_launch_cluster(ctx, name, true, cl, k.fn, dim3(f8_grid(f8_gpu(ctx), rows, cl)), dim3(F8_THREADS), (size_t)k.smem, st, a, w, x);
 }
 // Pairs of a tile by what an expert gets on average: longer runs are cut into tiles, which read the expert's weights again, and a tile that is not full
 // wastes its MMAs.  Gate/up + down of 512 experts of 2048 / 512: 20 pairs an expert 310 us with 32, 359 with 128 (39 pairs: 476, 375; 10 pairs: 294, and 293
@@ -364,7 +335,7 @@ int hb_fp8_quantize(hb_ctx* ctx, const void* w, int bf16, int N, int K, uint8_t*
   return hb_launch(ctx, "fp8_quantize", false, fp8_quantize_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float*>(w), N, K, q, s);
 }
 
-size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(M <= 16 ? 16 : M <= F8S_ROWS ? 32 : F8P_ROWS) : 0; }
+size_t hb_fp8_gemm_ws_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? f8_part_bytes(f8_most_rows(M)) : 0; }
 
 int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const float* xs, int lds, int M, void* yb, float* yf, int ldy, void* ws, void* stream) {
   if (!ctx) return HB_ERR_INVALID;
@@ -377,13 +348,13 @@ int hb_fp8_gemm(hb_ctx* ctx, const hb_qmat* W, const uint8_t* xq, int ldq, const
   HB_REQUIRE(ctx, hb_aligned(W->w, 16) && hb_aligned(xq, 16) && hb_aligned(W->s, 4) && hb_aligned(xs, 4) && hb_aligned(yb, 2) && hb_aligned(yf, 4), HB_ERR_INVALID,
              "fp8_gemm: codes must be 16-byte aligned, scales and outputs to their elements");
   HB_REQUIRE(ctx, ws && hb_aligned(ws, 256), HB_ERR_WORKSPACE, "fp8_gemm: ws NULL or not 256-byte aligned");
-  const F8Cut cut = f8_cut(ctx, M, W->N, W->K);
+  const F8Cut cut = f8_cut(f8_gpu(ctx), M, W->N, W->K);
   const int rows = cut.rows, nt = (M + rows - 1) / rows;
   F8Args a{};
   a.M = M; a.per = rows == F8P_ROWS ? rows : ((M + nt - 1) / nt + 15) & ~15; a.N = W->N; a.K = W->K; a.n_nt = (W->N + 255) / 256;
   HB_REQUIRE(ctx, (long long)nt * a.n_nt < (1ll << 31), HB_ERR_UNSUPPORTED, "fp8_gemm: M=%d N=%d", M, W->N);
   a.ws = reinterpret_cast<const float*>(W->s); a.xs = xs; a.lds = lds;
-  a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.count = f8_counters(ctx); a.err = ctx->dev_err;
+  a.yb = reinterpret_cast<__nv_bfloat16*>(yb); a.yf = yf; a.ldy = ldy; a.part = reinterpret_cast<float*>(ws); a.room = (uint32_t)(f8_part_bytes(f8_most_rows(M)) / 4); a.count = f8_counters(ctx); a.err = ctx->dev_err;
   CUtensorMap tw, tx;
   const bool many = rows >= F8S_ROWS;
   a.split = cut.split;
@@ -442,7 +413,7 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
     if ((r = f8_rows(ctx, q, st))) return r;
   }
   F8Args a{};
-  a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.count = f8_counters(ctx); a.err = ctx->dev_err;
+  a.tiles = W.tiles; a.n_tiles = W.n_tiles; a.tab = tab; a.limit = limit; a.part = W.cut; a.room = (uint32_t)(f8_part_bytes(rows) / 4); a.count = f8_counters(ctx); a.err = ctx->dev_err;
   a.N = I; a.K = H; a.n_nt = I / 128; a.off_w = L.w1; a.off_s0 = L.s1; a.off_s1 = L.s3; a.row2 = I; a.maps = W.maps;
   a.xs = W.xs; a.lds = P; a.yq = W.yq; a.ys = W.ys; a.ldys = P;
   if (own_plan) a.plan = pr.plan;

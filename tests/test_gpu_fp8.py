@@ -140,6 +140,24 @@ def test_gemm_split_items(E, M, N, K, dt):
     test_gemm(E, M, N, K, dt)
 
 
+# few weight tiles and a long K: the sums stay in the workspace that the library asks for
+@pytest.mark.parametrize("K", [13312, 16384, 20480])
+@pytest.mark.parametrize("N", [64, 256, 1024])
+@pytest.mark.parametrize("M", [5, 30, 33, 64, 128, 140])
+def test_gemm_long_k_stays_in_its_workspace(E, M, N, K):
+    import torch
+    q, s = matrix(N, K, N + K)
+    xq, xs = E.fp8_quant_rows(rows(M, K, M))
+    room = E.fp8_gemm_ws_bytes(M, N, K)
+    buf = torch.full((room + (64 << 20),), 0x5a, dtype=torch.uint8, device="cuda")
+    y = E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q, s), xq, xs, out_dtype=torch.float32, ws=buf[:room])
+    assert (buf[room:] == 0x5a).all()
+    y0, a = R.gemm(R.codes_to_f64(xq), xs.double(), q.double(), s.double())
+    tol = R.sum_bound(K) * a
+    assert ((y.double() - y0).abs() <= tol + R.HALF[torch.float32] * (y0.abs() + tol)).all()
+    E.context().check_device()
+
+
 def test_gemm_strides_and_what_lies_around(E):
     import torch
     M, N, K = 37, 201, 336
