@@ -12,8 +12,8 @@
 namespace hb {
 
 // One warp takes a row.  The scores are worked out in fp32 with an error bound, and so is the selection; wherever two neighbours of the result (two
-// picks next to each other, the last pick and the best expert left out, the last group kept and the best one dropped) are closer than
-// their bounds, and are not equal by their inputs, 64 bits decide: between experts for the candidates alone, a lane each; between groups for the groups' values; for scores at the end of
+// picks next to each other, the last pick and the best expert left out that is not its equal by its inputs, the last group kept and the best one dropped) are
+// closer than their bounds, and are not equal by their inputs, 64 bits decide: between experts for the candidates alone, a lane each; between groups for the groups' values; for scores at the end of
 // fp32's range the warp does the whole row again.  64 bits for every row took 37 us for 8192 rows of 256 experts (this way 15)
 // and 12 us for one (6).
 constexpr int RG_WARPS = 4;
@@ -290,7 +290,27 @@ __device__ __forceinline__ bool route_grouped_row32(const RouteGroupedArgs& a, c
   const float v = rg_val(mykey), vn = __shfl_down_sync(0xffffffffu, v, 1);
   const float ln = __shfl_down_sync(0xffffffffu, l, 1), bn = __shfl_down_sync(0xffffffffu, b, 1);
   const bool next = __shfl_down_sync(0xffffffffu, mykey, 1) != 0u;               // (there may be no expert left to be left out)
-  const bool close = lane < a.k && next && !(v - vn > err(v) + err(vn)) && !(l == ln && b == bn);
+  const bool same = l == ln && b == bn;
+  bool close = lane < a.k && next && !(v - vn > err(v) + err(vn)) && !same;
+  if (__any_sync(0xffffffffu, lane == a.k - 1 && next && same)) {
+    // A tie at the border settles nothing about those behind it: the last pick has to stand clear of the best one left out that is not its equal
+    const uint32_t kk = __shfl_sync(0xffffffffu, mykey, a.k - 1);
+    const float lk = __shfl_sync(0xffffffffu, l, a.k - 1), bk = __shfl_sync(0xffffffffu, b, a.k - 1);
+    uint32_t rest = lane >= a.k && mykey && !(l == lk && b == bk) ? mykey : 0u;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      uint32_t x = rounds || key[j] < bound ? key[j] : 0u;                       // neither picked nor listed
+      if (x == kk) {
+        const int e = lane + 32 * j;
+        const float xl = fmaxf(__ldg(lr + e), -INFINITY);
+        if (xl == lk && rg_bias(a, e) == bk) x = 0u;
+      }
+      rest = max(rest, x);
+    }
+    rest = __reduce_max_sync(0xffffffffu, rest);
+    const float vk = rg_val(kk), vr = rg_val(rest);
+    close = close || (rest != 0u && !(vk - vr > err(vk) + err(vr)));
+  }
   safe = safe && !__any_sync(0xffffffffu, lane < a.k && mykey == 0u);
   if (!safe) return false;
   if (__any_sync(0xffffffffu, close)) {

@@ -64,6 +64,39 @@ def test_neighbours_that_fp32_scores_do_not_tell_apart(E, score, ng, tg):
     check(E, lg, bias, 7, ng, tg, 2, score, True, 1.0)
 
 
+@pytest.mark.parametrize("n", [2, 3, 9, 31, 32, 33, 60, 150])
+@pytest.mark.parametrize("score,tied,better,best", [("sigmoid", 20.0, 25.0, 30.0), ("softmax", 1.0, np.nextafter(np.float32(1), np.float32(2)), 10.0), ("softmax", -np.inf, -100.0, 0.0),
+                                                    ("sigmoid", -np.inf, -200.0, 0.0), ("sigmoid", -3e38, -120.0, 1.0)])
+def test_a_better_expert_behind_a_tie_at_the_border(E, score, tied, better, best, n):
+    """n equal logits, of which the picks take some, and behind them one that is better by less than fp32 scores show."""
+    size = max(n + 2, 8)
+    rng = np.random.default_rng(n)
+    for Ex in (size, 256):
+        lg = np.full((40, Ex), -np.inf if tied > -1e38 else tied, np.float32)
+        for m in range(40):
+            at = rng.permutation(Ex)[: n + 2]
+            lg[m, at] = tied
+            lg[m, max(at)] = better                                                   # (behind, by its index, all that it ties with in fp32)
+            if m % 2:
+                lg[m, at[0] if at[0] != max(at) else at[1]] = best
+        for k in sorted({1, 2, min(n, 5), min(n, 16)}):
+            check(E, lg, None, k, 1, 1, 1, score, False, 1.0)
+    check(E, np.array([[20, 20, 25, 0]], np.float32), None, 1, 1, 1, 1, "sigmoid", False, 1.0)
+    check(E, np.array([[1, 1, 1.0000001, 10]], np.float32), None, 2, 1, 1, 1, "softmax", False, 1.0)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("Ex,k,ng,tg,gt", [(256, 8, 8, 4, 2), (160, 6, 8, 3, 1), (64, 4, 1, 1, 1), (512, 10, 1, 1, 1), (1024, 16, 16, 9, 2), (24, 3, 1, 1, 1)])
+def test_logits_as_a_bf16_product_leaves_them(E, score, Ex, k, ng, tg, gt):
+    """Many equal logits, scores near the end of their range."""
+    import torch
+    rng = np.random.default_rng(Ex + k)
+    for by in (1.0, 8.0, 30.0):
+        lg = torch.from_numpy(np.clip(rng.normal(0, by, (700, Ex)), -30, 30).astype(np.float32)).to(torch.bfloat16).float().numpy()
+        check(E, lg, None, k, ng, tg, gt, score, True, 2.5)
+        check(E, lg, (rng.integers(-2, 3, Ex) * 2.0 ** -22).astype(np.float32), k, ng, tg, gt, score, False, 1.0)
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_masks_and_extremes(E, score):
     rng = np.random.default_rng(6)
