@@ -24,7 +24,7 @@ bool hbk_moe_layer_a16_takes(const hb_ctx* ctx, int M, int K, int E, int H, int 
 int hbk_moe_layer_a16(hb_ctx* ctx, const uint8_t* const* lt, int E, const uint8_t* shared_rec, const int32_t* ids, const float* w, int M, int K, const void* x, int H,
                       int I, float limit, const float* lg, int ld, int col, void* out, void* ws, cudaStream_t st);
 int hbk_nvfp4_setup(hb_ctx* ctx);
-// the plan of a grouped GEMM (k_moe_prefill.cu): pairs sorted by expert, runs cut into tiles of equal size of at most bm pairs
+// the plan of a grouped GEMM (k_moe_prefill.cu): pairs sorted by expert and then by their number, runs cut into tiles of equal size of at most bm pairs
 namespace hb { struct TileRef; }
 struct hbk_plan {
   const int32_t* ids; int P, E; const uint8_t* const* tab; int bm;

@@ -390,8 +390,9 @@ __global__ void __launch_bounds__(128, 1) pf_peak_kernel(int n_rounds, uint32_t*
 // [CTAs][E] table.  After the meeting every CTA adds up the table's columns for itself — the column total gives the expert's run
 // (an exclusive scan over the experts, done redundantly by every CTA), the rows above its own give where its slice's share of the run
 // starts — and places its pairs with shared-memory cursors.  No global atomics on the data, no separate scan launch, and a pair's
-// slot depends only on which CTA holds it and on the order inside that CTA (any order inside an expert's run gives the same
-// results: a pair's output depends on its own row alone).  CTA 0 also writes the tile list.  pos_of[p] = slot of pair p, or -1 for
+// slot depends only on which CTA holds it and on the order inside that CTA: with ORDERED that of the pairs, else any (where a pair's
+// output depends on its own row alone every order gives the same results; where the tile it lies in decides how its sums are cut, as in the
+// 8-bit GEMMs, the order has to be the same in every run).  CTA 0 also writes the tile list.  pos_of[p] = slot of pair p, or -1 for
 // a pair that contributes nothing (id outside [0, E), or no record for the expert on this GPU).
 constexpr int PLAN_THREADS = 1024, PLAN_MAX_CTAS = 64;
 struct PlanArgs {
@@ -403,13 +404,16 @@ struct PlanArgs {
   unsigned int* meet;              // two context-owned counters, zero between launches
   uint32_t* err;
 };
+template <bool ORDERED>
 __global__ void __launch_bounds__(PLAN_THREADS) pf_plan_kernel(const PlanArgs a) {
+  extern __shared__ uint16_t plan_cnt[];               // ORDERED: [32 warps][E], zero between chunks
   __shared__ int cur[1024];
   __shared__ int wsum[2][32];
   const int G = gridDim.x, cta = blockIdx.x, t = threadIdx.x, lane = t & 31, wp = t >> 5;
   const int per = (a.P + G - 1) / G, p0 = min(a.P, cta * per), p1 = min(a.P, p0 + per);
   auto expert_of = [&](int p) -> int { const int e = a.ids[p]; return (e >= 0 && e < a.E && a.tab[e] != nullptr) ? e : -1; };
   cur[t] = 0;
+  if constexpr (ORDERED) { for (int i = t; i < 32 * a.E; i += PLAN_THREADS) plan_cnt[i] = 0; }
   __syncthreads();
   for (int p = p0 + t; p < p1; p += PLAN_THREADS) { const int e = expert_of(p); if (e >= 0) atomicAdd(&cur[e], 1); }
   __syncthreads();
@@ -458,11 +462,42 @@ __global__ void __launch_bounds__(PLAN_THREADS) pf_plan_kernel(const PlanArgs a)
     if (t == PLAN_THREADS - 1) { *a.n_tiles = wsum[1][31]; *a.n_slots = wsum[0][31]; }
   }
   __syncthreads();
-  for (int p = p0 + t; p < p1; p += PLAN_THREADS) {
-    const int e = expert_of(p);
-    int pos = -1;
-    if (e >= 0) { pos = atomicAdd(&cur[e], 1); if (HB_BOUND(a.err, pos >= 0 && pos < a.P, 0x201u, pos)) a.perm[pos] = p; }
+  auto place = [&](int p, int pos) {
+    if (pos >= 0 && HB_BOUND(a.err, pos < a.P, 0x201u, pos)) a.perm[pos] = p;
     a.pos_of[p] = pos;
+  };
+  if constexpr (ORDERED) {
+    // 1024 pairs at a time: each warp counts its own by expert, the counts are summed up over the warps in order, a pair's place is behind those of the warps
+    // in front and of the lanes in front.  (3 to 4 us more than cursors that the threads race for, of a call of some 2000 to 65536 pairs.)
+    int before = 0;                                    // pairs of expert t in the chunk before this one
+    for (int c0 = p0; c0 < p1; c0 += PLAN_THREADS) {
+      const int p = c0 + t, e = p < p1 ? expert_of(p) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, e);
+      const int front = __popc(same & ((1u << lane) - 1u));
+      uint16_t* mine = plan_cnt + (e >= 0 ? wp * a.E + e : 0);
+      if (e >= 0 && front == 0) *mine = (uint16_t)__popc(same);
+      __syncthreads();
+      if (t < a.E) {
+        cur[t] += before;
+        before = 0;
+#pragma unroll 8
+        for (int w = 0; w < 32; ++w) {
+          const int c = plan_cnt[w * a.E + t];
+          if (c) plan_cnt[w * a.E + t] = (uint16_t)before;
+          before += c;
+        }
+      }
+      __syncthreads();
+      if (p < p1) place(p, e >= 0 ? cur[e] + *mine + front : -1);
+      __syncwarp();
+      if (e >= 0 && front == 0) *mine = 0;
+      __syncwarp();
+    }
+  } else {
+    for (int p = p0 + t; p < p1; p += PLAN_THREADS) {
+      const int e = expert_of(p);
+      place(p, e >= 0 ? atomicAdd(&cur[e], 1) : -1);
+    }
   }
 }
 
@@ -657,7 +692,7 @@ int pf_a16_run(hb_ctx* ctx, const uint8_t* const* lt, int E, const int32_t* ids,
     int plan_ctas = (P + 2047) / 2048;
     if (plan_ctas > PLAN_MAX_CTAS) plan_ctas = PLAN_MAX_CTAS;
     if (plan_ctas > ctx->sm_count) plan_ctas = ctx->sm_count;
-    if ((r = hb_launch(ctx, "pf_plan", false, pf_plan_kernel, dim3(plan_ctas), dim3(PLAN_THREADS), 0, st, pl))) return r;
+    if ((r = hb_launch(ctx, "pf_plan", false, pf_plan_kernel<false>, dim3(plan_ctas), dim3(PLAN_THREADS), 0, st, pl))) return r;
     if ((r = hb_launch(ctx, "a16_gather", false, a16_gather_kernel, dim3((P < ctx->sm_count * 16 ? P : ctx->sm_count * 16) + 1), dim3(256), 0, st, x + (size_t)s0 * H,
                        (const int*)W.perm, (const int*)W.n_slots, K, H, W.part, wm)))
       return r;
@@ -716,11 +751,12 @@ int hbk_pf_plan(hb_ctx* ctx, const hbk_plan& p, cudaStream_t st) {
   int ctas = (p.P + 2047) / 2048;
   if (ctas > PLAN_MAX_CTAS) ctas = PLAN_MAX_CTAS;
   if (ctas > ctx->sm_count) ctas = ctx->sm_count;                              // the CTAs meet inside the kernel: all must be resident
-  return hb_launch(ctx, "pf_plan", false, pf_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), 0, st, pl);
+  return hb_launch(ctx, "pf_plan", false, pf_plan_kernel<true>, dim3(ctas), dim3(PLAN_THREADS), (size_t)32 * p.E * 2, st, pl);
 }
 size_t hbk_pf_plan_hist_bytes(int E) { return (size_t)PLAN_MAX_CTAS * E * 4; }
 
 int hbk_moe_prefill_setup(hb_ctx* ctx) {
+  HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(pf_plan_kernel<true>), cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * HB_MAX_EXPERTS * 2));
   HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(pf_gemm_kernel<PF_PLAIN>), cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM));
   HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(pf_gemm_kernel<PF_GU>), cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM));
   HB_CUDA(ctx, cudaFuncSetAttribute(reinterpret_cast<const void*>(pf_gemm_kernel<PF_DOWN>), cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM));
@@ -806,7 +842,7 @@ int hb_moe_prefill(hb_ctx* ctx, const uint8_t* const* rec_tab, int li, int E, co
     int plan_ctas = (P + 2047) / 2048;
     if (plan_ctas > PLAN_MAX_CTAS) plan_ctas = PLAN_MAX_CTAS;
     if (plan_ctas > ctx->sm_count) plan_ctas = ctx->sm_count;                   // the CTAs meet inside the kernel: all must be resident
-    if ((r = hb_launch(ctx, "pf_plan", false, pf_plan_kernel, dim3(plan_ctas), dim3(PLAN_THREADS), 0, st, pl))) return r;
+    if ((r = hb_launch(ctx, "pf_plan", false, pf_plan_kernel<false>, dim3(plan_ctas), dim3(PLAN_THREADS), 0, st, pl))) return r;
     // x quantised once per row and written straight into its pairs' slots
     if ((r = hbk_quant_rows_scatter(ctx, x + (size_t)s0 * H, H, n, H, W.pos_of, K, W.xq_s, W.xs_s, W.xg_s, st))) return r;
     PfGemmArgs a{};

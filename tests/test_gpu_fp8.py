@@ -300,6 +300,22 @@ def test_moe_lists_of_pairs(E, M, Ex, K):
     assert torch.equal(out, E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=torch.float32))
 
 
+# experts whose runs take several tiles, of which some items are cut and others are not: tiles of 128 rows behind a round of whole items, tiles of 32 rows of more
+# pairs than the kernels order for themselves, and a list that several CTAs put in order
+@pytest.mark.parametrize("M,H,I,Ex,K,hot", [(1000, 2304, 1280, 4, 2, None), (750, 1024, 256, 80, 2, None), (750, 2304, 256, 80, 2, 3), (3000, 2304, 512, 6, 4, 1), (1200, 640, 384, 600, 12, None)])
+def test_moe_long_lists_give_the_same_bits_every_time(E, M, H, I, Ex, K, hot):
+    import torch
+    R0 = min(Ex, 6)
+    recs = [record(E, H, I, 10 * e + M)[0] for e in range(R0)]
+    tab = torch.tensor([recs[e % R0].data_ptr() for e in range(Ex)], dtype=torch.int64, device="cuda")
+    ids, w = routing(M, K, Ex, M, hot)
+    x = (torch.randn(M, H, device="cuda", generator=gen(M)) * 2).to(torch.bfloat16)
+    ref = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=torch.float32)
+    for _ in range(10):
+        assert torch.equal(ref, E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=torch.float32))
+    E.context().check_device()
+
+
 def test_few_ctas_and_many(E):
     """Contexts that may use fewer CTAs cut the items elsewhere: the results stay within fp32 summation order, cut items or not."""
     import torch
