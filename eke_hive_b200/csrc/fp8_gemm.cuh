@@ -148,7 +148,7 @@ struct F8Args {
   uint8_t* maps;                                       // GU / DOWN: room for F8_MAPS tensor maps a CTA
   const float* xs; int lds;                            // scales of the rows
   float limit;
-  __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN
+  __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN: one of them
   uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
   float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256]; arrivals, by the CTA of an item's first step (zero before and after)
   uint32_t room;                                       // of part, in sums: range checks of the debug build
@@ -544,19 +544,19 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
         }
         named_bar_sync(2 + h, 128);                                            // the magnitudes have been read
       } else {
+        auto store = [&](auto* y, auto value) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int n = nt * 256 + u * 128 + row;
-          if (n < a.N && ok) {
+          for (int u = 0; u < 2; ++u) {
+            const int n = nt * 256 + u * 128 + row;
+            if (n < a.N && ok) {
 #pragma unroll
-            for (int c = 0; c < C::CW; ++c)
-              if (c < cols) {
-                const size_t at = (size_t)(tl.slot0 + h * C::CW + c) * a.ldy + n;
-                if (MODE == F8_DOWN || a.yb) a.yb[at] = __float2bfloat16(acc[u][c]);
-                else a.yf[at] = acc[u][c];
-              }
+              for (int c = 0; c < C::CW; ++c)
+                if (c < cols) y[(size_t)(tl.slot0 + h * C::CW + c) * a.ldy + n] = value(acc[u][c]);
+            }
           }
-        }
+        };
+        if (a.yb) store(a.yb, [](float v) { return __float2bfloat16(v); });
+        else store(a.yf, [](float v) { return v; });
       }
     }
   }

@@ -159,48 +159,58 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
 }
 
 // ---- the sum over a row's pairs: out[m] = Σ_k w[m,k]·part[slot of (m,k)], k in order (+ gate·shared[m]) ----------------------------------
-// A warp takes 512 columns of a row, a lane twice eight of them (16 bytes of every pair's part).  Lane k looks up pair k; only pairs that have a slot are gone
-// through, four parts fetched at a time.  8192 rows of 7168 with a pair each and shared rows: 75 us, 4.7 TB/s (two at a time and more warps: 69, but ten pairs a row
-// of 2048, 16 rows: 10.7 us instead of 9).
+// A warp takes 512 columns of a row (fp32 parts: 256), a lane twice 16 bytes of every pair's part.  Lane k looks up pair k; only pairs that have a slot are gone
+// through, four parts fetched at a time.  T, what the parts are held in: fp32 for an fp32 result; for one that is rounded to bf16 in the end bf16, which is off by 2^-9
+// of a pair's own share and half the bytes (8192 rows of 7168 with a pair each: a whole layer of 32 held experts of 256 takes 677 us, with fp32 parts 734; of 1000
+// rows of 4096 with eight pairs each 586, 620).
 constexpr int F8_SUM_THREADS = 128;
+template <class T>
 struct F8SumArgs {
-  const __nv_bfloat16* part; const int* pos_of; const float* w; int M, K, H; float* out;
+  const T* part; const int* pos_of; const float* w; int M, K, H; float* out;
   const __nv_bfloat16* shared; const float* lg; int ld, col; __nv_bfloat16* cout;
 };
-__global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs a) {
+template <class T>
+constexpr int F8_SUM_COLS = 2 * 32 * (16 / (int)sizeof(T));
+template <class T>
+__global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs<T> a) {
+  constexpr int WARPS = F8_SUM_THREADS / 32, V = 16 / (int)sizeof(T), COLS = F8_SUM_COLS<T>, HALF = COLS / 2;
   bool waited = false;                                                         // only the parts are of the kernel in front
-  const int chunks = (a.H + 511) / 512, lane = threadIdx.x & 31;
+  const int chunks = (a.H + COLS - 1) / COLS, lane = threadIdx.x & 31;
   const long long total = (long long)a.M * chunks;
-  constexpr int WARPS = F8_SUM_THREADS / 32;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   for (long long i = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); i < total; i += (long long)gridDim.x * WARPS) {
-    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * 512 + lane * 8;
-    const bool in[2] = {n < a.H, n + 256 < a.H};                               // H is a multiple of 128
+    const int m = (int)(i / chunks), n = (int)(i - (long long)m * chunks) * COLS + lane * V;
+    const bool in[2] = {n < a.H, n + HALF < a.H};                              // H is a multiple of 128
     const size_t o = (size_t)m * a.H + n;
     const int slot = lane < a.K ? __ldg(a.pos_of + (size_t)m * a.K + lane) : -1;
     const float wk = lane < a.K ? __ldg(a.w + (size_t)m * a.K + lane) : 0.f;
-    uint4 sv[2];
+    uint4 sv[2] = {zero, zero};
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) sv[h] = a.shared && in[h] ? __ldg(reinterpret_cast<const uint4*>(a.shared + o + 256 * h)) : zero;
+      for (int h = 0; h < 2; ++h) if (a.shared && in[h]) sv[h] = __ldg(reinterpret_cast<const uint4*>(a.shared + o + HALF * h));
+    }
     const float gate = a.lg ? 1.f / (1.f + expf(-__ldg(a.lg + (size_t)m * a.ld + a.col))) : 1.f;
     if (!waited) { griddep_wait(); waited = true; }
-    float acc[2][8];
+    float acc[2][V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
-    auto add = [&](float (&to)[8], const uint4& v, float f) {
+    for (int j = 0; j < V; ++j) acc[0][j] = acc[1][j] = 0.f;
+    auto add = [&](float (&to)[V], const uint4& v, float f) {
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { to[2 * j] = fmaf(f, __uint_as_float(u[j] << 16), to[2 * j]); to[2 * j + 1] = fmaf(f, __uint_as_float(u[j] & 0xffff0000u), to[2 * j + 1]); }
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) to[j] = fmaf(f, __uint_as_float(u[j]), to[j]);
+        else { to[2 * j] = fmaf(f, __uint_as_float(u[j] << 16), to[2 * j]); to[2 * j + 1] = fmaf(f, __uint_as_float(u[j] & 0xffff0000u), to[2 * j + 1]); }
+      }
     };
     for (uint32_t on = __ballot_sync(0xffffffffu, slot >= 0); on;) {
       uint4 v[4][2]; float f[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int k = on ? __ffs(on) - 1 : 0;
-        const __nv_bfloat16* p = a.part + (size_t)__shfl_sync(0xffffffffu, slot, k) * a.H + n;
+        const T* p = a.part + (size_t)__shfl_sync(0xffffffffu, slot, k) * a.H + n;
         f[j] = on ? __shfl_sync(0xffffffffu, wk, k) : 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[j][h] = on && in[h] ? __ldcs(reinterpret_cast<const uint4*>(p + 256 * h)) : zero;
+        for (int h = 0; h < 2; ++h) v[j][h] = on && in[h] ? __ldcs(reinterpret_cast<const uint4*>(p + HALF * h)) : zero;
         on &= on - 1u;
       }
 #pragma unroll
@@ -209,12 +219,10 @@ __global__ void __launch_bounds__(F8_SUM_THREADS) fp8_sum_kernel(const F8SumArgs
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (!in[h]) continue;
-      if (!a.cout) {
-        *reinterpret_cast<float4*>(a.out + o + 256 * h) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
-        *reinterpret_cast<float4*>(a.out + o + 256 * h + 4) = make_float4(acc[h][4], acc[h][5], acc[h][6], acc[h][7]);
-      } else {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(a.out + o + HALF * h) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+      else {
         if (a.shared) add(acc[h], sv[h], gate);
-        *reinterpret_cast<uint4*>(a.cout + o + 256 * h) = f8_pack8(acc[h]);
+        *reinterpret_cast<uint4*>(a.cout + o + HALF * h) = f8_pack8(acc[h]);
       }
     }
   }
@@ -263,7 +271,7 @@ int f8_map(hb_ctx* ctx, CUtensorMap* m, const void* base, size_t row_bytes, size
 }
 
 struct F8Ws {
-  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; uint8_t* yq; float* ys; __nv_bfloat16* part; float* cut; uint8_t* maps;
+  int* hist; int* n_slots; int* n_tiles; TileRef* tiles; int* perm; int* pos_of; uint8_t* xq; float* xs; uint8_t* yq; float* ys; void* part; float* cut; uint8_t* maps;
 };
 size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   size_t off = 0;
@@ -273,9 +281,12 @@ size_t f8_carve(void* ws, int M, int K, int E, int H, int I, F8Ws* w) {
   F8Ws t;
   t.hist = (int*)take(hbk_pf_plan_hist_bytes(E)); t.n_slots = (int*)take(4); t.n_tiles = (int*)take(4);
   t.tiles = (TileRef*)take((P / 16 + E) * sizeof(TileRef)); t.perm = (int*)take(P * 4); t.pos_of = (int*)take(P * 4);
-  t.xq = (uint8_t*)take(P * H); t.xs = (float*)take(P * f8_blocks(H) * 4);
   t.yq = (uint8_t*)take(P * I); t.ys = (float*)take(P * f8_blocks(I) * 4);
-  t.part = (__nv_bfloat16*)take(P * H * 2);
+  // The down pass writes its results, of two or four bytes, over the rows that the gate/up pass was given (codes and scales, 1 + 1 / 32 bytes a value)
+  const size_t rows = off;
+  t.xq = (uint8_t*)take(P * H); t.xs = (float*)take(P * f8_blocks(H) * 4);
+  off = rows;
+  t.part = take(P * H * 4);
   t.cut = (float*)take(f8_part_bytes(bn));
   t.maps = (uint8_t*)take((size_t)2 * F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap));   // of the gate/up pass and of the down pass
   if (w) *w = t;
@@ -420,15 +431,19 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   a.split = 2;                                                                 // (all SMs are in reach of clusters of two)
   if ((r = f8_launch<F8_GU>(ctx, "fp8_gemm_gu", rows, a, tg, tx, st))) return r;
   a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.maps = W.maps + (size_t)F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap);
-  a.xs = W.ys; a.yb = W.part; a.ldy = H;
+  a.xs = W.ys; a.ldy = H;
+  if (cmb) a.yb = reinterpret_cast<__nv_bfloat16*>(W.part); else a.yf = reinterpret_cast<float*>(W.part);
   if ((r = f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, td, ty, st))) return r;
-  F8SumArgs su{W.part, W.pos_of, w, M, K, H, out, nullptr, nullptr, 0, 0, nullptr};
-  if (cmb) {
-    su.cout = reinterpret_cast<__nv_bfloat16*>(cmb->out); su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
-    if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
-  }
-  const long long sums = ((long long)M * ((H + 511) / 512) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
-  return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel, dim3((unsigned)(sums < cap ? sums : cap)), dim3(F8_SUM_THREADS), 0, st, su);
+  auto sum = [&](auto su) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(su.part)>>;
+    const long long sums = ((long long)M * ((H + F8_SUM_COLS<T> - 1) / F8_SUM_COLS<T>) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
+    return hb_launch(ctx, "fp8_sum", true, fp8_sum_kernel<T>, dim3((unsigned)(sums < cap ? sums : cap)), dim3(F8_SUM_THREADS), 0, st, su);
+  };
+  if (!cmb) return sum(F8SumArgs<float>{reinterpret_cast<const float*>(W.part), W.pos_of, w, M, K, H, out, nullptr, nullptr, 0, 0, nullptr});
+  F8SumArgs<__nv_bfloat16> su{reinterpret_cast<const __nv_bfloat16*>(W.part), W.pos_of, w, M, K, H, nullptr, nullptr, nullptr, 0, 0, reinterpret_cast<__nv_bfloat16*>(cmb->out)};
+  su.shared = reinterpret_cast<const __nv_bfloat16*>(cmb->shared);
+  if (cmb->shared) { su.lg = cmb->lg; su.ld = cmb->ld; su.col = cmb->col; }
+  return sum(su);
 }
 
 }  // extern "C"

@@ -337,7 +337,8 @@ typedef struct hb_fp8_rec_layout {
 HB_API int hb_fp8_rec_layout_make(int H, int I, hb_fp8_rec_layout* out);
 /* Routed experts of FP8 records for any number of rows (the operator of engine/include/hive/qwen/fn_moe.h:38-41 with 8-bit activations): per pair
  * (row m, expert ids[m,k]) x[m] is quantised by hb_fp8_quant_rows' rule, g and u are its products with w1 and w3 (fp32), y = silu(g)·u (limit > 0:
- * g ≤ limit, |u| ≤ limit first) is quantised by the same rule, d = bf16 of its product with w2, and
+ * g ≤ limit, |u| ≤ limit first) is quantised by the same rule, d is its product with w2, held in fp32 for an fp32
+ * result and in bf16 for a bf16 one, and
  *   routed[m] = Σ_k w[m,k]·d (fp32, in k order).
  * cmb == NULL: out fp32 [M,H] = routed.  Else cmb->out bf16 [M,H] = bf16(routed + gate·shared[m]), gate = sigmoid(lg[m·ld + col]) or 1 where
  * cmb->lg is NULL, no shared term where cmb->shared is NULL; `out` is not used.  Records come from rec_tab[li·E + id] (16-byte aligned); ids outside

@@ -401,6 +401,44 @@ def test_gemm_matrix_beyond_32_bits(E):
     assert ((y[-256:].double() - y0).abs() <= R.sum_bound(K) * a + R.HALF[torch.float32] * (y0.abs() + R.sum_bound(K) * a)).all()
 
 
+def exact_experts(E, M, Ex, seed):
+    """Experts whose y is known to the last bit: x holds e4m3 values up to 448 (scale 1), every gate is 56 (silu leaves it), up adds a few exact products, w2 is
+    the unit matrix.  Returns (x, ids, w, table, its records, y fp32 [M, I])."""
+    import torch
+    H = I = 256
+    g = gen(seed)
+    unit = lambda n: torch.ones(n // 128, n // 128, device="cuda")
+    x = torch.zeros(M, H, device="cuda")
+    x[:, 0] = 448.0
+    x[:, 1:9] = (torch.rand(M, 8, device="cuda", generator=g) * 400 + 40).to(torch.float8_e4m3fn).float() * torch.where(torch.rand(M, 8, device="cuda", generator=g) < 0.5, 1.0, -1.0)
+    recs, ups = [], []
+    for e in range(Ex):
+        gate, up, down = (torch.zeros(n, k, device="cuda") for n, k in ((I, H), (I, H), (H, I)))
+        gate[:, 0] = 1.0
+        up[:, 1:9] = (torch.randn(I, 8, device="cuda", generator=g) * 2).to(torch.float8_e4m3fn).float()
+        up[:, 1:9] = torch.where(up[:, 1:9].abs() < 0.25, 0.25, up[:, 1:9])                # (a sum of eight products then fits into 24 bits)
+        down[torch.arange(H), torch.arange(I)] = 1.0
+        f8 = [m.to(torch.float8_e4m3fn) for m in (gate, up, down)]
+        recs.append(E.fp8_record(H, I, (f8[0], unit(I) * 0.125), (f8[1], unit(I) * 2.0 ** -9), (f8[2], unit(I))))
+        ups.append(up)
+    ids = torch.randint(0, Ex, (M, 1), device="cuda", generator=g, dtype=torch.int32)
+    y = torch.stack([(x[m].double() @ ups[int(ids[m, 0])].double().T) * 2.0 ** -9 for m in range(M)])
+    assert (y == y.float().double()).all()                                               # up's sums are fp32 values
+    return x.to(torch.bfloat16), ids, torch.ones(M, 1, device="cuda"), E.rec_table(recs), recs, 56.0 * y.float()
+
+
+@pytest.mark.parametrize("M,Ex", [(1, 4), (9, 4), (40, 4), (90, 4), (150, 4), (1100, 150), (1100, 60)])
+def test_moe_sums_fp32_values(E, M, Ex):
+    """A pair's result is no bf16 number on its way into the sum: each is a code of y times its block's scale, to fp32 precision."""
+    import torch
+    x, ids, w, tab, _recs, y = exact_experts(E, M, Ex, M)
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, 256, 256, out_dtype=torch.float32).double()
+    s = (y.abs().view(M, 2, 128).amax(2).double() / 448.0).float().double().repeat_interleave(128, 1)
+    v = out / s
+    assert ((v - y.double() / s).abs() <= 2.0 ** -4 * (y.double() / s).abs() + 2.0 ** -10 + 1e-4).all()      # its own code, or off a border the other one
+    assert ((v - R.nearest_e4m3(v.clamp(-448, 448))).abs() <= 2.0 ** -22 * v.abs()).all()                   # the scale's product and the sum's rounding: half a step each
+
+
 def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
