@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
 #pragma unroll
         for (int c = 0; c < C::CW; ++c) {
           if (c < cols && ok) {
-            F8BlockFast blk;
+            F8Block blk;
             const float sc = blk.init(max(max(am[c], am[C::CW + c]), max(am[2 * C::CW + c], am[3 * C::CW + c])));
             const int slot = tl.slot0 + h * C::CW + c;
             a.yq[(size_t)slot * a.N + nt * 128 + row] = (uint8_t)blk.pair(acc[0][c], 0.f);

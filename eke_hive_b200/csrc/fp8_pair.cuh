@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         }
         amx[h * 128 + row] = mx;
         named_bar_sync(1, 256);
-        F8BlockFast blk;
+        F8Block blk;
         const float sc = blk.init(max(amx[row], amx[128 + row]));
         if (valid && ok) {
           uint8_t* to = a.yq + (slot0 + row) * a.N + nt * 128 + h * 64;

@@ -439,6 +439,40 @@ def test_moe_sums_fp32_values(E, M, Ex):
     assert ((v - R.nearest_e4m3(v.clamp(-448, 448))).abs() <= 2.0 ** -22 * v.abs()).all()                   # the scale's product and the sum's rounding: half a step each
 
 
+@pytest.mark.parametrize("M,Ex", [(1, 1), (8, 1), (30, 4), (90, 4), (600, 4), (1100, 60)])
+def test_moe_quantises_y_by_the_rows_rule(E, M, Ex):
+    """y · 448 / amax is a border between two codes, exactly, in every row and for every size of y: the code is the even one."""
+    import torch
+    H = I = 128
+    mids = [m * 2.0 ** p for p in (-1, 0, 1, 2, 3) for m in range(17, 32, 2) if m * 2.0 ** p < 440]
+    gate, up, down = (torch.zeros(n, k, device="cuda") for n, k in ((I, H), (I, H), (H, I)))
+    gate[:, 0] = 1.0
+    down[torch.arange(H), torch.arange(I)] = 1.0
+    for i, m in enumerate([448.0] + mids):                                               # up's row i is m times a row's number: m in two codes, for a number in three values
+        c = float(R.nearest_e4m3(torch.tensor([m * (1 - 2.0 ** -6)], dtype=torch.float64)))
+        up[i, 1:4], up[i, 4:7] = c, m - c
+    assert (up.to(torch.float8_e4m3fn).float() == up).all() and ((up[1:len(mids) + 1, 1] + up[1:len(mids) + 1, 4]).cpu() == torch.tensor(mids)).all()
+    one = torch.ones(1, 1, device="cuda")
+    f8 = [m.to(torch.float8_e4m3fn) for m in (gate, up, down)]
+    rec = E.fp8_record(H, I, (f8[0], one * 0.125), (f8[1], one * 2.0 ** -9), (f8[2], one))
+    x = torch.zeros(M, H, dtype=torch.float64, device="cuda")
+    x[:, 0] = 448.0
+    number = (torch.arange(M, device="cuda", dtype=torch.float64) * 7 + 3) % 700 + 1
+    left = number.clone()
+    for j in range(3):
+        part = torch.where(left > 0, torch.floor(left / torch.exp2(torch.floor(torch.log2(left.clamp_min(1))) - 3)) * torch.exp2(torch.floor(torch.log2(left.clamp_min(1))) - 3), 0.0).clamp(max=448)
+        x[:, 1 + j] = x[:, 4 + j] = part
+        left -= part
+    assert (left == 0).all()                                                             # (up to 700: 448 and seven or eight bits more)
+    ids = torch.randint(0, Ex, (M, 1), device="cuda", generator=gen(M), dtype=torch.int32)
+    out = E.moe_fp8(ids, torch.ones(M, 1, device="cuda"), E.rec_table([rec] * Ex), 0, Ex, x.to(torch.bfloat16), H, I, out_dtype=torch.float32).double()
+    s = (56.0 * 448.0 * 2.0 ** -9 * number / 448.0).float().double()[:, None]
+    want = R.nearest_e4m3(torch.tensor([448.0] + mids, dtype=torch.float64, device="cuda")) * s
+    n = len(mids) + 1
+    assert torch.equal(out[:, :n], want.float().double()), ((out[:, :n] - want).abs() / want).max().item()
+    assert (out[:, n:] == 0).all()
+
+
 def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
