@@ -206,7 +206,7 @@ __device__ __forceinline__ uint4 f8_pack8(const float* v) {                     
   return make_uint4(p[0], p[1], p[2], p[3]);
 }
 // A warp's staged 32 rows × 64 bytes to memory, eight rows an instruction (a lane has a row: its own stores would touch 32 rows each).  to: the first
-// row's place; bytes: how much of a row there is room for.
+// row's place; bytes: how much of the 64 there is room for.
 __device__ __forceinline__ void f8_flush(const uint8_t* stg, uint8_t* to, size_t ld, int rows, int bytes, int lane) {
   __syncwarp();
   const int c = (lane & 3) * 16;

@@ -412,14 +412,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
           for (int c = 0; c < 128; c += 32) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * F8_STG_PITCH + 16 * j) = f8_pack8(&acc[c + 8 * j]);
-            f8_flush(stg, reinterpret_cast<uint8_t*>(a.yb + row0 * a.ldy + n0 + c), (size_t)a.ldy * 2, nrow, (a.N - n0 - c) * 2, lane);
+            f8_flush(stg, reinterpret_cast<uint8_t*>(a.yb + row0 * a.ldy + n0 + c), (size_t)a.ldy * 2, nrow, min(a.N - n0 - c, 32) * 2, lane);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < 128; c += 16) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(stg + lane * F8_STG_PITCH + 16 * j) = make_float4(acc[c + 4 * j], acc[c + 4 * j + 1], acc[c + 4 * j + 2], acc[c + 4 * j + 3]);
-            f8_flush(stg, reinterpret_cast<uint8_t*>(a.yf + row0 * a.ldy + n0 + c), (size_t)a.ldy * 4, nrow, (a.N - n0 - c) * 4, lane);
+            f8_flush(stg, reinterpret_cast<uint8_t*>(a.yf + row0 * a.ldy + n0 + c), (size_t)a.ldy * 4, nrow, min(a.N - n0 - c, 16) * 4, lane);
           }
         }
       }

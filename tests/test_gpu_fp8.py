@@ -473,6 +473,28 @@ def test_moe_quantises_y_by_the_rows_rule(E, M, Ex):
     assert (out[:, n:] == 0).all()
 
 
+@pytest.mark.parametrize("N,dt", [((1 << 29) + 40, "float32"), (1 << 30, "bfloat16")])
+def test_gemm_rows_of_the_result_beyond_31_bits_of_bytes(E, N, dt):
+    """The most columns a product may have: what is left of a row is more than 2^31 bytes at its front."""
+    import torch
+    M, K, n = 33, 16, 700
+    q = torch.zeros(N, K, dtype=torch.uint8, device="cuda")
+    s = torch.ones(R.up(N), 1, device="cuda")
+    part, ps = matrix(2 * n, K, 1)
+    q[:n], q[-n:] = part[:n].view(torch.uint8), part[n:].view(torch.uint8)
+    xq, xs = E.fp8_quant_rows(rows(M, K, M))
+    y = torch.empty(M, N, dtype=getattr(torch, dt), device="cuda")
+    y[:, :2 * n] = -7; y[:, -2 * n:] = -7
+    E.fp8_gemm(E.GMat(E.FMT_FP8_B128, N, K, q, s), xq, xs, y=y)
+    for cols, w in ((y[:, :n], part[:n]), (y[:, -n:], part[n:])):
+        y0, a = R.gemm(R.codes_to_f64(xq), xs.double(), w.double(), torch.ones(R.up(n), 1, dtype=torch.float64, device="cuda"))
+        tol = R.sum_bound(K) * a
+        assert ((cols.double() - y0).abs() <= tol + R.HALF[y.dtype] * (y0.abs() + tol)).all()
+    assert (y[:, n:2 * n] == 0).all() and (y[:, -2 * n:-n] == 0).all()
+    del y, q
+    torch.cuda.empty_cache()
+
+
 def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
