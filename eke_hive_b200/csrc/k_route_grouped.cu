@@ -79,8 +79,7 @@ __device__ __noinline__ void route_grouped_row64(const RouteGroupedArgs& a, cons
     if ((at & 31) == lane) gone |= 1u << (at >> 5);
     if (lane == r) id = at;
   }
-  double s = lane < a.k ? score(id) : 0.0, tot = 0.0;
-  if (!(s == s)) s = 0.0;
+  double s = lane < a.k ? score(id) : 0.0, tot = 0.0;                            // (NaN in a softmax row with +inf)
   for (int r = 0; r < a.k; ++r) tot += __shfl_sync(0xffffffffu, s, r);
   if (a.renorm) s /= tot + 1e-20;
   w = (float)(s * (double)a.scale);

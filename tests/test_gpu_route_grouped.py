@@ -121,6 +121,26 @@ def test_masks_and_extremes(E, score):
                 assert all(len(set(r)) == 6 for r in i.tolist())
 
 
+@pytest.mark.parametrize("Ex,k,ng,tg", [(64, 6, 8, 2), (64, 6, 1, 1), (20, 8, 10, 4), (1024, 16, 8, 4)])
+def test_a_softmax_row_with_infinity_has_no_weights(E, Ex, k, ng, tg):
+    """Its weights are NaN, as the header says, its picks are experts, all different; the rows beside it, and a sigmoid, take no harm."""
+    import torch
+    rng = np.random.default_rng(Ex)
+    lg = rng.normal(0, 1, (9, Ex)).astype(np.float32)
+    bad = lg.copy()
+    bad[2, 3] = np.inf; bad[5, :] = np.inf; bad[7, -1] = np.inf; bad[7, 0] = np.nan
+    ok = [0, 1, 3, 4, 6, 8]
+    for bias in (None, rng.normal(0, 0.1, Ex).astype(np.float32)):
+        b = None if bias is None else torch.from_numpy(bias).cuda()
+        for renorm in (False, True):
+            i0, w0 = R.route(lg, bias, k, ng, tg, 2, "softmax", renorm, 1.0)
+            ids, w = E.router_grouped_topk(torch.from_numpy(bad).cuda(), k, ng, tg, score="softmax", bias=b, renorm=renorm)
+            assert np.array_equal(ids.cpu().numpy()[ok], i0[ok]) and (np.abs(w.cpu().numpy()[ok] - w0[ok]) <= R.route_bound(lg, "softmax") * np.abs(w0[ok]) + 2.0 ** -149).all()
+            assert torch.isnan(w[[2, 5, 7]]).all()
+            assert all(len(set(r)) == k and min(r) >= 0 and max(r) < Ex for r in ids.tolist())
+            check(E, bad, bias, k, ng, tg, 2, "sigmoid", renorm, 1.0)
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 @pytest.mark.parametrize("Ex,k,ng,tg", [(64, 6, 8, 2), (64, 6, 1, 1), (20, 8, 10, 4), (256, 8, 8, 4)])
 def test_bias_that_is_not_finite(E, score, Ex, k, ng, tg):
