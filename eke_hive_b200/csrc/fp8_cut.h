@@ -3,6 +3,7 @@
 #pragma once
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #ifdef __CUDACC__
 #define HB_HD __host__ __device__ __forceinline__

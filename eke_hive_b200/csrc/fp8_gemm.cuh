@@ -20,6 +20,7 @@
 #pragma once
 #include <type_traits>
 
+#include "device_error.h"
 #include "fp8_common.cuh"
 #include "hb_kernels.h"
 #include "tc_common.cuh"
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
           }
         }
         for (; kb < kb1; ++kb) {
-          if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
+          if (!(ok = mbar_wait(&empty[s], ph, a.err, kErrFp8Stage))) break;
           weights(s, kb);
           rows(s, kb);
           if (++s == C::ST) { s = 0; ph ^= 1u; }
@@ -368,8 +369,8 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
         const uint32_t idesc = (1u << 4) | ((uint32_t)((rows + 15) >> 4) << 18) | ((128u >> 4) << 24);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t buf = it & 1u;
-          if (!(ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x200u))) break;
-          if (!(ok = mbar_wait(&full[s], ph, a.err, 0x400u))) break;
+          if (!(ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, kErrFp8AccFree))) break;
+          if (!(ok = mbar_wait(&full[s], ph, a.err, kErrFp8Loads))) break;
           tc_fence_after();
           const uint32_t sb = base + s * C::STAGE, d = tmem + buf * (2 * BN);
           const uint64_t ad = tc_desc_sw128(sb), bd = tc_desc_sw128(sb + 2 * F8_A_BYTES);
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
         }
       }
       tc_commit(mma_done);                                                     // nothing is in flight when tensor memory is freed
-      mbar_wait(mma_done, 0, a.err, 0x800u);
+      mbar_wait(mma_done, 0, a.err, kErrFp8Mma);
     }
   } else if (warp == F8_W_SCALE) {
     // ------------------------------------------------------------------------------------------------ scales of a step: weight block × row, a step ahead
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
 #pragma unroll
         for (int i = 0; i < NL; ++i) x[i] = nx[i];
         if (kb + 1 < kb1) fetch(kb + 1);
-        ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x2000u);
+        ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, a.err, kErrFp8ScaleFree);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         float* d = scl + (it & 3u) * (2 * BN);
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
       // added up (one at a time, each behind the other's additions: 730 clocks a step of 256 columns)
       uint32_t ra[C::CW], rb[C::CW];
       auto arrived = [&](uint32_t n) {
-        const bool o = mbar_wait(&acc_full[n & 1u], (n >> 1) & 1u, a.err, 0x1000u);
+        const bool o = mbar_wait(&acc_full[n & 1u], (n >> 1) & 1u, a.err, kErrFp8Acc);
         tc_fence_after();
         return (bool)__all_sync(0xffffffffu, o);
       };

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
             s = n == C::ST ? 0 : n; ph = n == C::ST ? 0 : 1;
           }
           for (; kb < kb1; ++kb) {
-            if (!(ok = mbar_wait(&empty[s], ph, a.err, 0x100u))) break;
+            if (!(ok = mbar_wait(&empty[s], ph, a.err, kErrFp8Stage))) break;
             weights(s, kb);
             rows(s, kb);
             if (++s == C::ST) { s = 0; ph ^= 1u; }
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         }
         // free stages are announced to both CTAs of a pair: the last announcements arrive before either ends
         for (int n = 0; ok && n < C::ST; ++n) {
-          ok = mbar_wait(&empty[s], ph, a.err, 0x100u);
+          ok = mbar_wait(&empty[s], ph, a.err, kErrFp8Stage);
           if (++s == C::ST) { s = 0; ph ^= 1u; }
         }
       }
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         while (ok && sch.next(item, kb0, kb1)) {
           for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t buf = it & 1u;
-            if (!(ok = mbar_wait(&full[s], ph, a.err, 0x400u))) break;
-            if (!(ok = mbar_wait(&acc_empty[h * 2 + buf], ((it >> 1) & 1u) ^ 1u, a.err, 0x200u))) break;
+            if (!(ok = mbar_wait(&full[s], ph, a.err, kErrFp8Loads))) break;
+            if (!(ok = mbar_wait(&acc_empty[h * 2 + buf], ((it >> 1) & 1u) ^ 1u, a.err, kErrFp8AccFree))) break;
             tc_fence_after();
             const uint64_t ad = ad0 + s * (uint32_t)(C::STAGE >> 4), bd = bd0 + s * (uint32_t)(C::STAGE >> 4);
 #pragma unroll
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
       for (int c = 0; c < 128; ++c) acc[c] = 0.f;
       uint32_t ra[32], rb[32];
       auto arrived = [&](uint32_t n) {
-        const bool o = mbar_wait(&acc_full[h * 2 + (n & 1u)], (n >> 1) & 1u, a.err, 0x1000u);
+        const bool o = mbar_wait(&acc_full[h * 2 + (n & 1u)], (n >> 1) & 1u, a.err, kErrFp8Acc);
         tc_fence_after();
         return (bool)__all_sync(0xffffffffu, o);
       };
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         // ---- an item split among the cluster's CTAs (this one's last): the sums take the operands' place in shared memory, CTA r goes on with everybody's
         // of its part of the rows, added up in the order of the CTAs
         if (kb1 - kb0 < KB) {
-          mbar_wait(mma_done, 0, a.err, 0x800u);                               // no MMA reads the operands any more
+          mbar_wait(mma_done, 0, a.err, kErrFp8Mma);                          // no MMA reads the operands any more
           float4* mine = reinterpret_cast<float4*>(sm) + h * 128 + row;        // [four columns][half][row]
           if (active) {
 #pragma unroll
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
   bool splits = false;
   if constexpr (!PAIR) splits = sch.splits();
   if (splits && warp >= 8) cluster_sync_all();                                 // the sums are in shared memory
-  if (warp == F8_W_TMA) mbar_wait(mma_done, 0, a.err, 0x800u);                 // in both CTAs: the last MMA has retired, and so has the announcement of it
+  if (warp == F8_W_TMA) mbar_wait(mma_done, 0, a.err, kErrFp8Mma);            // in both CTAs: the last MMA has retired, and so has the announcement of it
   tc_fence_before();
   __syncthreads();
   if (PAIR || splits) cluster_sync_all();                                      // nobody reads this CTA's shared memory any more

@@ -2,6 +2,7 @@
 // falls back to host arithmetic — if the device or a kernel is unusable the call fails with a message.
 #include <new>
 
+#include "device_error.h"
 #include "hb_common.cuh"
 #include "hb_kernels.h"
 
@@ -130,8 +131,9 @@ int hb_check_device(hb_ctx* ctx, void* stream) {
   HB_CUDA(ctx, cudaMemsetAsync(ctx->dev_err + kErrCounters, 0, kErrCounterWords * 4, as_stream(stream)));   // a product that gave up left its counts where they were
   if (v & 0x80000000u)
     return hb_fail(ctx, HB_ERR_DEVICE_FLAG, "device error word 0x%x: range check 0x%x failed with value %d (debug build)", v, site[0], (int)site[1]);
-  return hb_fail(ctx, HB_ERR_DEVICE_FLAG, "device error word 0x%x (bits 0x1-0x80: a pipeline wait inside a decode or prefill kernel; 0x400-0x2000: the decode layer kernel's tables and grid barrier; "
-                 "0x40000: rows of another rank did not arrive; 0x80000: partial sums of another rank did not arrive; 0x400000: an expert record that is not 16-byte aligned)", v);
+  char text[sizeof ctx->err];
+  hb_device_error_text(v, text, sizeof text);
+  return hb_fail(ctx, HB_ERR_DEVICE_FLAG, "%s", text);
 }
 
 int hb_rec_layout_make(int H, int I, hb_rec_layout* L) {

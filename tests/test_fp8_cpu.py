@@ -73,3 +73,30 @@ def test_route_definition():
     assert ids.tolist() == [[4, 7]] and abs(w.sum() - 1) < 1e-12
     ids, _ = R.route(lg, np.array([0, 0, 5, 0, 0, 0, 0, 0], np.float32), 2, 4, 1, 1, "sigmoid", False, 1.0)
     assert ids.tolist() == [[2, 3]]
+
+
+def test_a_wait_that_gave_up_names_its_kernel(tmp_path):
+    """The 8-bit products' waits share bits with other kernels': a bit of their own tells them apart, in every wait, and the message says so."""
+    import re
+    import subprocess
+    from pathlib import Path
+    csrc = Path(__file__).resolve().parent.parent / "eke_hive_b200" / "csrc"
+    (tmp_path / "text.cpp").write_text(r"""#include "device_error.h"
+#include <cstdlib>
+#include <initializer_list>
+int main(int argc, char** argv) {
+  for (uint32_t v : {kErrFp8Stage, kErrFp8AccFree, kErrFp8Loads, kErrFp8Mma, kErrFp8Acc, kErrFp8ScaleFree}) printf("%x\n", v);
+  for (int i = 1; i < argc; ++i) { char s[512]; hb_device_error_text(strtoul(argv[i], nullptr, 16), s, sizeof s); printf("%s\n", s); }
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-I", str(csrc), str(tmp_path / "text.cpp"), "-o", str(tmp_path / "text")], check=True)
+    out = subprocess.run([str(tmp_path / "text"), "800400", "400", "c00000", "40000"], capture_output=True, text=True, check=True).stdout.splitlines()
+    sites, text = [int(v, 16) for v in out[:6]], out[6:]
+    assert len(set(sites)) == 6 and all(v & 0x800000 and bin(v).count("1") == 2 for v in sites)
+    assert "0x800400" in text[0] and "8-bit product" in text[0] and "decode layer" not in text[0]
+    assert "decode layer" in text[1] and "8-bit" not in text[1]
+    assert "8-bit product" in text[2] and "not 16-byte aligned" in text[2]
+    assert "rows of another rank" in text[3] and all(len(t) < 511 for t in text)
+    for f in ("fp8_gemm.cuh", "fp8_pair.cuh"):
+        waits = re.findall(r"mbar_wait\([^;]*?a\.err, (\w+)\)", (csrc / f).read_text())
+        assert len(waits) >= 5 and all(w.startswith("kErrFp8") for w in waits), (f, waits)
