@@ -40,20 +40,31 @@ def _p(t):
     return int(t)
 
 
-def _stream(device: int | None = None):
-    # the stream's handle without the Python object around it: a third of what a call costs on the host
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
-
-
+# What torch's own generated code calls: the stream's handle without the Python object around it (a third of what a call costs on the host), and memory
+# without the dispatcher (a third of torch.empty's time).  A torch without these names goes the public way, and so does every allocation that
+# somebody wants to see or to have filled: under a dispatch mode and with deterministic algorithms.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
 try:
-    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_cuda     # what compiled graphs allocate with: a third of torch.empty's time
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_cuda
 except ImportError:
-    def _empty_cuda(size, stride, dtype):
+    _empty_cuda = None
+
+
+def _stream(device: int | None = None):
+    d = torch.cuda.current_device() if device is None else device
+    return _raw_stream(d) if _raw_stream else torch.cuda.current_stream(d).cuda_stream
+
+
+def _empty_strided(size, stride, dtype):
+    """Uninitialised memory on the current device."""
+    if _empty_cuda is None or _dispatch_modes is None or _dispatch_modes() or torch.are_deterministic_algorithms_enabled():
         return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+    return _empty_cuda(size, stride, dtype)
 
 
 def _empty(rows: int, cols: int, dtype):
-    return _empty_cuda((rows, cols), (cols, 1), dtype)                         # on the current device
+    return _empty_strided((rows, cols), (cols, 1), dtype)
 
 
 def _out(t, rows_: int, cols: int, dtype, rows: bool = False):
@@ -64,7 +75,7 @@ def _out(t, rows_: int, cols: int, dtype, rows: bool = False):
 
 
 def _bytes(n: int):
-    return _empty_cuda((n,), (1,), torch.uint8)
+    return _empty_strided((n,), (1,), torch.uint8)
 
 
 def _here(t: torch.Tensor, ctx: "Context | None"):
@@ -72,7 +83,7 @@ def _here(t: torch.Tensor, ctx: "Context | None"):
     d = torch.cuda.current_device()
     if t.get_device() != d or (ctx is not None and ctx.device != d):
         raise HbError(-1, f"tensor on {t.device}, context on cuda:{d if ctx is None else ctx.device}, current device cuda:{d}: they have to be the same")
-    return ctx or _CTX.get(d) or context(d), torch._C._cuda_getCurrentRawStream(d)
+    return ctx or _CTX.get(d) or context(d), _stream(d)
 
 
 def _row_ptr(t: torch.Tensor):
