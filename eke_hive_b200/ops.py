@@ -457,7 +457,8 @@ def lb_dequant(W: GMat, out=None, ctx: Context | None = None):
 def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     """hb_fp8_quant_rows: x bf16 [M, K] → (codes u8 [M, K], scales fp32 [ceil(K/128), M])."""
     ctx, st = _here(x, ctx)
-    assert x.dtype == torch.bfloat16
+    if x.dtype is not torch.bfloat16:
+        raise HbError(-1, f"rows of {x.dtype}: bf16 wanted")
     M, K = x.shape
     q = _empty(M, K, torch.uint8) if q is None else _out(q, M, K, torch.uint8, rows=True)
     s = _empty(-(-K // 128), M, torch.float32) if s is None else _out(s, -(-K // 128), M, torch.float32, rows=True)
@@ -469,7 +470,8 @@ def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     """hb_fp8_quantize: a weight fp32 or bf16 [N, K] → (codes u8 [N, K], scales fp32 [ceil(N/128), ceil(K/128)])."""
     ctx, st = _here(w, ctx)
     bf16 = w.dtype == torch.bfloat16
-    assert (bf16 or w.dtype == torch.float32) and w.is_contiguous()
+    if not (bf16 or w.dtype == torch.float32) or not w.is_contiguous():
+        raise HbError(-1, f"matrix of {w.dtype}, strides {w.stride()}: fp32 or bf16, contiguous, wanted")
     N, K = w.shape
     q = _empty(N, K, torch.uint8) if q is None else _out(q, N, K, torch.uint8)
     s = _empty(-(-N // 128), -(-K // 128), torch.float32) if s is None else _out(s, -(-N // 128), -(-K // 128), torch.float32)
@@ -520,7 +522,8 @@ def fp8_record(H: int, I: int, gate, up, down, out=None):
     L = Fp8RecLayout(H, I)
     out = torch.zeros(L.total, dtype=torch.uint8, device=gate[0].device) if out is None else out
     for (q, s), w0, s0, n in ((gate, L.w1, L.s1, (I, H)), (up, L.w3, L.s3, (I, H)), (down, L.w2, L.s2, (H, I))):
-        assert tuple(q.shape) == n and tuple(s.shape) == (n[0] // 128, n[1] // 128) and s.dtype == torch.float32
+        if tuple(q.shape) != n or q.element_size() != 1 or tuple(s.shape) != (n[0] // 128, n[1] // 128) or s.dtype is not torch.float32:
+            raise HbError(-1, f"codes {tuple(q.shape)} of {q.dtype}, scales {tuple(s.shape)} of {s.dtype}: {n} of one byte and {(n[0] // 128, n[1] // 128)} of fp32 wanted")
         out[w0:w0 + q.numel()] = q.contiguous().view(torch.uint8).view(-1)
         out[s0:s0 + 4 * s.numel()] = s.contiguous().view(-1).view(torch.uint8)
     return out
@@ -549,8 +552,8 @@ def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg
     op, cmb = out.data_ptr(), None
     if out.dtype == torch.bfloat16:
         cmb = C.byref(PfCombine(None if shared is None else shared.data_ptr(), _p(lg), 0 if lg is None else lg.stride(0), col, op))
-    else:
-        assert shared is None and lg is None, "shared rows are added to a bf16 output"
+    elif shared is not None or lg is not None:
+        raise HbError(-1, "shared rows are added to a bf16 output")
     ctx.check(L.hb_moe_fp8(ctx.handle, ids.data_ptr(), w.data_ptr(), M, K, rec_tab.data_ptr(), li, E, x.data_ptr(), H, I, limit, None if cmb else op, cmb,
                            ws.data_ptr(), st))
     return out
