@@ -83,15 +83,32 @@ def _here(t: torch.Tensor, ctx: "Context | None"):
     d = torch.cuda.current_device()
     if t.get_device() != d or (ctx is not None and ctx.device != d):
         raise HbError(-1, f"tensor on {t.device}, context on cuda:{d if ctx is None else ctx.device}, current device cuda:{d}: they have to be the same")
-    return ctx or _CTX.get(d) or context(d), _stream(d)
+    return ctx or _CTX.get(d) or context(d), _raw_stream(d) if _raw_stream else _stream(d)
+
+
+def _same(ctx: "Context", *tensors):
+    """All of them (None: not given; an address is the caller's own business) lie on the context's device: the kernels read their addresses."""
+    d = ctx.device
+    for t in tensors:
+        if t is not None and not isinstance(t, int) and t.get_device() != d:
+            raise HbError(-1, f"tensor on {t.device}, the call is on cuda:{ctx.device}")
+
+
+def _room(ws, n: int):
+    """The given workspace, which has to have n bytes in one piece; or new memory."""
+    if ws is None:
+        return _bytes(n)
+    if not ws.is_contiguous() or ws.numel() * ws.element_size() < n:
+        raise HbError(-5, f"workspace of {ws.numel() * ws.element_size()} bytes: {n} in one piece wanted")
+    return ws
 
 
 def _row_ptr(t: torch.Tensor):
     """(address, elements from row to row) of a matrix whose rows are contiguous."""
-    r, c = t.stride()
-    if c != 1 and t.shape[1] > 1:
+    (r, c), (n, cols) = t.stride(), t.shape
+    if c != 1 and cols > 1:
         raise HbError(-1, "rows must be contiguous")
-    return t.data_ptr(), max(r, t.shape[1]) if t.shape[0] <= 1 else r
+    return t.data_ptr(), max(r, cols) if n <= 1 else r
 
 
 class Context:
@@ -262,10 +279,15 @@ def router_grouped_topk(logits: torch.Tensor, k: int, n_group: int = 1, topk_gro
     E = cols if E is None else E
     if logits.dtype is not torch.float32 or E > cols or (bias is not None and (bias.dtype is not torch.float32 or bias.numel() < E or not bias.is_contiguous())):
         raise HbError(-1, "logits and bias have to be fp32, the bias contiguous, with a value for every expert")
+    kind = _SCORE.get(score)
+    if kind is None:
+        raise HbError(-1, f"score {score!r}: one of {tuple(_SCORE)} wanted")
+    if bias is not None or ids is not None or w is not None:
+        _same(ctx, bias, ids, w)
     ids = _empty(M, k, torch.int32) if ids is None else _out(ids, M, k, torch.int32)
     w = _empty(M, k, torch.float32) if w is None else _out(w, M, k, torch.float32)
     lp, ld = _row_ptr(logits)
-    ctx.check(_L().hb_route_grouped_topk(ctx.handle, lp, ld, M, E, k, n_group, topk_group, group_top, _SCORE[score],
+    ctx.check(_L().hb_route_grouped_topk(ctx.handle, lp, ld, M, E, k, n_group, topk_group, group_top, kind,
                                          None if bias is None else bias.data_ptr(), renorm, scale, ids.data_ptr(), w.data_ptr(), st))
     return ids, w
 
@@ -417,6 +439,9 @@ class GMat:
 
     def __init__(self, fmt: int, N: int, K: int, w, s, zp=None, g: float = 1.0):
         from ._lib import QMat
+        if fmt == FMT_FP8_B128 and isinstance(w, torch.Tensor) and isinstance(s, torch.Tensor) and (w.element_size() != 1 or w.numel() < N * K or s.dtype is not torch.float32 or s.numel() < -(-N // 128) * -(-K // 128)
+                                    or not (w.is_contiguous() and s.is_contiguous())):
+            raise HbError(-1, f"codes {tuple(w.shape)}, scales {tuple(s.shape)} of {s.dtype}: {(N, K)} of one byte and {(-(-N // 128), -(-K // 128))} of fp32, contiguous, wanted")
         self.fmt, self.N, self.K, self.w, self.s, self.zp, self.g = fmt, N, K, w, s, zp, g
         self.c = QMat(fmt, N, K, _p(w), _p(s), _p(zp), g)
 
@@ -460,9 +485,16 @@ def fp8_quant_rows(x: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     if x.dtype is not torch.bfloat16:
         raise HbError(-1, f"rows of {x.dtype}: bf16 wanted")
     M, K = x.shape
-    q = _empty(M, K, torch.uint8) if q is None else _out(q, M, K, torch.uint8, rows=True)
-    s = _empty(-(-K // 128), M, torch.float32) if s is None else _out(s, -(-K // 128), M, torch.float32, rows=True)
-    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, *_row_ptr(x), M, K, *_row_ptr(q), *_row_ptr(s), st))
+    qp, sp = (), ()
+    if q is not None or s is not None:
+        _same(ctx, q, s)
+        qp = () if q is None else _row_ptr(_out(q, M, K, torch.uint8, rows=True))
+        sp = () if s is None else _row_ptr(_out(s, -(-K // 128), M, torch.float32, rows=True))
+    if q is None:
+        q = _empty(M, K, torch.uint8)
+    if s is None:
+        s = _empty(-(-K // 128), M, torch.float32)
+    ctx.check(_L().hb_fp8_quant_rows(ctx.handle, *_row_ptr(x), M, K, *(qp or (q.data_ptr(), K)), *(sp or (s.data_ptr(), M)), st))
     return q, s
 
 
@@ -472,6 +504,7 @@ def fp8_quantize(w: torch.Tensor, q=None, s=None, ctx: Context | None = None):
     bf16 = w.dtype == torch.bfloat16
     if not (bf16 or w.dtype == torch.float32) or not w.is_contiguous():
         raise HbError(-1, f"matrix of {w.dtype}, strides {w.stride()}: fp32 or bf16, contiguous, wanted")
+    _same(ctx, q, s)
     N, K = w.shape
     q = _empty(N, K, torch.uint8) if q is None else _out(q, N, K, torch.uint8)
     s = _empty(-(-N // 128), -(-K // 128), torch.float32) if s is None else _out(s, -(-N // 128), -(-K // 128), torch.float32)
@@ -490,15 +523,19 @@ def fp8_gemm(W: GMat, xq, xs, out_dtype=torch.bfloat16, y=None, ws=None, ctx: Co
     """hb_fp8_gemm: y [M, N] (bf16 or fp32) = rows quantised by fp8_quant_rows times the block-scaled matrix W (FMT_FP8_B128)."""
     ctx, st = _here(xq, ctx)
     L = _L()
-    M = xq.shape[0]
+    (M, cols), (blocks, scales), N, K = xq.shape, xs.shape, W.N, W.K
     if y is not None:
         out_dtype = y.dtype
-    if out_dtype not in _FP8_OUT or xq.element_size() != 1 or xs.dtype is not torch.float32 or xq.shape[1] < W.K or xs.shape[0] * 128 < W.K:
+    if out_dtype not in _FP8_OUT or xq.element_size() != 1 or xs.dtype is not torch.float32 or cols < K or blocks * 128 < K or scales < M:
         raise HbError(-1, "codes [M, K] of one byte, scales fp32 [ceil(K/128), M], result bf16 or fp32")
-    y = _empty(M, W.N, out_dtype) if y is None else _out(y, M, W.N, out_dtype, rows=True)
-    ws = _bytes(L.hb_fp8_gemm_ws_bytes(M, W.N, W.K)) if ws is None else ws
-    yp, ldy = _row_ptr(y)
-    yb, yf = (yp, None) if y.dtype == torch.bfloat16 else (None, yp)
+    _same(ctx, xs, W.w, W.s, y, ws)
+    if y is None:
+        y = _empty(M, N, out_dtype)
+        yp, ldy = y.data_ptr(), N
+    else:
+        yp, ldy = _row_ptr(_out(y, M, N, out_dtype, rows=True))
+    ws = _room(ws, L.hb_fp8_gemm_ws_bytes(M, N, K))
+    yb, yf = (yp, None) if out_dtype is torch.bfloat16 else (None, yp)
     ctx.check(L.hb_fp8_gemm(ctx.handle, C.byref(W.c), *_row_ptr(xq), *_row_ptr(xs), M, yb, yf, ldy, ws.data_ptr(), st))
     return y
 
@@ -543,12 +580,16 @@ def moe_fp8(ids, w, rec_tab, li: int, E: int, x, H: int, I: int, shared=None, lg
     if out is not None:
         out_dtype = out.dtype
     if (out_dtype not in _FP8_OUT or ids.dtype is not torch.int32 or w.dtype is not torch.float32 or x.dtype is not torch.bfloat16 or rec_tab.dtype is not torch.int64
-            or w.shape != ids.shape or x.shape != (M, H) or rec_tab.numel() < (li + 1) * E or not (x.is_contiguous() and ids.is_contiguous() and w.is_contiguous())
+            or w.shape != ids.shape or x.shape != (M, H) or rec_tab.numel() < (li + 1) * E
+            or not (x.is_contiguous() and ids.is_contiguous() and w.is_contiguous() and rec_tab.is_contiguous())
             or (shared is not None and (shared.dtype is not torch.bfloat16 or shared.shape != (M, H) or not shared.is_contiguous()))
-            or (lg is not None and (lg.dtype is not torch.float32 or lg.shape[0] != M))):
-        raise HbError(-1, "ids int32 and w fp32 [M, K], x and shared bf16 [M, H], lg fp32 [M, ·], rec_tab int64 with li + 1 layers, all contiguous, result bf16 or fp32")
+            or (lg is not None and (lg.dtype is not torch.float32 or lg.shape[0] != M or not 0 <= col < (lg.shape[1] if lg.dim() == 2 else 1)
+                                    or (lg.dim() == 2 and lg.stride(1) != 1 and lg.shape[1] > 1)))):
+        raise HbError(-1, "ids int32 and w fp32 [M, K], x and shared bf16 [M, H], lg fp32 [M, more than col] of contiguous rows, rec_tab int64 with li + 1 layers, all else contiguous, "
+                          "result bf16 or fp32")
+    _same(ctx, ids, w, rec_tab, shared, lg, out, ws)
     out = _empty(M, H, out_dtype) if out is None else _out(out, M, H, out_dtype)
-    ws = _bytes(L.hb_moe_fp8_ws_bytes(M, K, E, H, I)) if ws is None else ws
+    ws = _room(ws, L.hb_moe_fp8_ws_bytes(M, K, E, H, I))
     op, cmb = out.data_ptr(), None
     if out.dtype == torch.bfloat16:
         cmb = C.byref(PfCombine(None if shared is None else shared.data_ptr(), _p(lg), 0 if lg is None else lg.stride(0), col, op))

@@ -102,3 +102,40 @@ def test_wrong_types_are_errors_of_the_library(host):
     with pytest.raises(Seen):
         ops.moe_fp8(ids, w, tab, 0, 3, bf, 256, 128, shared=bf)
     refused(lambda: ops.moe_fp8(ids, w, tab, 0, 3, bf, 256, 128, shared=bf, out_dtype=torch.float32))
+
+
+def test_calls_that_would_be_read_out_of_range_are_refused(host):
+    """Tensors that hold less than the call says, lie in other strides than it can say, or on another device."""
+    class Elsewhere(torch.Tensor):
+        get_device = lambda self: 1
+    away = lambda t: t.clone().as_subclass(Elsewhere)
+    N, K, M = 200, 256, 40
+    q, s = torch.zeros(N, K, dtype=torch.uint8), torch.ones(2, 2)
+    W = ops.GMat(ops.FMT_FP8_B128, N, K, q, s)
+    xq, xs = torch.zeros(M, K, dtype=torch.uint8), torch.ones(2, M)
+    ws, y = torch.zeros(4096, dtype=torch.uint8), torch.zeros(M, N)
+    ok = [lambda: ops.fp8_gemm(W, xq, xs, y=y, ws=ws), lambda: ops.fp8_gemm(W, xq, torch.ones(2, M + 3)[:, :M]), lambda: ops.fp8_gemm(W, xq[:1], torch.ones(2, M))]
+    refused(*(lambda a=a: ops.GMat(ops.FMT_FP8_B128, N, K, *a) for a in ((q[:199], s), (q, s[:1]), (q, s.double()), (q.short(), s), (q.t().contiguous().t(), s), (q, s.t().contiguous().t()))),
+            lambda: ops.fp8_gemm(W, xq, torch.ones(2, M + 3)[:, :M - 1]), lambda: ops.fp8_gemm(W, xq, torch.ones(1, M - 1)), lambda: ops.fp8_gemm(W, xq, xs, ws=ws[:4095]),
+            lambda: ops.fp8_gemm(W, xq, xs, ws=torch.zeros(8192, dtype=torch.uint8)[::2]), lambda: ops.fp8_gemm(W, xq, away(xs)), lambda: ops.fp8_gemm(W, xq, xs, y=away(y)),
+            lambda: ops.fp8_gemm(W, xq, xs, ws=away(ws)), lambda: ops.fp8_gemm(ops.GMat(ops.FMT_FP8_B128, N, K, away(q), s), xq, xs),
+            lambda: ops.fp8_gemm(ops.GMat(ops.FMT_FP8_B128, N, K, q, away(s)), xq, xs), lambda: ops.fp8_gemm(W, away(xq), xs))
+    bf = torch.zeros(M, K, dtype=torch.bfloat16)
+    ok += [lambda: ops.fp8_quant_rows(bf, q=xq, s=xs), lambda: ops.fp8_quantize(bf)]
+    refused(lambda: ops.fp8_quant_rows(bf, q=away(xq)), lambda: ops.fp8_quant_rows(bf, s=away(xs)), lambda: ops.fp8_quantize(bf, q=away(xq)), lambda: ops.fp8_quantize(bf, s=away(torch.ones(1, 2))))
+    lgt, bias = torch.zeros(M, 64), torch.zeros(64)
+    i, w = torch.zeros(M, 2, dtype=torch.int32), torch.zeros(M, 2)
+    ok += [lambda: ops.router_grouped_topk(lgt, 2, bias=bias, ids=i, w=w)]
+    refused(lambda: ops.router_grouped_topk(lgt, 2, bias=away(bias)), lambda: ops.router_grouped_topk(lgt, 2, ids=away(i)), lambda: ops.router_grouped_topk(lgt, 2, w=away(w)),
+            lambda: ops.router_grouped_topk(lgt, 2, score="tanh"))
+    tab = torch.zeros(6, dtype=torch.int64)
+    out = torch.zeros(M, K, dtype=torch.bfloat16)
+    moe = lambda **k: ops.moe_fp8(**{**dict(ids=i, w=w, rec_tab=tab, li=1, E=3, x=bf, H=K, I=128, shared=bf), **k})
+    ok += [moe, lambda: moe(lg=torch.zeros(M)), lambda: moe(lg=torch.zeros(M, 5), col=4), lambda: moe(lg=torch.zeros(M, 9)[:, 2:5], col=2), lambda: moe(lg=torch.zeros(M, 5)[:, 1]),
+           lambda: moe(ws=ws, out=out), lambda: moe(lg=torch.zeros(M, 5)[:, 1:2])]
+    refused(lambda: moe(lg=torch.zeros(5, M).t(), col=2), lambda: moe(lg=torch.zeros(M, 10)[:, ::2], col=1), lambda: moe(lg=torch.zeros(M, 9)[:, :3], col=3), lambda: moe(lg=torch.zeros(M), col=1),
+            lambda: moe(rec_tab=torch.zeros(12, dtype=torch.int64)[::2]), lambda: moe(ws=ws[1:]), *(lambda k=k, v=v: moe(**{k: away(v)}) for k, v in
+            dict(ids=i, w=w, rec_tab=tab, shared=bf, lg=torch.zeros(M), out=out, ws=ws, x=bf).items()))
+    for c in ok:
+        with pytest.raises(Seen):
+            c()
