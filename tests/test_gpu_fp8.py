@@ -495,6 +495,53 @@ def test_gemm_rows_of_the_result_beyond_31_bits_of_bytes(E, N, dt):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_moe_offsets_beyond_32_bits(E, dt):
+    """Pairs' results more than 2^32 bytes from their first: the rows at the end are those of the formula."""
+    import torch
+    M, H, I, Ex, K = 70000, 8192, 128, 4, 4
+    recs = [record(E, H, I, 10 * e) for e in range(Ex)]
+    tab = E.rec_table([r[0] for r in recs])
+    ids = torch.arange(M * K, device="cuda", dtype=torch.int32).view(M, K) % Ex
+    w = torch.rand(M, K, device="cuda", generator=gen(1)) * 0.5
+    x = torch.randn(M, H, device="cuda", generator=gen(2)).to(torch.bfloat16)
+    assert M * K * H * 2 > 1 << 32
+    out = E.moe_fp8(ids, w, tab, 0, Ex, x, H, I, out_dtype=getattr(torch, dt))
+    for at in (0, M - 40):
+        sl = slice(at, at + 40)
+        o0, tol, _ = R.moe(ids[sl], w[sl], [r[1] for r in recs], x[sl])
+        tol = tol + (R.HALF[out.dtype] * (o0.abs() + tol) if dt == "bfloat16" else 0.0)
+        assert ((out[sl].double() - o0).abs() <= tol + 1e-30).all()
+    del out, x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M,Ex,K", [(400, 16, 4), (700, 100, 3), (300, 4, 2)])
+def test_moe_long_lists_in_graphs_and_without_dependent_launches(E, M, Ex, K):
+    """Lists of pairs that a kernel of their own puts in order, replayed with other inputs; and every kernel behind the one in front."""
+    import torch
+    H, I = 640, 256
+    recs = [record(E, H, I, 10 * e)[0] for e in range(4)]
+    tab = torch.tensor([recs[e % 4].data_ptr() for e in range(Ex)], dtype=torch.int64, device="cuda")
+    ins = [(*routing(M, K, Ex, i), torch.randn(M, H, device="cuda", generator=gen(i)).to(torch.bfloat16)) for i in range(3)]
+    call = lambda a, dt, ctx=None: E.moe_fp8(a[0], a[1], tab, 0, Ex, a[2], H, I, out_dtype=dt, ctx=ctx)
+    for dt in (torch.float32, torch.bfloat16):
+        ref = [call(a, dt) for a in ins]
+        plain = E.Context(flags=E.HB_FLAG_NO_PDL)
+        assert all(torch.equal(call(a, dt, plain), r) for a, r in zip(ins, ref))
+        plain.check_device()
+        buf = [t.clone() for t in ins[0]]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = call(buf, dt)
+        for i in (1, 2, 0, 1):
+            for b, t in zip(buf, ins[i]):
+                b.copy_(t)
+            g.replay()
+            assert torch.equal(got, ref[i])
+    E.context().check_device()
+
+
 def test_moe_limit_and_gateless_shared(E):
     moe_check(E, 9, 512, 256, 6, 3, 1, limit=1.5, gate=False)
     moe_check(E, 200, 256, 128, 6, 3, 2, limit=0.7, shared=False)
