@@ -27,7 +27,7 @@
 
 namespace hb {
 
-enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2 };
+enum { F8_PLAIN = 0, F8_GU = 1, F8_DOWN = 2, F8_DOWN32 = 3 };   // the down pass of a bf16 and of an fp32 result
 
 constexpr int F8_COUNTERS = F8_MAX_CTAS;               // items that are cut, at most: a CTA's last one
 constexpr int F8_THREADS = 12 * 32, F8_W_TMA = 8, F8_W_MMA = 9, F8_W_SCALE = 10;
@@ -141,15 +141,15 @@ struct F8Cfg {
 };
 
 struct F8Args {
-  const TileRef* tiles; const int* n_tiles;            // GU / DOWN: tiles of slots; PLAIN: ceil(M / per) tiles of `per` rows
+  const TileRef* tiles; const int* n_tiles;            // GU / DOWN / DOWN32: tiles of slots; PLAIN: ceil(M / per) tiles of `per` rows
   F8Plan plan;                                         // GU with plan.P > 0: the tiles are worked out here
   int M, per, N, K, n_nt;                              // n_nt: items a tile has (GU: N / 128 with N = I, else ceil(N / 256))
   int split;                                           // fp8_pair.cuh, tiles of single CTAs: CTAs of a cluster, 1, 2 or 4
   const float* ws; const uint8_t* const* tab; uint64_t off_w, off_s0, off_s1; int row2;   // PLAIN: scales; else records, offsets of the codes and of the two tiles' scales, rows from the first tile's matrix to the second's (GU)
-  uint8_t* maps;                                       // GU / DOWN: room for F8_MAPS tensor maps a CTA
+  uint8_t* maps;                                       // GU / DOWN / DOWN32: room for F8_MAPS tensor maps a CTA
   const float* xs; int lds;                            // scales of the rows
   float limit;
-  __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN / DOWN: one of them
+  __nv_bfloat16* yb; float* yf; int ldy;               // PLAIN: one of them; DOWN: yb; DOWN32: yf
   uint8_t* yq; float* ys; int ldys;                    // GU: codes [slot, I], scales [I / 128][ldys]
   float* part; unsigned int* count;                    // sums of cut items [CTA][2][BN][256]; arrivals, by the CTA of an item's first step (zero before and after)
   uint32_t room;                                       // of part, in sums: range checks of the debug build
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(BN <= 16 ? 512 : F8_THREADS, 1) fp8_gemm_kerne
             }
           }
         };
-        if (a.yb) store(a.yb, [](float v) { return __float2bfloat16(v); });
+        if (MODE == F8_DOWN || (MODE == F8_PLAIN && a.yb)) store(a.yb, [](float v) { return __float2bfloat16(v); });
         else store(a.yf, [](float v) { return v; });
       }
     }

@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) fp8_many_kernel(const __grid_co
         uint8_t* stg = sm + C::ST * C::STAGE + (size_t)warp * F8_STG_BYTES;
         const int nrow = min(32, rows - 32 * q), n0 = nt * 256 + h * 128;
         const size_t row0 = slot0 + 32 * q;
-        if (a.yb) {
+        if (MODE == F8_DOWN || (MODE == F8_PLAIN && a.yb)) {
 #pragma unroll
           for (int c = 0; c < 128; c += 32) {
 #pragma unroll

@@ -301,7 +301,7 @@ int f8_rows(hb_ctx* ctx, const F8RowsArgs& a, cudaStream_t st) {
 
 int hbk_fp8_setup(hb_ctx* ctx) {
   for (int bn : {16, 32, F8S_ROWS, F8P_ROWS})
-    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn)}) {   // (256: the dense product alone)
+    for (const F8Pick& k : {f8_kernel<F8_PLAIN>(bn), f8_kernel<F8_GU>(bn), f8_kernel<F8_DOWN>(bn), f8_kernel<F8_DOWN32>(bn)}) {   // (256: the dense product alone)
       cudaFuncAttributes at;
       HB_CUDA(ctx, cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(k.fn)));
       // a warp that asks for more registers than the block was launched with would wait for good
@@ -433,7 +433,7 @@ int hb_moe_fp8(hb_ctx* ctx, const int32_t* ids, const float* w, int M, int K, co
   a.N = H; a.K = I; a.n_nt = (H + 255) / 256; a.off_w = L.w2; a.off_s0 = a.off_s1 = L.s2; a.maps = W.maps + (size_t)F8_MAX_CTAS * F8_MAPS * sizeof(CUtensorMap);
   a.xs = W.ys; a.ldy = H;
   if (cmb) a.yb = reinterpret_cast<__nv_bfloat16*>(W.part); else a.yf = reinterpret_cast<float*>(W.part);
-  if ((r = f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, td, ty, st))) return r;
+  if ((r = cmb ? f8_launch<F8_DOWN>(ctx, "fp8_gemm_down", rows, a, td, ty, st) : f8_launch<F8_DOWN32>(ctx, "fp8_gemm_down", rows, a, td, ty, st))) return r;
   auto sum = [&](auto su) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(su.part)>>;
     const long long sums = ((long long)M * ((H + F8_SUM_COLS<T> - 1) / F8_SUM_COLS<T>) + F8_SUM_THREADS / 32 - 1) / (F8_SUM_THREADS / 32), cap = (long long)ctx->sm_count * 16;
