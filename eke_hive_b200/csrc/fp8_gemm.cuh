@@ -13,7 +13,8 @@
 // ends.  A CTA that holds part of an item leaves its sums in the workspace; the last
 // one to arrive (a counter an item) adds all parts in the order of the CTAs — the same order in every run — and finishes the item.  So a product
 // with one row of x keeps all SMs streaming weights to the end.  Nobody waits for anybody.  What bounds it: HBM (one row of 139264 x 5120: 112 us, 6.35 TB/s; 32
-// rows 123) behind some 7 us of start, join and end (17408 x 5120: 20 us).//
+// rows 123) behind some 7 us of start, join and end (17408 x 5120: 20 us).
+//
 // Per CTA (persistent, one per SM, 12 warps): warp 8 (one thread) loads the operand tiles by TMA under the 128-byte swizzle, warp 9 (one thread) issues the
 // MMAs, warp 10 multiplies the step's scales, warps 0-7 read the sums back (a warp reaches the 32 lanes of its number mod 4; warps 0-3 take the first half
 // of the columns, 4-7 the second) and end the items.  Two accumulator buffers: one fills while the other is read.  Every wait is bounded.
