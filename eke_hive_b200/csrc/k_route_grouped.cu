@@ -295,18 +295,20 @@ __device__ __forceinline__ bool route_grouped_row32(const RouteGroupedArgs& a, c
     // A tie at the border settles nothing about those behind it: the last pick has to stand clear of the best one left out that is not its equal
     const uint32_t kk = __shfl_sync(0xffffffffu, mykey, a.k - 1);
     const float lk = __shfl_sync(0xffffffffu, l, a.k - 1), bk = __shfl_sync(0xffffffffu, b, a.k - 1);
-    uint32_t rest = lane >= a.k && mykey && !(l == lk && b == bk) ? mykey : 0u;
+    uint32_t rest = __reduce_max_sync(0xffffffffu, lane >= a.k && mykey && !(l == lk && b == bk) ? mykey : 0u);
+    if (rest == 0u) {                                                            // (what is listed comes before all that is not)
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      uint32_t x = rounds || key[j] < bound ? key[j] : 0u;                       // neither picked nor listed
-      if (x == kk) {
-        const int e = lane + 32 * j;
-        const float xl = fmaxf(__ldg(lr + e), -INFINITY);
-        if (xl == lk && rg_bias(a, e) == bk) x = 0u;
+      for (int j = 0; j < R; ++j) {
+        uint32_t x = rounds || key[j] < bound ? key[j] : 0u;                     // neither picked nor listed
+        if (x == kk) {
+          const int e = lane + 32 * j;
+          const float xl = fmaxf(__ldg(lr + e), -INFINITY);
+          if (xl == lk && rg_bias(a, e) == bk) x = 0u;
+        }
+        rest = max(rest, x);
       }
-      rest = max(rest, x);
+      rest = __reduce_max_sync(0xffffffffu, rest);
     }
-    rest = __reduce_max_sync(0xffffffffu, rest);
     const float vk = rg_val(kk), vr = rg_val(rest);
     close = close || (rest != 0u && !(vk - vr > err(vk) + err(vr)));
   }
