@@ -558,6 +558,8 @@ def fp8_record(H: int, I: int, gate, up, down, out=None):
     """One expert's record (u8 tensor of Fp8RecLayout(H, I).total bytes) from its (codes, scales) pairs as fp8_quantize gives them."""
     L = Fp8RecLayout(H, I)
     out = torch.zeros(L.total, dtype=torch.uint8, device=gate[0].device) if out is None else out
+    if out.dtype is not torch.uint8 or out.dim() != 1 or out.numel() < L.total or not out.is_contiguous():
+        raise HbError(-1, f"record {tuple(out.shape)} of {out.dtype}: {L.total} bytes in one piece wanted")
     for (q, s), w0, s0, n in ((gate, L.w1, L.s1, (I, H)), (up, L.w3, L.s3, (I, H)), (down, L.w2, L.s2, (H, I))):
         if tuple(q.shape) != n or q.element_size() != 1 or tuple(s.shape) != (n[0] // 128, n[1] // 128) or s.dtype is not torch.float32:
             raise HbError(-1, f"codes {tuple(q.shape)} of {q.dtype}, scales {tuple(s.shape)} of {s.dtype}: {n} of one byte and {(n[0] // 128, n[1] // 128)} of fp32 wanted")

@@ -139,3 +139,12 @@ def test_calls_that_would_be_read_out_of_range_are_refused(host):
     for c in ok:
         with pytest.raises(Seen):
             c()
+
+
+def test_a_record_is_bytes_in_one_piece(host):
+    u8, s = torch.zeros(256, 256, dtype=torch.uint8), torch.ones(2, 2)
+    n = ops.Fp8RecLayout(256, 256).total
+    make = lambda out: ops.fp8_record(256, 256, (u8, s), (u8, s), (u8, s), out=out)
+    room = torch.full((n + 32,), 7, dtype=torch.uint8)
+    assert make(room[16:]).data_ptr() == room.data_ptr() + 16 and (room[:16] == 7).all() and (room[n + 16:] == 7).all()
+    refused(lambda: make(torch.zeros(n - 1, dtype=torch.uint8)), lambda: make(torch.zeros(n)), lambda: make(torch.zeros(2 * n, dtype=torch.uint8)[::2]), lambda: make(torch.zeros(1, n, dtype=torch.uint8)))
